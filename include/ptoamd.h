@@ -6,7 +6,7 @@
  * void* (NULL = the default stream).  Every function returns 0 on success and a negative PTOAMD_E_* code on
  * failure; ptoamd_last_error() gives the text.  Launches are asynchronous on `stream`.
  *
- * Two groups of entry points:
+ * Three groups of entry points:
  *   1. the host runtime the reference's tests and demos reach through `aclrt*`
  *      (reference: include/pto/common/cpu_stub.hpp:73-120, 524-555);
  *   2. whole-kernel launchers, the counterpart of the reference's per-kernel
@@ -14,7 +14,8 @@
  *      (reference: tests/cpu/st/testcase/tmatmul/tmatmul_kernel.cpp:175-203,
  *       kernels/manual/a5/matmul_mxfp8_performance/mxmatmul_performance_kernel.cpp:360-380),
  *      each of which runs one TLOAD -> TMATMUL/TMATMUL_ACC -> TSTORE pipeline (or one TQUANT / TDEQUANT pass)
- *      over whole matrices in HBM.
+ *      over whole matrices in HBM;
+ *   3. what stands between the products of a decoder layer: rotary positions, a cache of keys and values in 8 bits, attention over it.
  */
 #ifndef PTOAMD_H
 #define PTOAMD_H
@@ -338,6 +339,107 @@ int ptoamd_mx_scale_relayout(uint8_t* dst, int dst_layout, const uint8_t* src, i
 /* Names the kernel the last ptoamd_gemm* / ptoamd_gemv* call on this thread dispatched to ("tile256x256_bf16", ...,
  * "generic"): lets tests assert that the MFMA path, not the order-exact generic kernel, produced a result. */
 const char* ptoamd_last_kernel(void);
+
+/* =========================================================================================================
+ * 3. Between the QKV product and the output product of a decoder layer: rotary positions, a cache of keys and
+ *    values held in 8 bits, attention over it.  No counterpart among the reference's tile instructions for this
+ *    path (its attention demos work on whole 16-bit matrices, demos/cpu/flash_attention_demo); names, error
+ *    codes, streams and ownership are those of the groups above.
+ * ========================================================================================================= */
+
+/*
+ * The rotations of positions 0 .. rows - 1: table[p][i] = magnitude * cos(p F_i), table[p][rot_dim / 2 + i] = magnitude * sin(p F_i)
+ * for i < rot_dim / 2, computed in 64 bits and rounded once, with
+ *   f_i = base^(-2 i / rot_dim),  t_i = clamp((i - ramp_low) / (ramp_high - ramp_low), 0, 1),  F_i = f_i (1 - t_i) + f_i t_i / factor
+ * factor 1: plain; ramp_low = ramp_high = 0: every frequency divided (t_i = 1: linear interpolation of positions); a ramp between two
+ * pairs: fast pairs kept, slow ones divided, which with a magnitude is how long contexts are reached without losing near ones.
+ */
+int ptoamd_rope_table(float* table, int rows, int rot_dim, double base, double factor, double ramp_low, double ramp_high, double magnitude,
+                      void* stream);
+
+/*
+ * Rotary positions: the first rot_dim elements of every head of x [tokens][heads][head_dim] in rot_dim / 2 pairs, each turned by its
+ * token's angle; the others are copied.  With c = table[position][i], s = table[position][rot_dim / 2 + i]:
+ *   a' = a c - b s,  b' = a s + b c;  backward != 0: the gradient of x from that of the result, a' = a c + b s, b' = b c - a s
+ *   interleaved : 0: pair i is elements i and i + rot_dim / 2;  1: elements 2 i and 2 i + 1
+ *   type        : PTOAMD_F32 | PTOAMD_F16 | PTOAMD_BF16; products and sums in f32, rounded once
+ *   strides     : of tokens and heads, in elements; elements of a head lie together.  out may be x (with x's strides), but overlap it in no
+ *                 other way.  So Q and K of a fused product are turned in one call, in place or not.
+ *   positions   : [tokens] int32.  A token whose position is not in 0 .. table_rows - 1 gets NaN for its rot_dim elements.
+ */
+int ptoamd_rope(void* out, const void* x, int type, const float* table, int table_rows, const int32_t* positions, int tokens, int heads,
+                int head_dim, int rot_dim, int64_t x_token_stride, int64_t x_head_stride, int64_t out_token_stride, int64_t out_head_stride,
+                int interleaved, int backward, void* stream);
+
+/*
+ * A cache of keys and values in pages.  A page holds page_size consecutive tokens of one sequence, for every key head; each page and
+ * head has one scale for its keys and one for its values: value = code * scale.
+ *   code_type     : PTOAMD_I8 | PTOAMD_E4M3
+ *   k, v          : element (page, head, token, i) at page * page_stride + head * head_stride + token * token_stride + i bytes; so both
+ *                   [pages][heads][page_size][head_dim] and [pages][page_size][heads][head_dim] are described.
+ *   k_scale, v_scale : [pages][kv_heads] f32, not negative.  A scale that is NaN makes what is read through it NaN.
+ *   block_table   : [sequences][max_pages] int32, the pages of each sequence in order.  Entries behind a sequence's last page are not
+ *                   read.  An entry that is no page of the cache (outside 0 .. pages - 1) takes nothing from an append, and a query that
+ *                   sees it gets NaN.
+ *   lengths       : [sequences] int32, tokens of each sequence with the new ones (those of this step, whose keys are appended and
+ *                   whose queries look back).  Taken as at least 0 and at most max_pages * page_size.
+ *   page_size     : 16, 32, 64, 128 or 256
+ */
+typedef struct ptoamd_kv8_cache {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    const int32_t* block_table;
+    const int32_t* lengths;
+    int code_type;
+    int pages;
+    int kv_heads;
+    int page_size;
+    int head_dim;
+    int sequences;
+    int max_pages;
+    int64_t k_page_stride, k_head_stride, k_token_stride;
+    int64_t v_page_stride, v_head_stride, v_token_stride;
+} ptoamd_kv8_cache;
+
+/*
+ * Appends new tokens' keys and values, k and v [tokens][kv_heads][head_dim] of `type` (PTOAMD_F32 | F16 | BF16).
+ *   cu_tokens  : [sequences + 1] int32: rows cu_tokens[s] .. cu_tokens[s + 1] - 1 of k and v are sequence s's; they become its tokens
+ *                lengths[s] - n .. lengths[s] - 1.  NULL: every sequence has max_tokens of them (tokens = sequences * max_tokens).
+ *   max_tokens : at least every sequence's n
+ * For each page that gets tokens, each head, K and V:  a = max |x| of the new ones;  s1 = max(s0, a / Q), s0 being the page's scale if
+ * it holds older tokens of the sequence and else 0, Q = 127 (int8) or 448 (E4M3);  where s1 > s0 the older codes become
+ * round(code * (s0 / s1));  new codes are round(x * (1 / s1)), ties to even, clamped.  The scale grows and never shrinks while a page
+ * fills, and an append repeated changes nothing.  A scale below 2^-126 is taken as 0, its codes as 0.  If a new value is infinite or NaN,
+ * the scale of its page and head is NaN from then on (and the new codes are 0): what sees it gets NaN instead of a wrong number.
+ * Pages that are written must not be shared between sequences.  Tokens that have no place (lengths[s] < n, or beyond max_pages) are left out.
+ */
+int ptoamd_kvcache_append(const ptoamd_kv8_cache* cache, const void* k, const void* v, int type, int tokens, const int32_t* cu_tokens,
+                          int max_tokens, int64_t k_token_stride, int64_t k_head_stride, int64_t v_token_stride, int64_t v_head_stride,
+                          void* stream);
+
+/*
+ * Attention of q [tokens][heads][head_dim] (PTOAMD_F16 | PTOAMD_BF16) over the cache; out has q's type.
+ * Query i of the n of a sequence of length L (cu_tokens and max_tokens as above) stands at place p = L - n + i and sees key j where
+ * 0 <= j < L, j <= p (causal != 0) and j > p - window (window > 0):
+ *   s_j = scale * (q . k_j);  out = sum_j e^(s_j) v_j / sum_j e^(s_j);  lse = log sum_j e^(s_j)
+ * heads is a multiple of kv_heads; query heads h * heads / kv_heads and on share key head h.  A query that sees no key gets zeros and
+ * lse = -infinity.  Codes of keys that a query does not see have no influence, NaN codes included.
+ *   lse        : [tokens][heads] f32, or NULL
+ *   max_length : at least every length; 0: max_pages * page_size is taken.  It sets how the work is split, so a tight bound helps.
+ *   scale      : positive and finite
+ *   workspace  : ptoamd_attention_kv8_workspace_bytes(...) bytes, 16-byte aligned, for work that is split over the keys of a sequence and
+ *                joined (few queries, many keys).  Nothing in it is kept from one call to the next.  NULL: not split, slower for such calls.
+ * Sums of a softmax, of scores and of values are held in f32; the scores' products take q as f16 scaled by a power of two for each row
+ * (bf16 and f16 queries lose nothing that is within 2^-14 of their row's largest element), the values' products take each weight rounded to
+ * f16, relative to the largest weight times scale so far.
+ */
+size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window);
+int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, const void* q, int type, int heads, int tokens,
+                         const int32_t* cu_tokens, int max_tokens, int max_length, int64_t q_token_stride, int64_t q_head_stride,
+                         int64_t out_token_stride, int64_t out_head_stride, float scale, int causal, int window, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -39,6 +39,7 @@ _lib.ptoamd_gemm_mx_workspace_bytes.restype = C.c_size_t
 _lib.ptoamd_gemm_mx_workspace_bytes_b_nd.restype = C.c_size_t
 _lib.ptoamd_gemm_workspace_bytes.restype = C.c_size_t
 _lib.ptoamd_gemv_mxfp4_packed_bytes.restype = C.c_size_t
+_lib.ptoamd_attention_kv8_workspace_bytes.restype = C.c_size_t
 
 EXPORTS = [
     "ptoamd_init", "ptoamd_finalize", "ptoamd_last_error", "ptoamd_device_info", "ptoamd_malloc", "ptoamd_free",
@@ -50,9 +51,10 @@ EXPORTS = [
     "ptoamd_gemm_mx_workspace_bytes", "ptoamd_gemm_mx_workspace_bytes_b_nd", "ptoamd_gemm_mx_static", "ptoamd_gemv_mxfp4", "ptoamd_gemv_mxfp4_packed_bytes", "ptoamd_gemv_mxfp4_pack", "ptoamd_gemv_mxfp4_packed", "ptoamd_tquant_int8",
     "ptoamd_tquant_int8_para", "ptoamd_tquant_mx", "ptoamd_tdequant", "ptoamd_tdequant_para", "ptoamd_mx_scale_relayout",
     "ptoamd_last_kernel", "ptoamd_reload_options",
+    "ptoamd_rope_table", "ptoamd_rope", "ptoamd_kvcache_append", "ptoamd_attention_kv8_workspace_bytes", "ptoamd_attention_kv8",
 ]
 
-# Argument types of the entry points called below (p: device address or stream, i: int, z: size_t): with them ctypes takes plain
+# Argument types of the entry points called below (p: device address or stream, i: int, l: int64_t, z: size_t, f: float, d: double): with them ctypes takes plain
 # integers, so that no c_void_p objects are made per call.
 _SIGNATURES = {
     "ptoamd_gemm": "pippip" + "iiiiiiii" + "p",
@@ -75,9 +77,14 @@ _SIGNATURES = {
     "ptoamd_tdequant": "ppipp" + "ii" + "p",
     "ptoamd_tdequant_para": "ppipp" + "iiii" + "p",
     "ptoamd_mx_scale_relayout": "pipiii" + "p",
+    "ptoamd_rope_table": "pii" + "ddddd" + "p",
+    "ptoamd_rope": "ppipip" + "iiii" + "llll" + "ii" + "p",
+    "ptoamd_kvcache_append": "pppiipi" + "llll" + "p",
+    "ptoamd_attention_kv8": "ppppiiipii" + "llll" + "fii" + "pzp",
 }
 for _name, _sig in _SIGNATURES.items():
-    getattr(_lib, _name).argtypes = [{"p": C.c_void_p, "i": C.c_int, "z": C.c_size_t}[c] for c in _sig]
+    getattr(_lib, _name).argtypes = [{"p": C.c_void_p, "i": C.c_int, "l": C.c_int64, "z": C.c_size_t, "f": C.c_float, "d": C.c_double}[c]
+                                    for c in _sig]
 
 
 class _EntryPoint(C.CFUNCTYPE(C.c_int)):
@@ -382,6 +389,134 @@ def mx_scale_relayout(src, src_layout, dst_layout, rows, cols, stream=None):
     return out
 
 
+# ---- rotary positions, a cache held in 8 bits, attention over it -------------------------------------------------------------
+def _require(cond, what):
+    if not cond:
+        raise PtoAmdError(what)
+
+
+def _int32(t, shape, what):
+    """Device address of an int32 tensor of that shape (what a kernel indexes by is checked, shape and type)."""
+    _require(t.is_cuda and t.dtype == torch.int32 and tuple(t.shape) == tuple(shape) and t.is_contiguous(),
+             f"{what} must be a contiguous int32 device tensor of shape {tuple(shape)}")
+    return t.data_ptr()
+
+
+def _heads(t, shape, what, dtype=None):
+    """Device address and (token, head) strides of a [tokens, heads, head_dim] tensor whose heads' elements lie together."""
+    _require(t.is_cuda and t.dim() == 3 and (shape is None or tuple(t.shape) == tuple(shape)) and (dtype is None or t.dtype == dtype)
+             and (t.stride(2) == 1 or t.shape[2] == 1),
+             f"{what} must be a device tensor [tokens, heads, head_dim]{'' if shape is None else f' of shape {tuple(shape)}'}"
+             f"{'' if dtype is None else f' and type {dtype}'} with unit stride inside a head")
+    return t.data_ptr(), t.stride(0), t.stride(1)
+
+
+def rope_table(rows, rot_dim, base=10000.0, factor=1.0, ramp_low=0.0, ramp_high=0.0, magnitude=1.0, device="cuda", stream=None):
+    """The rotations of positions 0 .. rows - 1 for rope(): [rows, rot_dim] f32, the cosines of rot_dim / 2 pairs and their sines.
+    factor divides the frequencies of pairs beyond ramp_high, those below ramp_low stay, a ramp between; both 0: all are divided."""
+    table = torch.empty((rows, rot_dim), dtype=torch.float32, device=device)
+    _check(_lib.ptoamd_rope_table(table.data_ptr(), rows, rot_dim, base, factor, ramp_low, ramp_high, magnitude, _stream(stream)),
+           "ptoamd_rope_table")
+    return table
+
+
+def rope(x, table, positions, interleaved=False, backward=False, stream=None, out=None):
+    """Rotary positions on the first table.shape[1] elements of every head of x [tokens, heads, head_dim] (f32, f16, bf16; tokens and
+    heads at any stride, so the queries and keys of a fused product in one call).  table: of rope_table(); positions: [tokens] int32.
+    interleaved: pairs (2 i, 2 i + 1), else (i, i + half).  backward=True turns a gradient back.  out may be x."""
+    _require(x.dim() == 3 and x.dtype in _SRC_TYPE, "rope: x must be [tokens, heads, head_dim] of f32, f16 or bf16")
+    tokens, heads, dim = x.shape
+    _require(table.is_cuda and table.dim() == 2 and table.dtype == torch.float32 and table.is_contiguous(),
+             "rope: table must be a contiguous f32 device tensor [rows, rot_dim]")
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=x.dtype, device=x.device)
+    xp, xt, xh = _heads(x, None, "rope: x")
+    op, ot, oh = _heads(out, x.shape, "rope: out", x.dtype)
+    _check(_lib.ptoamd_rope(op, xp, _SRC_TYPE[x.dtype], table.data_ptr(), table.shape[0], _int32(positions, (tokens,), "rope: positions"), tokens,
+                            heads, dim, table.shape[1], xt, xh, ot, oh, int(interleaved), int(backward), _stream(stream)), "ptoamd_rope")
+    return out
+
+
+class _Kv8Cache(C.Structure):
+    _fields_ = ([(n, C.c_void_p) for n in ("k", "v", "k_scale", "v_scale", "block_table", "lengths")]
+                + [(n, C.c_int) for n in ("code_type", "pages", "kv_heads", "page_size", "head_dim", "sequences", "max_pages")]
+                + [(n, C.c_int64) for n in ("k_page_stride", "k_head_stride", "k_token_stride", "v_page_stride", "v_head_stride", "v_token_stride")])
+
+
+def _kv8_cache(what, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type):
+    _require(k_cache.dim() == 4 and block_table.dim() == 2, f"{what}: the caches are [pages, kv_heads, page_size, head_dim], block_table [sequences, max_pages]")
+    pages, heads, page, dim = k_cache.shape
+    for t, name in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _require(t.is_cuda and tuple(t.shape) == (pages, heads, page, dim) and t.element_size() == 1 and t.stride(3) == 1,
+                 f"{what}: {name} must be a device tensor [pages, kv_heads, page_size, head_dim] of one byte an element, unit stride inside a head")
+    for t, name in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        _require(t.is_cuda and t.dtype == torch.float32 and tuple(t.shape) == (pages, heads) and t.is_contiguous(),
+                 f"{what}: {name} must be a contiguous f32 device tensor [pages, kv_heads]")
+    seqs, wide = block_table.shape
+    return _Kv8Cache(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                     _int32(block_table, (seqs, wide), f"{what}: block_table"), _int32(lengths, (seqs,), f"{what}: lengths"),
+                     code_type, pages, heads, page, dim, seqs, wide, *k_cache.stride()[:3], *v_cache.stride()[:3])
+
+
+def _tokens_of(what, tokens, seqs, cu_tokens, max_tokens):
+    """(address of cu_tokens, max_tokens); without cu_tokens every sequence has the same number of tokens."""
+    if cu_tokens is not None:
+        _require(max_tokens is not None, f"{what}: cu_tokens needs max_tokens, the most tokens of a sequence")
+        return _int32(cu_tokens, (seqs + 1,), f"{what}: cu_tokens"), max_tokens
+    _require(seqs > 0 and tokens % seqs == 0 and max_tokens in (None, tokens // seqs),
+             f"{what}: without cu_tokens every sequence has the same number of tokens ({tokens} tokens, {seqs} sequences, max_tokens {max_tokens})")
+    return None, tokens // seqs
+
+
+def kvcache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, cu_tokens=None, max_tokens=None, stream=None):
+    """Quantises the new tokens' k and v [tokens, kv_heads, head_dim] into the pages of a cache [pages, kv_heads, page_size, head_dim]
+    (code_type I8 or E4M3, any one-byte dtype, strided views too) with one scale for each page and head, [pages, kv_heads] f32.
+    lengths [sequences]: with the new tokens; cu_tokens [sequences + 1]: where each sequence's rows start (None: equal shares).
+    Changes the caches and the scales in place."""
+    what = "kvcache_append"
+    _require(k.dim() == 3 and k.dtype in _SRC_TYPE, f"{what}: k must be [tokens, kv_heads, head_dim] of f32, f16 or bf16")
+    cache = _kv8_cache(what, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type)
+    tokens = k.shape[0]
+    kp, kt, kh = _heads(k, (tokens, cache.kv_heads, cache.head_dim), f"{what}: k")
+    vp, vt, vh = _heads(v, k.shape, f"{what}: v", k.dtype)
+    cu, most = _tokens_of(what, tokens, cache.sequences, cu_tokens, max_tokens)
+    _check(_lib.ptoamd_kvcache_append(C.addressof(cache), kp, vp, _SRC_TYPE[k.dtype], tokens, cu, most, kt, kh, vt, vh, _stream(stream)),
+           "ptoamd_kvcache_append")
+
+
+def attention_kv8_workspace_bytes(q, k_cache, block_table, max_tokens, max_length=0, window=0):
+    """Bytes of workspace that attention_kv8 of these sizes splits its work with (0: not split)."""
+    pages, heads, page, dim = k_cache.shape
+    cache = _Kv8Cache(pages=pages, kv_heads=heads, page_size=page, head_dim=dim, sequences=block_table.shape[0], max_pages=block_table.shape[1])
+    return int(_lib.ptoamd_attention_kv8_workspace_bytes(C.byref(cache), q.shape[1], q.shape[0], max_tokens, max_length, window))
+
+
+def attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, cu_tokens=None, max_tokens=None, max_length=0,
+                  scale=None, causal=True, window=0, want_lse=False, stream=None, out=None, workspace=None):
+    """Attention of q [tokens, heads, head_dim] (f16, bf16) over a cache that kvcache_append fills; query i of a sequence's n stands at
+    lengths[s] - n + i.  max_length: a bound on the lengths, where the caller has a tighter one than the block table.  scale: by default
+    head_dim ** -0.5.  want_lse: returns (out, lse), lse [tokens, heads] f32.  workspace: a uint8 device tensor of
+    attention_kv8_workspace_bytes(...) bytes; by default one is allocated where the call needs it."""
+    what = "attention_kv8"
+    _require(q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16), f"{what}: q must be [tokens, heads, head_dim] of f16 or bf16")
+    cache = _kv8_cache(what, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type)
+    tokens, heads, dim = q.shape
+    qp, qt, qh = _heads(q, (tokens, heads, cache.head_dim), f"{what}: q")
+    cu, most = _tokens_of(what, tokens, cache.sequences, cu_tokens, max_tokens)
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    op, ot, oh = _heads(out, q.shape, f"{what}: out", q.dtype)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if want_lse else None
+    if workspace is None:
+        need = _lib.ptoamd_attention_kv8_workspace_bytes(C.byref(cache), heads, tokens, most, max_length, window)
+        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+    _check(_lib.ptoamd_attention_kv8(op, _ptr(lse), C.addressof(cache), qp, _SRC_TYPE[q.dtype], heads, tokens, cu, most, max_length, qt, qh, ot, oh,
+                                     dim ** -0.5 if scale is None else scale, int(causal), window, _ptr(workspace),
+                                     0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(stream)),
+           "ptoamd_attention_kv8")
+    return (out, lse) if want_lse else out
+
+
 # ---- the entry points above as native callables (binding/entry_points.cpp): they take the plain calls and hand every other one to the
 # function of that name above
 def _native_entry_points():
@@ -402,7 +537,7 @@ def _native_entry_points():
         warnings.warn(f"{path} is not used, calls take the slower way through ctypes: {e}", RuntimeWarning, stacklevel=2)
         return
     binding.set_error(PtoAmdError)
-    for f in (gemm, gemm_w8a8, gemm_mx, gemv_mxfp4, gemv_mxfp4_packed, tquant_int8, tquant_mx, tdequant):
+    for f in (gemm, gemm_w8a8, gemm_mx, gemv_mxfp4, gemv_mxfp4_packed, tquant_int8, tquant_mx, tdequant, rope, kvcache_append, attention_kv8):
         globals()[f.__name__] = binding.entry_point(f)
 
 

@@ -19,13 +19,14 @@
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <climits>
+#include <cmath>
 #include <cstring>
 
 #include "../../include/ptoamd.h"
 
 namespace {
 
-constexpr int MAX_PARAMS = 16;
+constexpr int MAX_PARAMS = 20;
 PyObject* g_error = nullptr;  // the package's PtoAmdError
 
 // Thrown where a call is none of the plain ones.
@@ -66,14 +67,42 @@ struct Call {
         if (v[i] == nullptr || !THPVariable_CheckExact(v[i]))
             throw NotPlain{};
         const at::Tensor& t = THPVariable_Unpack(v[i]);
-        static const c10::DispatchKeySet wrapped({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
-                                                  c10::DispatchKey::Functionalize, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative,
-                                                  c10::DispatchKey::ZeroTensor});
-        if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.key_set().has_any(wrapped) || t.dim() != dim)
+        if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.key_set().has_any(wrapped()) || t.dim() != dim)
             throw NotPlain{};
         if (!t.is_contiguous() && !(strided && dim == 2 && t.stride(1) == 1))
             throw NotPlain{};
         return t;
+    }
+    // the same for a view of any strides whose last dimension lies together
+    const at::Tensor& rows(int i, int dim) const
+    {
+        if (v[i] == nullptr || !THPVariable_CheckExact(v[i]))
+            throw NotPlain{};
+        const at::Tensor& t = THPVariable_Unpack(v[i]);
+        if (!t.defined() || !t.is_cuda() || t.layout() != at::kStrided || !t.has_storage() || t.key_set().has_any(wrapped()) || t.dim() != dim ||
+            t.stride(dim - 1) != 1)
+            throw NotPlain{};
+        return t;
+    }
+    const at::Tensor& typed(int i, int dim, at::ScalarType type) const
+    {
+        const at::Tensor& t = tensor(i, dim, false);
+        if (t.scalar_type() != type)
+            throw NotPlain{};
+        return t;
+    }
+    double real(int i) const
+    {
+        if (v[i] == nullptr || !PyFloat_CheckExact(v[i]))
+            throw NotPlain{};
+        return PyFloat_AS_DOUBLE(v[i]);
+    }
+    static const c10::DispatchKeySet& wrapped()
+    {
+        static const c10::DispatchKeySet keys({c10::DispatchKey::Python, c10::DispatchKey::FuncTorchBatched, c10::DispatchKey::FuncTorchGradWrapper,
+                                               c10::DispatchKey::Functionalize, c10::DispatchKey::Conjugate, c10::DispatchKey::Negative,
+                                               c10::DispatchKey::ZeroTensor});
+        return keys;
     }
 };
 
@@ -324,6 +353,146 @@ PyObject* tdequant(const Call& c)
     return wrap(std::move(out));
 }
 
+int real_type(const at::Tensor& t)
+{
+    const at::ScalarType s = t.scalar_type();
+    if (s != at::kFloat && s != at::kHalf && s != at::kBFloat16)
+        throw NotPlain{};
+    return s == at::kFloat ? PTOAMD_F32 : s == at::kHalf ? PTOAMD_F16 : PTOAMD_BF16;
+}
+
+// x, table, positions, interleaved, backward, stream, out
+PyObject* rope(const Call& c)
+{
+    c.only_default(5);
+    const at::Tensor &x = c.rows(0, 3), &table = c.typed(1, 2, at::kFloat), &positions = c.typed(2, 1, at::kInt);
+    const bool interleaved = c.truth(3, false), backward = c.truth(4, false);
+    const int type = real_type(x), tokens = extent(x.size(0)), heads = extent(x.size(1)), dim = extent(x.size(2));
+    const int rows = extent(table.size(0)), rot = extent(table.size(1));
+    at::Tensor out;
+    if (c.given(6))
+        out = c.rows(6, 3);
+    if (positions.size(0) != tokens || (out.defined() && (out.sizes() != x.sizes() || out.scalar_type() != x.scalar_type())))
+        throw NotPlain{};
+    {
+        Released no_gil;
+        if (!out.defined())
+            out = empty(x.sizes(), x.scalar_type(), x);
+        check(ptoamd_rope(address(out), address(x), type, address_as<const float>(table), rows, address_as<const int32_t>(positions), tokens, heads, dim,
+                          rot, x.stride(0), x.stride(1), out.stride(0), out.stride(1), interleaved, backward, stream()), "ptoamd_rope");
+    }
+    return wrap(std::move(out));
+}
+
+// The cache that parameters at .. at + 6 describe: k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type
+ptoamd_kv8_cache kv8_cache(const Call& c, int at)
+{
+    const at::Tensor &k = c.rows(at, 4), &v = c.rows(at + 1, 4), &ks = c.typed(at + 2, 2, at::kFloat), &vs = c.typed(at + 3, 2, at::kFloat);
+    const at::Tensor &table = c.typed(at + 4, 2, at::kInt), &lengths = c.typed(at + 5, 1, at::kInt);
+    if (k.element_size() != 1 || v.element_size() != 1 || k.sizes() != v.sizes() || ks.size(0) != k.size(0) || ks.size(1) != k.size(1) ||
+        vs.sizes() != ks.sizes() || lengths.size(0) != table.size(0))
+        throw NotPlain{};
+    ptoamd_kv8_cache r{};
+    r.k = address(k);
+    r.v = address(v);
+    r.k_scale = address_as<float>(ks);
+    r.v_scale = address_as<float>(vs);
+    r.block_table = address_as<const int32_t>(table);
+    r.lengths = address_as<const int32_t>(lengths);
+    r.code_type = c.integer(at + 6);
+    r.pages = extent(k.size(0));
+    r.kv_heads = extent(k.size(1));
+    r.page_size = extent(k.size(2));
+    r.head_dim = extent(k.size(3));
+    r.sequences = extent(table.size(0));
+    r.max_pages = extent(table.size(1));
+    r.k_page_stride = k.stride(0), r.k_head_stride = k.stride(1), r.k_token_stride = k.stride(2);
+    r.v_page_stride = v.stride(0), r.v_head_stride = v.stride(1), r.v_token_stride = v.stride(2);
+    return r;
+}
+// cu_tokens at `at`, max_tokens behind it
+const int32_t* tokens_of(const Call& c, int at, int tokens, const ptoamd_kv8_cache& cache, int* most)
+{
+    if (c.given(at)) {
+        const at::Tensor& cu = c.typed(at, 1, at::kInt);
+        if (cu.size(0) != (int64_t)cache.sequences + 1)
+            throw NotPlain{};
+        *most = c.integer(at + 1);
+        return address_as<const int32_t>(cu);
+    }
+    if (cache.sequences <= 0 || tokens % cache.sequences != 0 || (c.given(at + 1) && c.integer(at + 1) != tokens / cache.sequences))
+        throw NotPlain{};
+    *most = tokens / cache.sequences;
+    return nullptr;
+}
+
+// k, v, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, cu_tokens, max_tokens, stream
+PyObject* kvcache_append(const Call& c)
+{
+    c.only_default(11);
+    const at::Tensor &k = c.rows(0, 3), &v = c.rows(1, 3);
+    const ptoamd_kv8_cache cache = kv8_cache(c, 2);
+    const int type = real_type(k), tokens = extent(k.size(0));
+    if (k.size(1) != cache.kv_heads || k.size(2) != cache.head_dim || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type())
+        throw NotPlain{};
+    int most = 0;
+    const int32_t* cu = tokens_of(c, 9, tokens, cache, &most);
+    {
+        Released no_gil;
+        check(ptoamd_kvcache_append(&cache, address(k), address(v), type, tokens, cu, most, k.stride(0), k.stride(1), v.stride(0), v.stride(1), stream()),
+              "ptoamd_kvcache_append");
+    }
+    Py_RETURN_NONE;
+}
+
+// q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, cu_tokens, max_tokens, max_length, scale, causal, window, want_lse, stream, out,
+// workspace
+PyObject* attention_kv8(const Call& c)
+{
+    c.only_default(15);
+    const at::Tensor& q = c.rows(0, 3);
+    const ptoamd_kv8_cache cache = kv8_cache(c, 1);
+    const int type = real_type(q), tokens = extent(q.size(0)), heads = extent(q.size(1));
+    if (type == PTOAMD_F32 || q.size(2) != cache.head_dim)
+        throw NotPlain{};
+    int most = 0;
+    const int32_t* cu = tokens_of(c, 8, tokens, cache, &most);
+    const int max_length = c.integer(10, 0), window = c.integer(13, 0);
+    const double scale = c.given(11) ? c.real(11) : 1.0 / std::sqrt((double)cache.head_dim);
+    const bool causal = c.truth(12, true), want_lse = c.truth(14, false);
+    at::Tensor out, lse, workspace;
+    if (c.given(16))
+        out = c.rows(16, 3);
+    if (c.given(17))
+        workspace = c.tensor(17, 1, false);
+    if (out.defined() && (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type()))
+        throw NotPlain{};
+    {
+        Released no_gil;
+        if (!out.defined())
+            out = empty(q.sizes(), q.scalar_type(), q);
+        if (want_lse)
+            lse = empty({tokens, heads}, at::kFloat, q);
+        if (!workspace.defined()) {
+            const size_t need = ptoamd_attention_kv8_workspace_bytes(&cache, heads, tokens, most, max_length, window);
+            if (need != 0)
+                workspace = empty({(int64_t)need}, at::kByte, q);
+        }
+        check(ptoamd_attention_kv8(address(out), want_lse ? address_as<float>(lse) : nullptr, &cache, address(q), type, heads, tokens, cu, most, max_length,
+                                   q.stride(0), q.stride(1), out.stride(0), out.stride(1), (float)scale, causal, window,
+                                   workspace.defined() ? address(workspace) : nullptr, workspace.defined() ? workspace.nbytes() : 0, stream()),
+              "ptoamd_attention_kv8");
+    }
+    if (!want_lse)
+        return wrap(std::move(out));
+    PyObject* result = PyTuple_New(2);
+    if (result == nullptr)
+        return nullptr;
+    PyTuple_SET_ITEM(result, 0, wrap(std::move(out)));
+    PyTuple_SET_ITEM(result, 1, wrap(std::move(lse)));
+    return result;
+}
+
 struct Native {
     const char* name;
     PyObject* (*run)(const Call&);
@@ -339,6 +508,11 @@ const Native natives[] = {
     {"tquant_int8", tquant_int8, 2, {"src", "scale", "offset", "stream", "out"}},
     {"tquant_mx", tquant_mx, 2, {"src", "alg", "axis", "want_aux", "stream", "out"}},
     {"tdequant", tdequant, 3, {"src", "scale", "offset", "stream", "out"}},
+    {"rope", rope, 3, {"x", "table", "positions", "interleaved", "backward", "stream", "out"}},
+    {"kvcache_append", kvcache_append, 9, {"k", "v", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "lengths", "code_type", "cu_tokens",
+                                           "max_tokens", "stream"}},
+    {"attention_kv8", attention_kv8, 8, {"q", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "lengths", "code_type", "cu_tokens", "max_tokens",
+                                         "max_length", "scale", "causal", "window", "want_lse", "stream", "out", "workspace"}},
 };
 
 // ---- the callable -------------------------------------------------------------------------------------------------------

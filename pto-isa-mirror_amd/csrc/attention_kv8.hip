@@ -1,0 +1,165 @@
+// Attention over a cache of keys and values held in 8 bits: the generic kernel, the choice of a kernel, the entry points.
+#include "common_host.hpp"
+#include "kv8.hpp"
+
+namespace ptoamd {
+
+struct AttentionArgs {
+    Kv8 cache;
+    const uint8_t* q;
+    uint8_t* out;
+    float* lse;
+    int64_t q_token, q_head, out_token, out_head;  // bytes
+    int heads, group;                              // query heads, and those that share a key head
+    int causal, window;
+    float scale;
+};
+
+// The keys that a query at `place` of a sequence of `length` tokens sees: [first, last).
+__device__ __forceinline__ int2 visible_keys(const AttentionArgs& a, int place, int length)
+{
+    const int last = a.causal ? min(place + 1, length) : length;
+    const int first = a.window > 0 ? max(place - a.window + 1, 0) : 0;
+    return make_int2(first, max(last, first));
+}
+
+// One wave a query and head, in f32 throughout: a lane's key of 64 at a time, then a lane's elements of the result.  Any head_dim that
+// is a multiple of 8 up to 512, any number of queries: what the other kernels are checked against, and what head sizes without a kernel
+// of their own run on.
+template <typename T, int CODE>
+__global__ void __launch_bounds__(64) attention_kv8_generic_kernel(AttentionArgs a)
+{
+    const Kv8& c = a.cache;
+    const int nth = blockIdx.x, head = blockIdx.y, seq = blockIdx.z, kv_head = head / a.group, lane = threadIdx.x;
+    const int first = c.first_token(seq), count = c.token_count(seq, first);
+    if (nth >= count)
+        return;
+    const int length = c.length(seq), dim = c.head_dim;
+    const int2 keys = visible_keys(a, length - count + nth, length);
+    __shared__ float q[512], weight[64];
+    const T* row = reinterpret_cast<const T*>(a.q + (int64_t)(first + nth) * a.q_token + (int64_t)head * a.q_head);
+    for (int i = lane; i < dim; i += 64)
+        q[i] = (float)row[i];
+    float top = -INFINITY, total = 0.0f, o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        o[i] = 0.0f;
+    for (int base = keys.x; base < keys.y; base += 64) {
+        __syncthreads();  // q; the weights of the tile before have been read
+        const int key = base + lane;
+        float s = -INFINITY;
+        if (key < keys.y) {
+            const int page = c.page_of(seq, key >> c.page_shift), slot = key & ((1 << c.page_shift) - 1);
+            const uint8_t* k = c.k.codes + (int64_t)max(page, 0) * c.k.page + (int64_t)kv_head * c.k.head + (int64_t)slot * c.k.token;
+            float dot = 0.0f;
+            for (int i = 0; i < dim; i += 8) {
+                const uint2 w = *reinterpret_cast<const uint2*>(k + i);
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    dot = fmaf(q[i + j], kv8_value<CODE>(((j < 4 ? w.x : w.y) >> (8 * (j % 4))) & 0xFFu), dot);
+            }
+            s = page < 0 ? NAN : dot * (c.k.scales[(int64_t)page * c.kv_heads + kv_head] * a.scale);
+        }
+        float high = s;  // (fmaxf leaves NaN out: a NaN score is no maximum and makes a NaN weight)
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1)
+            high = fmaxf(high, __shfl_xor(high, d));
+        const float before = top;
+        top = fmaxf(top, high);
+        const float from = top == -INFINITY ? 0.0f : top;
+        const float p = expf(s - from), fade = expf(before - from);
+        float sum = p;
+#pragma unroll
+        for (int d = 32; d > 0; d >>= 1)
+            sum += __shfl_xor(sum, d);
+        total = total * fade + sum;
+        weight[lane] = p;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            o[i] *= fade;
+        for (int j = 0; j < min(64, keys.y - base); ++j) {
+            const float w = weight[j];
+            const int page = c.page_of(seq, (base + j) >> c.page_shift), slot = (base + j) & ((1 << c.page_shift) - 1);
+            const uint8_t* v = c.v.codes + (int64_t)max(page, 0) * c.v.page + (int64_t)kv_head * c.v.head + (int64_t)slot * c.v.token;
+            const float wv = page < 0 ? NAN : w * c.v.scales[(int64_t)page * c.kv_heads + kv_head];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (lane + 64 * i < dim)
+                    o[i] = fmaf(wv, kv8_value<CODE>(v[lane + 64 * i]), o[i]);
+        }
+    }
+    T* out = reinterpret_cast<T*>(a.out + (int64_t)(first + nth) * a.out_token + (int64_t)head * a.out_head);
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (lane + 64 * i < dim)
+            out[lane + 64 * i] = (T)(total == 0.0f ? 0.0f : o[i] * inverse);
+    if (a.lse != nullptr && lane == 0)
+        a.lse[(int64_t)(first + nth) * a.heads + head] = total == 0.0f ? -INFINITY : top + logf(total);
+}
+
+template <typename T, int CODE>
+static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t stream)
+{
+    hipLaunchKernelGGL((attention_kv8_generic_kernel<T, CODE>), dim3((unsigned)a.cache.max_tokens, (unsigned)a.heads, (unsigned)sequences), dim3(64), 0, stream, a);
+    PTOAMD_HIP_CHECK(hipGetLastError());
+    set_last_kernel("attention_kv8_generic");
+    return PTOAMD_OK;
+}
+
+}  // namespace ptoamd
+
+using namespace ptoamd;
+
+extern "C" {
+
+size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache*, int, int, int, int, int) { return 0; }
+
+int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, const void* q, int type, int heads, int tokens,
+                         const int32_t* cu_tokens, int max_tokens, int max_length, int64_t q_token_stride, int64_t q_head_stride,
+                         int64_t out_token_stride, int64_t out_head_stride, float scale, int causal, int window, void* workspace,
+                         size_t workspace_bytes, void* stream)
+{
+    const char* what = "ptoamd_attention_kv8";
+    AttentionArgs a{};
+    const int rc = kv8_from(what, cache, tokens, cu_tokens, max_tokens, &a.cache);
+    if (rc != PTOAMD_OK)
+        return rc;
+    TraceScope trace("ATTENTION_KV8", "mix", tokens, heads, cache->head_dim);
+    trace.in(q, tokens, (long)heads * cache->head_dim, "ND", type)
+        .in(cache->k, cache->pages, (long)cache->kv_heads * cache->page_size * cache->head_dim, "ND", cache->code_type)
+        .in(cache->v, cache->pages, (long)cache->kv_heads * cache->page_size * cache->head_dim, "ND", cache->code_type)
+        .out(out, tokens, (long)heads * cache->head_dim, "ND", type).out(lse, tokens, heads, "ND", PTOAMD_F32);
+    PTOAMD_REQUIRE(type == PTOAMD_F16 || type == PTOAMD_BF16, PTOAMD_E_UNSUPPORTED, "%s: queries must be f16 or bf16", what);
+    PTOAMD_REQUIRE(heads > 0 && heads % cache->kv_heads == 0 && heads <= 65535, PTOAMD_E_INVALID,
+                   "%s: heads must be a positive multiple of kv_heads, at most 65535 (%d, %d)", what, heads, cache->kv_heads);
+    PTOAMD_REQUIRE(cache->head_dim % 8 == 0 && cache->head_dim <= 512, PTOAMD_E_UNSUPPORTED,
+                   "%s: head_dim must be a multiple of 8 and at most 512 (%d)", what, cache->head_dim);
+    PTOAMD_REQUIRE(scale > 0 && isfinite(scale), PTOAMD_E_INVALID, "%s: scale must be positive and finite", what);
+    PTOAMD_REQUIRE(window >= 0 && max_length >= 0, PTOAMD_E_INVALID, "%s: window and max_length must not be negative (%d, %d)", what, window, max_length);
+    if (tokens == 0 || max_tokens == 0)
+        return PTOAMD_OK;
+    PTOAMD_REQUIRE(out && q, PTOAMD_E_INVALID, "%s: null operand", what);
+    PTOAMD_REQUIRE((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % 2 == 0 && reinterpret_cast<uintptr_t>(lse) % 4 == 0, PTOAMD_E_ALIGNMENT,
+                   "%s: q, out and lse must be aligned to their elements", what);
+    a.q = static_cast<const uint8_t*>(q);
+    a.out = static_cast<uint8_t*>(out);
+    a.lse = lse;
+    a.q_token = q_token_stride * 2;
+    a.q_head = q_head_stride * 2;
+    a.out_token = out_token_stride * 2;
+    a.out_head = out_head_stride * 2;
+    a.heads = heads;
+    a.group = heads / cache->kv_heads;
+    a.causal = causal != 0;
+    a.window = window;
+    a.scale = scale;
+    hipStream_t s = as_stream(stream);
+    const bool i8 = cache->code_type == PTOAMD_I8;
+    if (type == PTOAMD_F16)
+        return i8 ? launch_generic<_Float16, PTOAMD_I8>(a, cache->sequences, s) : launch_generic<_Float16, PTOAMD_E4M3>(a, cache->sequences, s);
+    return i8 ? launch_generic<__bf16, PTOAMD_I8>(a, cache->sequences, s) : launch_generic<__bf16, PTOAMD_E4M3>(a, cache->sequences, s);
+}
+
+}  // extern "C"

@@ -1,27 +1,7 @@
 // Attention over a cache of keys and values held in 8 bits: the generic kernel, the choice of a kernel, the entry points.
-#include "common_host.hpp"
-#include "kv8.hpp"
+#include "attention_kv8.hpp"
 
 namespace ptoamd {
-
-struct AttentionArgs {
-    Kv8 cache;
-    const uint8_t* q;
-    uint8_t* out;
-    float* lse;
-    int64_t q_token, q_head, out_token, out_head;  // bytes
-    int heads, group;                              // query heads, and those that share a key head
-    int causal, window;
-    float scale;
-};
-
-// The keys that a query at `place` of a sequence of `length` tokens sees: [first, last).
-__device__ __forceinline__ int2 visible_keys(const AttentionArgs& a, int place, int length)
-{
-    const int last = a.causal ? min(place + 1, length) : length;
-    const int first = a.window > 0 ? max(place - a.window + 1, 0) : 0;
-    return make_int2(first, max(last, first));
-}
 
 // One wave a query and head, in f32 throughout: a lane's key of 64 at a time, then a lane's elements of the result.  Any head_dim that
 // is a multiple of 8 up to 512, any number of queries: what the other kernels are checked against, and what head sizes without a kernel
@@ -108,13 +88,55 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
     return PTOAMD_OK;
 }
 
+// Which kernel runs and how the keys are split, from sizes alone: the same for the workspace's size as for the call.
+//   few  : at most 32 rows (new tokens of a sequence times the query heads that share a key head)
+// Parts: enough for two workgroups a CU over sequences and key heads, none below 256 keys (two tiles a wave: below, a part's start and
+// the join cost more than its keys).
+struct AttentionPlan {
+    bool few;
+    int splits, chunk;
+};
+static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int max_tokens, int max_length, int window)
+{
+    AttentionPlan p{false, 1, 0};
+    const bool sized = c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256;
+    const long rows = (long)max_tokens * (heads / c->kv_heads);
+    p.few = sized && rows <= 32;
+    if (!p.few)
+        return p;
+    long keys = (long)c->max_pages * c->page_size;
+    if (max_length > 0 && max_length < keys)
+        keys = max_length;
+    if (window > 0 && (long)window + max_tokens + 31 < keys)
+        keys = (long)window + max_tokens + 31;
+    const long items = (long)c->sequences * c->kv_heads, wanted = 2 * device_compute_units();
+    long splits = (wanted + items - 1) / items;
+    const long most = (keys + 255) / 256;
+    splits = splits < most ? splits : most;
+    if (splits <= 1)
+        return p;
+    p.chunk = (int)(((keys + splits - 1) / splits + 127) / 128 * 128);
+    p.splits = (int)((keys + p.chunk - 1) / p.chunk);
+    return p;
+}
+static size_t part_bytes(const AttentionPlan& p, int heads, int tokens, int head_dim)
+{
+    return p.splits > 1 ? (size_t)p.splits * tokens * heads * (head_dim * sizeof(float) + sizeof(float2)) : 0;
+}
+
 }  // namespace ptoamd
 
 using namespace ptoamd;
 
 extern "C" {
 
-size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache*, int, int, int, int, int) { return 0; }
+size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window)
+{
+    if (cache == nullptr || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads != 0 || tokens <= 0 || max_tokens <= 0 || cache->sequences <= 0 ||
+        cache->max_pages <= 0 || cache->page_size <= 0)
+        return 0;
+    return part_bytes(plan_attention(cache, heads, max_tokens, max_length, window), heads, tokens, cache->head_dim);
+}
 
 int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, const void* q, int type, int heads, int tokens,
                          const int32_t* cu_tokens, int max_tokens, int max_length, int64_t q_token_stride, int64_t q_head_stride,
@@ -123,9 +145,9 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
 {
     const char* what = "ptoamd_attention_kv8";
     AttentionArgs a{};
-    const int rc = kv8_from(what, cache, tokens, cu_tokens, max_tokens, &a.cache);
-    if (rc != PTOAMD_OK)
-        return rc;
+    const int checked = kv8_from(what, cache, tokens, cu_tokens, max_tokens, &a.cache);
+    if (checked != PTOAMD_OK)
+        return checked;
     TraceScope trace("ATTENTION_KV8", "mix", tokens, heads, cache->head_dim);
     trace.in(q, tokens, (long)heads * cache->head_dim, "ND", type)
         .in(cache->k, cache->pages, (long)cache->kv_heads * cache->page_size * cache->head_dim, "ND", cache->code_type)
@@ -156,7 +178,25 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
     a.window = window;
     a.scale = scale;
     hipStream_t s = as_stream(stream);
-    const bool i8 = cache->code_type == PTOAMD_I8;
+    const bool i8 = cache->code_type == PTOAMD_I8, f16 = type == PTOAMD_F16;
+    const AttentionPlan plan = plan_attention(cache, heads, max_tokens, max_length, window);
+    const size_t need = part_bytes(plan, heads, tokens, cache->head_dim);
+    PTOAMD_REQUIRE(workspace == nullptr || workspace_bytes >= need, PTOAMD_E_INVALID, "%s: a workspace of %zu bytes is needed (%zu)", what, need, workspace_bytes);
+    PTOAMD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, PTOAMD_E_ALIGNMENT, "%s: the workspace must be 16-byte aligned", what);
+    const uint64_t cache_bits = (uint64_t)(uintptr_t)cache->k | (uint64_t)(uintptr_t)cache->v | (uint64_t)cache->k_page_stride | (uint64_t)cache->k_head_stride |
+                                (uint64_t)cache->k_token_stride | (uint64_t)cache->v_page_stride | (uint64_t)cache->v_head_stride | (uint64_t)cache->v_token_stride;
+    if (plan.few && cache_bits % 16 == 0 && !options().force_generic) {
+        a.wide = ((uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)out | (uint64_t)a.q_token | (uint64_t)a.q_head | (uint64_t)a.out_token | (uint64_t)a.out_head) % 16 == 0;
+        a.splits = workspace != nullptr ? plan.splits : 1;
+        a.chunk = plan.chunk;
+        a.part_out = static_cast<float*>(workspace);
+        a.part_sum = reinterpret_cast<float2*>(a.part_out + (size_t)plan.splits * tokens * heads * cache->head_dim);
+        const int rc = launch_attention_few(a, cache->code_type, f16, cache->sequences, s);
+        if (rc != PTOAMD_OK)
+            return rc;
+        set_last_kernel(a.splits > 1 ? "attention_kv8_few_split" : "attention_kv8_few");
+        return a.splits > 1 ? launch_attention_join(a, f16, cache->sequences, s) : PTOAMD_OK;
+    }
     if (type == PTOAMD_F16)
         return i8 ? launch_generic<_Float16, PTOAMD_I8>(a, cache->sequences, s) : launch_generic<_Float16, PTOAMD_E4M3>(a, cache->sequences, s);
     return i8 ? launch_generic<__bf16, PTOAMD_I8>(a, cache->sequences, s) : launch_generic<__bf16, PTOAMD_E4M3>(a, cache->sequences, s);

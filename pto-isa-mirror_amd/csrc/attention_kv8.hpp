@@ -1,0 +1,150 @@
+// Attention over a cache held in 8 bits: what its kernels share.
+#pragma once
+#include "common_host.hpp"
+#include "kv8.hpp"
+#include "lds_dma.hpp"
+
+namespace ptoamd {
+
+struct AttentionArgs {
+    Kv8 cache;
+    const uint8_t* q;
+    uint8_t* out;
+    float* lse;
+    int64_t q_token, q_head, out_token, out_head;  // bytes
+    int heads, group;                              // query heads, and those that share a key head
+    int causal, window;
+    float scale;
+    int wide;  // rows of q and out allow 16-byte accesses
+    // The keys of a sequence in parts of `chunk` tokens, each a workgroup's, where splits > 1: every part leaves its sums of a row (unscaled)
+    // and the row's reference and sum, [split][token][head]; a second kernel joins them in the order of the parts.
+    int splits, chunk;
+    float* part_out;
+    float2* part_sum;
+};
+
+int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
+int launch_attention_join(const AttentionArgs& a, bool f16, int sequences, hipStream_t stream);
+int prepare_attention_kernels();
+
+// Wave-uniform reads of what no kernel writes (tables, lengths, scales) through the scalar cache.
+template <typename T>
+__device__ __forceinline__ T load_uniform(const T* p)
+{
+    typedef const __attribute__((address_space(4))) T* constant_ptr;
+    return *(constant_ptr)(uintptr_t)p;
+}
+
+// A sequence's place in the call: its rows of q, its length, the keys that any of its queries sees (aligned down to 32 tokens at the start).
+struct Span {
+    int first, count, length, begin;
+};
+__device__ __forceinline__ Span span_of(const AttentionArgs& a, int seq)
+{
+    const Kv8& c = a.cache;
+    Span s;
+    s.first = seq * c.max_tokens;
+    s.count = c.max_tokens;
+    if (c.cu_tokens != nullptr) {
+        s.first = min(max(load_uniform(c.cu_tokens + seq), 0), c.tokens);
+        s.count = min(max(load_uniform(c.cu_tokens + seq + 1), s.first) - s.first, min(c.max_tokens, c.tokens - s.first));
+    }
+    s.length = min(max(load_uniform(c.lengths + seq), 0), c.max_pages << c.page_shift);
+    s.begin = a.window > 0 ? max(s.length - s.count + 1 - a.window, 0) & ~31 : 0;
+    return s;
+}
+// The keys that a query at `place` of a sequence of `length` tokens sees: [x, y).
+__device__ __forceinline__ int2 visible_keys(const AttentionArgs& a, int place, int length)
+{
+    const int last = a.causal ? min(max(place + 1, 0), length) : length;
+    const int first = a.window > 0 ? max(place - a.window + 1, 0) : 0;
+    return make_int2(first, max(last, first));
+}
+
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// Two codes side by side in a dword's low (HIGH false) or high half -> two f16.  Every int8 and every E4M3 value is one.
+// int8: with its sign bit turned a code is c + 128; under a high byte of 0x64 that is the f16 1024 + 128 + c, exactly.  (`w` then comes turned
+// from kv8_turn.)
+template <int CODE>
+__device__ __forceinline__ uint32_t kv8_turn(uint32_t w) { return CODE == PTOAMD_I8 ? w ^ 0x80808080u : w; }
+template <int CODE, bool HIGH>
+__device__ __forceinline__ uint32_t kv8_pair_to_f16(uint32_t w)
+{
+    if (CODE == PTOAMD_I8) {
+        const f16x2 biased = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(w, 0x64646464u, HIGH ? 0x00070006u : 0x00050004u));
+        const f16x2 bias = {(_Float16)1152.0f, (_Float16)1152.0f};
+        return __builtin_bit_cast(uint32_t, biased - bias);
+    }
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HIGH));
+}
+__device__ __forceinline__ uint32_t pack_f16(float a, float b)
+{
+    typedef float f32x2 __attribute__((ext_vector_type(2)));
+    const f32x2 v = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
+}
+
+// Eight elements of a row of q as f32.
+template <typename T>
+__device__ __forceinline__ void load_row8(const uint8_t* p, bool wide, float* x)
+{
+    struct alignas(16) V { T e[8]; } v;
+    if (wide) {
+        v = *reinterpret_cast<const V*>(p);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v.e[i] = reinterpret_cast<const T*>(p)[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = (float)v.e[i];
+}
+template <typename T>
+__device__ __forceinline__ void store_row8(uint8_t* p, bool wide, const float* x)
+{
+    struct alignas(16) V { T e[8]; } v;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v.e[i] = (T)x[i];
+    if (wide) {
+        *reinterpret_cast<V*>(p) = v;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            reinterpret_cast<T*>(p)[i] = v.e[i];
+    }
+}
+
+// A row of queries is multiplied as f16, scaled by the power of two that brings its largest element into [1, 2): what that takes off an
+// element of bf16 or f16 is below 2^-25 of the largest.  The factor that undoes it; NaN for a row that holds an infinity or a NaN.
+struct RowScale {
+    float down, up;
+};
+__device__ __forceinline__ RowScale row_scale(float largest)
+{
+    const uint32_t bits = f2u(largest) & 0x7FFFFFFFu;
+    if (bits >= 0x7F800000u)
+        return RowScale{1.0f, NAN};
+    const uint32_t e = min(max(bits >> 23, 1u), 253u);
+    return RowScale{u2f((254u - e) << 23), u2f(e << 23)};
+}
+
+// A softmax reference starts here: finite, so that a row that has seen no key yet subtracts nothing undefined.
+constexpr float NO_REFERENCE = -3.0e38f;
+// How far, in powers of two, a weight may pass its reference before the reference follows: weights up to 2^8 are as exact in f16, and the
+// sums are scaled again in few of the tiles.
+constexpr float LAZY = 8.0f;
+// The scale of a page's values as a weight: its logarithm goes into the weight, its inverse back out of the sum.  Scales below 2^-64 count as
+// 2^-64 in both: beside any other page such values are nothing in f16.
+struct ValueScale {
+    float log2, inverse;
+};
+__device__ __forceinline__ ValueScale value_scale(float s)
+{
+    const float at_least = s < 0x1p-64f ? 0x1p-64f : s;  // (NaN stays)
+    return ValueScale{__builtin_amdgcn_logf(at_least), __builtin_amdgcn_rcpf(at_least)};
+}
+
+}  // namespace ptoamd

@@ -1,0 +1,416 @@
+// Attention over an 8-bit cache for few queries: decode, and a few tokens guessed ahead.
+#include "attention_kv8.hpp"
+
+namespace ptoamd {
+
+// The rows of a sequence and key head -- its new tokens times the query heads that share the head, token-major -- are the columns of the
+// matrix instructions, 16 a tile, NT tiles; keys are their rows.  A wave takes 32 keys at a time straight from memory into registers:
+//   S^T = K q^T : a lane's fragment is 8 codes of one key.  Which elements of the head make up a step is free as long as q's fragment has
+//                 the same, so a lane reads 16 bytes in a row and has two steps of them.
+//   o^T = V^T p^T : a lane holds the scores of keys 4 g .. 4 g + 3 and 16 + 4 g .. (g = lane / 16) for its column: with these eight
+//                 keys as its share of the product's sum, the weights are the fragment as they stand.  V's fragment is one element of
+//                 the same eight keys: the lane reads D / 16 elements in a row of each and pairs them up by byte.
+// So nothing passes through LDS, and no lane needs another's data but for the maximum and the sums of a row.  Codes become f16 on the way,
+// exactly.  Each wave has its own keys (every fourth tile of the workgroup's part) and the waves join at the end.
+// Scores, references and sums are f32; a page's value scale goes into the weight (ValueScale).
+// Bound: HBM (two bytes an element and head for 2 D flops a query); the next tile's codes are in flight while one is computed.
+template <int D>
+struct FewTile {
+    static constexpr int VW = D / 64;  // dwords a lane reads of one key's values
+    uint4 k[2][D / 64];
+    uint32_t v[8][VW];
+    float ks[2];
+    float vs[2];
+};
+
+template <typename T, int CODE, int D, int NT>
+__global__ void __launch_bounds__(256) attention_kv8_few_kernel(AttentionArgs a)
+{
+    constexpr int WAVES = 4, STEPS = D / 32, VW = D / 64, MT = D / 16, PITCH = D + 4;
+    extern __shared__ __attribute__((aligned(16))) float shared[];  // [2][16 NT][PITCH]
+    __shared__ float wave_top[WAVES][16 * NT], wave_sum[WAVES][16 * NT];
+    const Kv8& c = a.cache;
+    const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 16, g = lane / 16;
+    const int part = blockIdx.x, kv_head = blockIdx.y, seq = blockIdx.z;
+    const Span span = span_of(a, seq);
+    const int rows = span.count * a.group;
+    const int begin = a.splits > 1 ? span.begin + part * a.chunk : span.begin;
+    const int end = part + 1 < a.splits ? min(span.length, begin + a.chunk) : span.length;  // (the last takes what a wrong max_length left out)
+    if (rows <= 0 || (begin >= end && part > 0))
+        return;
+
+    // the queries, as fragments: step st = 2 cc + e of a lane is elements 64 cc + 16 g + 8 e ..
+    uint4 q[NT][STEPS];
+    float cq[NT];  // what a product of codes is multiplied with beside the key scale, in units of log2
+    int2 seen[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        const int row = 16 * t + col, token = row / a.group;
+        const bool valid = row < rows;
+        seen[t] = valid ? visible_keys(a, span.length - span.count + token, span.length) : make_int2(0, 0);
+        const uint8_t* p = a.q + (int64_t)(span.first + (valid ? token : 0)) * a.q_token + (int64_t)(kv_head * a.group + (valid ? row - token * a.group : 0)) * a.q_head;
+        float x[STEPS][8], largest = 0.0f;
+        bool nan = false;
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+            load_row8<T>(p + 2 * (64 * (st / 2) + 16 * g + 8 * (st % 2)), a.wide, x[st]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[st][i] = valid ? x[st][i] : 0.0f;
+                largest = fmaxf(largest, fabsf(x[st][i]));
+                nan |= x[st][i] != x[st][i];
+            }
+        }
+        largest = nan ? INFINITY : largest;
+        largest = fmaxf(largest, __shfl_xor(largest, 16));
+        largest = fmaxf(largest, __shfl_xor(largest, 32));
+        const RowScale r = row_scale(largest);
+        cq[t] = r.up * (a.scale * 1.44269504088896341f);
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[st][i] *= r.down;
+            q[t][st] = make_uint4(pack_f16(x[st][0], x[st][1]), pack_f16(x[st][2], x[st][3]), pack_f16(x[st][4], x[st][5]), pack_f16(x[st][6], x[st][7]));
+        }
+    }
+    // tiles of keys that every row sees need no mask; keys that none sees have their codes cleared
+    const int every_from = a.window > 0 ? max(span.length - a.window, 0) : 0;
+    const int every_to = a.causal ? span.length - span.count + 1 : span.length;
+    const int any_from = a.window > 0 ? max(span.length - span.count + 1 - a.window, 0) : 0;
+
+    const int last_key = max(span.length - 1, 0);
+    auto page_at = [&](int key) { return load_uniform(c.table + (int64_t)seq * c.max_pages + (min(key, last_key) >> c.page_shift)); };
+    auto fetch = [&](FewTile<D>& tile, int key, const int* ids) {
+        const int mask = (1 << c.page_shift) - 1;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int id = __builtin_amdgcn_readfirstlane(ids[h]);
+            const bool known = (unsigned)id < (unsigned)c.pages;
+            const int64_t page = known ? id : 0;
+            const int slot = min(key + 16 * h, last_key) & mask & ~15;
+            const uint8_t* kp = c.k.codes + page * c.k.page + kv_head * c.k.head + slot * c.k.token;
+            const uint8_t* vp = c.v.codes + page * c.v.page + kv_head * c.v.head + slot * c.v.token;
+#pragma unroll
+            for (int cc = 0; cc < D / 64; ++cc)
+                tile.k[h][cc] = *reinterpret_cast<const uint4*>(kp + col * c.k.token + 64 * cc + 16 * g);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t* p = reinterpret_cast<const uint32_t*>(vp + (4 * g + i) * c.v.token + col * (D / 16));
+#pragma unroll
+                for (int w = 0; w < VW; ++w)
+                    tile.v[4 * h + i][w] = p[w];
+            }
+            const float ks = load_uniform(c.k.scales + page * c.kv_heads + kv_head), vs = load_uniform(c.v.scales + page * c.kv_heads + kv_head);
+            tile.ks[h] = known ? ks : NAN;
+            tile.vs[h] = known ? vs : NAN;
+        }
+    };
+
+    f32x4 o[NT][MT];
+    float top[NT], sum[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        top[t] = NO_REFERENCE;
+        sum[t] = 0.0f;
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+            o[t][m] = f32x4{0, 0, 0, 0};
+    }
+
+    auto compute = [&](FewTile<D>& tile, int key) {
+        f32x4 s[NT][2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int t = 0; t < NT; ++t)
+                s[t][h] = f32x4{0, 0, 0, 0};
+            static_for<D / 64>([&](auto cc_) {
+                constexpr int cc = decltype(cc_)::value;
+                const uint4 raw = tile.k[h][cc];
+                const uint32_t w[4] = {kv8_turn<CODE>(raw.x), kv8_turn<CODE>(raw.y), kv8_turn<CODE>(raw.z), kv8_turn<CODE>(raw.w)};
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint4 f = make_uint4(kv8_pair_to_f16<CODE, false>(w[2 * e]), kv8_pair_to_f16<CODE, true>(w[2 * e]),
+                                               kv8_pair_to_f16<CODE, false>(w[2 * e + 1]), kv8_pair_to_f16<CODE, true>(w[2 * e + 1]));
+#pragma unroll
+                    for (int t = 0; t < NT; ++t)
+                        s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, f), __builtin_bit_cast(f16x8, q[t][2 * cc + e]), s[t][h], 0, 0, 0);
+                }
+            });
+        }
+        const bool whole = key >= every_from && key + 32 <= every_to;
+        const ValueScale value[2] = {value_scale(tile.vs[0]), value_scale(tile.vs[1])};
+        uint4 p[NT];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            float w[2][4], high = -INFINITY;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const float scale = cq[t] * tile.ks[h];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    w[h][i] = fmaf(s[t][h][i], scale, value[h].log2);
+                    if (!whole) {
+                        const int at = key + 16 * h + 4 * g + i;
+                        w[h][i] = at >= seen[t].x && at < seen[t].y ? w[h][i] : -INFINITY;
+                    }
+                    high = fmaxf(high, w[h][i]);
+                }
+            }
+            if (__ballot(high > top[t] + LAZY) != 0) {
+                high = fmaxf(high, __shfl_xor(high, 16));
+                high = fmaxf(high, __shfl_xor(high, 32));
+                const float to = fmaxf(top[t], high), fade = __builtin_amdgcn_exp2f(top[t] - to);
+                top[t] = to;
+                sum[t] *= fade;
+#pragma unroll
+                for (int m = 0; m < MT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        o[t][m][i] *= fade;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    w[h][i] = __builtin_amdgcn_exp2f(w[h][i] - top[t]);
+                const float four = (w[h][0] + w[h][1]) + (w[h][2] + w[h][3]);
+                sum[t] = four == 0.0f ? sum[t] : fmaf(four, value[h].inverse, sum[t]);  // (a NaN scale that the row does not see)
+            }
+            p[t] = make_uint4(pack_f16(w[0][0], w[0][1]), pack_f16(w[0][2], w[0][3]), pack_f16(w[1][0], w[1][1]), pack_f16(w[1][2], w[1][3]));
+        }
+        if (key < any_from || key + 32 > span.length) {  // a weight of zero does not undo a NaN code
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int at = key + 16 * (j / 4) + 4 * g + j % 4;
+#pragma unroll
+                for (int w = 0; w < VW; ++w)
+                    tile.v[j][w] = at >= any_from && at < span.length ? tile.v[j][w] : 0u;
+            }
+        }
+        static_for<VW>([&](auto w_) {
+            constexpr int w = decltype(w_)::value;
+            uint32_t low[4], high[4];  // of keys 2 j and 2 j + 1: bytes 0 and 1 of both, bytes 2 and 3
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t x = kv8_turn<CODE>(tile.v[2 * j][w]), y = kv8_turn<CODE>(tile.v[2 * j + 1][w]);
+                low[j] = __builtin_amdgcn_perm(x, y, 0x01050004u);
+                high[j] = __builtin_amdgcn_perm(x, y, 0x03070206u);
+            }
+            static_for<4>([&](auto b_) {
+                constexpr int b = decltype(b_)::value;
+                uint32_t f[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    f[j] = kv8_pair_to_f16<CODE, b % 2 == 1>(b < 2 ? low[j] : high[j]);
+                const uint4 frag = make_uint4(f[0], f[1], f[2], f[3]);
+#pragma unroll
+                for (int t = 0; t < NT; ++t)
+                    o[t][4 * w + b] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, frag), __builtin_bit_cast(f16x8, p[t]), o[t][4 * w + b], 0, 0, 0);
+            });
+        });
+    };
+
+    // every fourth tile is a wave's; the pages of the tile after the next are asked for while the next one's codes are
+    const int first = begin + 32 * wave;
+    if (first < end) {
+        int ids[2] = {page_at(first), page_at(first + 16)};
+        FewTile<D> now, next;
+        fetch(now, first, ids);
+        ids[0] = page_at(first + 32 * WAVES);
+        ids[1] = page_at(first + 32 * WAVES + 16);
+        for (int key = first; key < end; key += 32 * WAVES) {
+            fetch(next, key + 32 * WAVES, ids);
+            ids[0] = page_at(key + 64 * WAVES);
+            ids[1] = page_at(key + 64 * WAVES + 16);
+            compute(now, key);
+            now = next;
+        }
+    }
+
+    // the waves' sums on one reference for each row
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        sum[t] += __shfl_xor(sum[t], 16);
+        sum[t] += __shfl_xor(sum[t], 32);
+        if (g == 0) {
+            wave_top[wave][16 * t + col] = top[t];
+            wave_sum[wave][16 * t + col] = sum[t];
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float to = wave_top[0][16 * t + col];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w)
+            to = fmaxf(to, wave_top[w][16 * t + col]);
+        const float fade = __builtin_amdgcn_exp2f(top[t] - to);
+#pragma unroll
+        for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                o[t][m][i] *= fade;
+    }
+    // a lane has D / 4 elements of its column's row from 4 g D / 16 on: element (4 g + i) D / 16 + m is o[t][m][i]
+    float* mine = shared + (wave % 2) * (16 * NT * PITCH) + col * PITCH + g * (D / 4);
+    auto each = [&](auto&& f) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int m = 0; m < MT; m += 4)
+                    f(reinterpret_cast<f32x4*>(mine + t * 16 * PITCH + i * MT + m), f32x4{o[t][m][i], o[t][m + 1][i], o[t][m + 2][i], o[t][m + 3][i]});
+    };
+    if (wave >= 2)
+        each([](f32x4* at, f32x4 x) { *at = x; });
+    __syncthreads();
+    if (wave < 2)
+        each([](f32x4* at, f32x4 x) { *at += x; });
+    __syncthreads();
+    for (int u = threadIdx.x; u < min(rows, 16 * NT) * (D / 8); u += 256) {
+        const int row = u / (D / 8), piece = u % (D / 8) * 8, token = row / a.group, head = kv_head * a.group + row - token * a.group;
+        float to = wave_top[0][row];
+#pragma unroll
+        for (int w = 1; w < WAVES; ++w)
+            to = fmaxf(to, wave_top[w][row]);
+        float total = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WAVES; ++w)
+            total += wave_sum[w][row] * __builtin_amdgcn_exp2f(wave_top[w][row] - to);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[i] = shared[row * PITCH + piece + i] + shared[(16 * NT + row) * PITCH + piece + i];
+        const int64_t at = (int64_t)(span.first + token) * a.heads + head;
+        if (a.splits > 1) {
+            float* out = a.part_out + ((int64_t)part * c.tokens * a.heads + at) * D + piece;
+#pragma unroll
+            for (int i = 0; i < 8; i += 4)
+                *reinterpret_cast<f32x4*>(out + i) = f32x4{x[i], x[i + 1], x[i + 2], x[i + 3]};
+            if (piece == 0)
+                a.part_sum[(int64_t)part * c.tokens * a.heads + at] = make_float2(to, total);
+        } else {
+            const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                x[i] = total == 0.0f ? 0.0f : x[i] * inverse;
+            store_row8<T>(a.out + (int64_t)(span.first + token) * a.out_token + (int64_t)head * a.out_head + 2 * piece, a.wide, x);
+            if (a.lse != nullptr && piece == 0)
+                a.lse[at] = total == 0.0f ? -INFINITY : (to + __builtin_amdgcn_logf(total)) * 0.69314718055994531f;
+        }
+    }
+}
+
+// The parts of a sequence's keys: one workgroup a row.  Groups of D / 4 threads take every (1024 / D)-th part, and the groups are added in
+// order, so the result does not depend on which part was done first.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) attention_kv8_join_kernel(AttentionArgs a)
+{
+    constexpr int LANES = D / 4, GROUPS = 256 / LANES;
+    __shared__ float4 partial[GROUPS][LANES];
+    __shared__ float group_sum[GROUPS], group_top[GROUPS];
+    const int nth = blockIdx.x, head = blockIdx.y, seq = blockIdx.z;
+    const Span span = span_of(a, seq);
+    if (nth >= span.count)
+        return;
+    const int64_t at = (int64_t)(span.first + nth) * a.heads + head, stride = (int64_t)a.cache.tokens * a.heads;
+    const int2 keys = visible_keys(a, span.length - span.count + nth, span.length);
+    const int from = min((keys.x - span.begin) / a.chunk, a.splits - 1);
+    const int to = keys.y > keys.x ? min((keys.y - 1 - span.begin) / a.chunk, a.splits - 1) + 1 : from;
+    const int i = threadIdx.x % LANES, group = threadIdx.x / LANES;
+    float top = NO_REFERENCE, sum = 0.0f;
+    float4 o = make_float4(0, 0, 0, 0);
+    for (int part = from + group; part < to; part += GROUPS) {
+        const float2 s = a.part_sum[part * stride + at];
+        const float4 x = *reinterpret_cast<const float4*>(a.part_out + (part * stride + at) * D + 4 * i);
+        const float high = fmaxf(top, s.x), fade = __builtin_amdgcn_exp2f(top - high), by = __builtin_amdgcn_exp2f(s.x - high);
+        top = high;
+        sum = sum * fade + s.y * by;
+        o = make_float4(o.x * fade + x.x * by, o.y * fade + x.y * by, o.z * fade + x.z * by, o.w * fade + x.w * by);
+    }
+    partial[group][i] = o;
+    if (i == 0) {
+        group_top[group] = top;
+        group_sum[group] = sum;
+    }
+    __syncthreads();
+    if (threadIdx.x >= LANES)
+        return;
+    top = group_top[0];
+#pragma unroll
+    for (int k = 1; k < GROUPS; ++k)
+        top = fmaxf(top, group_top[k]);
+    sum = 0.0f;
+    o = make_float4(0, 0, 0, 0);
+#pragma unroll
+    for (int k = 0; k < GROUPS; ++k) {
+        const float by = __builtin_amdgcn_exp2f(group_top[k] - top);
+        const float4 x = partial[k][i];
+        sum += group_sum[k] * by;
+        o = make_float4(o.x + x.x * by, o.y + x.y * by, o.z + x.z * by, o.w + x.w * by);
+    }
+    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
+    T* out = reinterpret_cast<T*>(a.out + (int64_t)(span.first + nth) * a.out_token + (int64_t)head * a.out_head) + 4 * i;
+    const float x[4] = {o.x, o.y, o.z, o.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        out[j] = (T)(sum == 0.0f ? 0.0f : x[j] * inverse);
+    if (a.lse != nullptr && i == 0)
+        a.lse[at] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+}
+
+template <typename T, int CODE, int D, int NT>
+static int launch_few(const AttentionArgs& a, int sequences, hipStream_t stream)
+{
+    constexpr int bytes = 2 * 16 * NT * (D + 4) * 4;
+    PTOAMD_HIP_CHECK((ensure_dynamic_lds<&attention_kv8_few_kernel<T, CODE, D, NT>>(bytes)));
+    hipLaunchKernelGGL((attention_kv8_few_kernel<T, CODE, D, NT>), dim3((unsigned)a.splits, (unsigned)a.cache.kv_heads, (unsigned)sequences), dim3(256), bytes,
+                       stream, a);
+    PTOAMD_HIP_CHECK(hipGetLastError());
+    return PTOAMD_OK;
+}
+template <typename T, int CODE, int D>
+static int choose_tiles(const AttentionArgs& a, int sequences, hipStream_t stream)
+{
+    return a.cache.max_tokens * a.group <= 16 ? launch_few<T, CODE, D, 1>(a, sequences, stream) : launch_few<T, CODE, D, 2>(a, sequences, stream);
+}
+template <typename T, int CODE>
+static int choose_size(const AttentionArgs& a, int sequences, hipStream_t stream)
+{
+    switch (a.cache.head_dim) {
+        case 64: return choose_tiles<T, CODE, 64>(a, sequences, stream);
+        case 128: return choose_tiles<T, CODE, 128>(a, sequences, stream);
+        default: return choose_tiles<T, CODE, 256>(a, sequences, stream);
+    }
+}
+int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream)
+{
+    if (f16)
+        return code == PTOAMD_I8 ? choose_size<_Float16, PTOAMD_I8>(a, sequences, stream) : choose_size<_Float16, PTOAMD_E4M3>(a, sequences, stream);
+    return code == PTOAMD_I8 ? choose_size<__bf16, PTOAMD_I8>(a, sequences, stream) : choose_size<__bf16, PTOAMD_E4M3>(a, sequences, stream);
+}
+
+template <typename T>
+static void launch_join(const AttentionArgs& a, int sequences, hipStream_t stream)
+{
+    const dim3 grid((unsigned)a.cache.max_tokens, (unsigned)a.heads, (unsigned)sequences);
+    switch (a.cache.head_dim) {
+        case 64: hipLaunchKernelGGL((attention_kv8_join_kernel<T, 64>), grid, dim3(256), 0, stream, a); break;
+        case 128: hipLaunchKernelGGL((attention_kv8_join_kernel<T, 128>), grid, dim3(256), 0, stream, a); break;
+        default: hipLaunchKernelGGL((attention_kv8_join_kernel<T, 256>), grid, dim3(256), 0, stream, a); break;
+    }
+}
+int launch_attention_join(const AttentionArgs& a, bool f16, int sequences, hipStream_t stream)
+{
+    if (f16)
+        launch_join<_Float16>(a, sequences, stream);
+    else
+        launch_join<__bf16>(a, sequences, stream);
+    PTOAMD_HIP_CHECK(hipGetLastError());
+    return PTOAMD_OK;
+}
+
+}  // namespace ptoamd

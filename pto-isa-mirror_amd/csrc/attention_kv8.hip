@@ -90,32 +90,38 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 
 // Which kernel runs and how the keys are split, from sizes alone: the same for the workspace's size as for the call.
 //   few  : at most 32 rows (new tokens of a sequence times the query heads that share a key head)
-// Parts: enough for two workgroups a CU over sequences and key heads, none below 256 keys (two tiles a wave: below, a part's start and
-// the join cost more than its keys).
+//   many : more rows, 256 of them a workgroup (128 for heads of 256 elements)
+// Parts of the keys: few rows get enough for two workgroups a CU over sequences and key heads, none below 256 keys (two tiles a wave: below,
+// a part's start and the join cost more than its keys); many rows where they leave CUs without a workgroup, none below 1024 keys.
 struct AttentionPlan {
-    bool few;
+    enum { GENERIC, FEW, MANY } kernel;
     int splits, chunk;
 };
 static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int max_tokens, int max_length, int window)
 {
-    AttentionPlan p{false, 1, 0};
-    const bool sized = c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256;
-    const long rows = (long)max_tokens * (heads / c->kv_heads);
-    p.few = sized && rows <= 32;
-    if (!p.few)
+    AttentionPlan p{AttentionPlan::GENERIC, 1, 0};
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
         return p;
+    const long rows = (long)max_tokens * (heads / c->kv_heads);
+    p.kernel = rows <= 32 ? AttentionPlan::FEW : AttentionPlan::MANY;
     long keys = (long)c->max_pages * c->page_size;
     if (max_length > 0 && max_length < keys)
         keys = max_length;
     if (window > 0 && (long)window + max_tokens + 31 < keys)
         keys = (long)window + max_tokens + 31;
-    const long items = (long)c->sequences * c->kv_heads, wanted = 2 * device_compute_units();
+    long items = (long)c->sequences * c->kv_heads, wanted = 2 * device_compute_units(), least = 256, step = 128;
+    if (p.kernel == AttentionPlan::MANY) {
+        const int tile = c->head_dim == 256 ? 128 : 256;
+        items *= (rows + tile - 1) / tile;
+        wanted = items < device_compute_units() ? 2 * device_compute_units() : 0;
+        least = 1024;
+    }
     long splits = (wanted + items - 1) / items;
-    const long most = (keys + 255) / 256;
+    const long most = (keys + least - 1) / least;
     splits = splits < most ? splits : most;
     if (splits <= 1)
         return p;
-    p.chunk = (int)(((keys + splits - 1) / splits + 127) / 128 * 128);
+    p.chunk = (int)(((keys + splits - 1) / splits + step - 1) / step * step);
     p.splits = (int)((keys + p.chunk - 1) / p.chunk);
     return p;
 }
@@ -185,16 +191,17 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
     PTOAMD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, PTOAMD_E_ALIGNMENT, "%s: the workspace must be 16-byte aligned", what);
     const uint64_t cache_bits = (uint64_t)(uintptr_t)cache->k | (uint64_t)(uintptr_t)cache->v | (uint64_t)cache->k_page_stride | (uint64_t)cache->k_head_stride |
                                 (uint64_t)cache->k_token_stride | (uint64_t)cache->v_page_stride | (uint64_t)cache->v_head_stride | (uint64_t)cache->v_token_stride;
-    if (plan.few && cache_bits % 16 == 0 && !options().force_generic) {
+    if (plan.kernel != AttentionPlan::GENERIC && cache_bits % 16 == 0 && !options().force_generic) {
         a.wide = ((uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)out | (uint64_t)a.q_token | (uint64_t)a.q_head | (uint64_t)a.out_token | (uint64_t)a.out_head) % 16 == 0;
         a.splits = workspace != nullptr ? plan.splits : 1;
         a.chunk = plan.chunk;
         a.part_out = static_cast<float*>(workspace);
         a.part_sum = reinterpret_cast<float2*>(a.part_out + (size_t)plan.splits * tokens * heads * cache->head_dim);
-        const int rc = launch_attention_few(a, cache->code_type, f16, cache->sequences, s);
+        const bool few = plan.kernel == AttentionPlan::FEW;
+        const int rc = few ? launch_attention_few(a, cache->code_type, f16, cache->sequences, s) : launch_attention_many(a, cache->code_type, f16, cache->sequences, s);
         if (rc != PTOAMD_OK)
             return rc;
-        set_last_kernel(a.splits > 1 ? "attention_kv8_few_split" : "attention_kv8_few");
+        set_last_kernel(few ? (a.splits > 1 ? "attention_kv8_few_split" : "attention_kv8_few") : (a.splits > 1 ? "attention_kv8_many_split" : "attention_kv8_many"));
         return a.splits > 1 ? launch_attention_join(a, f16, cache->sequences, s) : PTOAMD_OK;
     }
     if (type == PTOAMD_F16)

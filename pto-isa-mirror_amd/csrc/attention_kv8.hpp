@@ -24,6 +24,7 @@ struct AttentionArgs {
 };
 
 int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
+int launch_attention_many(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_join(const AttentionArgs& a, bool f16, int sequences, hipStream_t stream);
 int prepare_attention_kernels();
 
@@ -85,18 +86,23 @@ __device__ __forceinline__ uint32_t pack_f16(float a, float b)
     return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, f16x2));
 }
 
-// Eight elements of a row of q as f32.
-template <typename T>
-__device__ __forceinline__ void load_row8(const uint8_t* p, bool wide, float* x)
+// Eight elements of a row of q, as they lie there.
+__device__ __forceinline__ uint4 load_row8(const uint8_t* p, bool wide)
 {
-    struct alignas(16) V { T e[8]; } v;
-    if (wide) {
-        v = *reinterpret_cast<const V*>(p);
-    } else {
+    if (wide)
+        return *reinterpret_cast<const uint4*>(p);
+    const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
+    uint32_t w[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            v.e[i] = reinterpret_cast<const T*>(p)[i];
-    }
+    for (int i = 0; i < 4; ++i)
+        w[i] = e[2 * i] | (uint32_t)e[2 * i + 1] << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void widen_row8(uint4 raw, float* x)
+{
+    struct V { T e[8]; };
+    const V v = __builtin_bit_cast(V, raw);
 #pragma unroll
     for (int i = 0; i < 8; ++i)
         x[i] = (float)v.e[i];
@@ -131,19 +137,53 @@ __device__ __forceinline__ RowScale row_scale(float largest)
     return RowScale{u2f((254u - e) << 23), u2f(e << 23)};
 }
 
+// The largest magnitude among a lane's elements of its row; infinity where one is a NaN.
+template <typename T, int STEPS>
+__device__ __forceinline__ float largest_of(const uint4* q)
+{
+    float largest = 0.0f;
+    bool nan = false;
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+        float x[8];
+        widen_row8<T>(q[st], x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            largest = fmaxf(largest, fabsf(x[i]));
+            nan |= x[i] != x[i];
+        }
+    }
+    return nan ? INFINITY : largest;
+}
+template <typename T, int STEPS>
+__device__ __forceinline__ void scale_to_f16(uint4* q, float by)
+{
+#pragma unroll
+    for (int st = 0; st < STEPS; ++st) {
+        float x[8];
+        widen_row8<T>(q[st], x);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            x[i] *= by;
+        q[st] = make_uint4(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]), pack_f16(x[4], x[5]), pack_f16(x[6], x[7]));
+    }
+}
+
 // A softmax reference starts here: finite, so that a row that has seen no key yet subtracts nothing undefined.
 constexpr float NO_REFERENCE = -3.0e38f;
-// How far, in powers of two, a weight may pass its reference before the reference follows: weights up to 2^8 are as exact in f16, and the
-// sums are scaled again in few of the tiles.
-constexpr float LAZY = 8.0f;
-// The scale of a page's values as a weight: its logarithm goes into the weight, its inverse back out of the sum.  Scales below 2^-64 count as
-// 2^-64 in both: beside any other page such values are nothing in f16.
+// Weights are 2^(score - reference), rounded to f16.  A reference is set so that the largest weight is 2^11, and follows only when one
+// would pass 2^15: f16 keeps all its bits down to 2^-25 of the largest weight and loses what is below 2^-36 of it, and the sums are scaled
+// again in few of the tiles.
+constexpr float SET_TO = 11.0f, MOST = 15.0f;
+// The scale of a page's values as a weight: its logarithm goes into the weight, its inverse back out of the sum.  A scale below 2^-64 counts
+// as 0: the page's codes are then taken as 0, and 2^-64 stands for it here.
+constexpr float LEAST_SCALE = 0x1p-64f;
 struct ValueScale {
     float log2, inverse;
 };
 __device__ __forceinline__ ValueScale value_scale(float s)
 {
-    const float at_least = s < 0x1p-64f ? 0x1p-64f : s;  // (NaN stays)
+    const float at_least = s < LEAST_SCALE ? LEAST_SCALE : s;  // (NaN stays)
     return ValueScale{__builtin_amdgcn_logf(at_least), __builtin_amdgcn_rcpf(at_least)};
 }
 

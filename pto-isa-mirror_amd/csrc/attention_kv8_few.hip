@@ -49,30 +49,15 @@ __global__ void __launch_bounds__(256) attention_kv8_few_kernel(AttentionArgs a)
         const bool valid = row < rows;
         seen[t] = valid ? visible_keys(a, span.length - span.count + token, span.length) : make_int2(0, 0);
         const uint8_t* p = a.q + (int64_t)(span.first + (valid ? token : 0)) * a.q_token + (int64_t)(kv_head * a.group + (valid ? row - token * a.group : 0)) * a.q_head;
-        float x[STEPS][8], largest = 0.0f;
-        bool nan = false;
 #pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-            load_row8<T>(p + 2 * (64 * (st / 2) + 16 * g + 8 * (st % 2)), a.wide, x[st]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x[st][i] = valid ? x[st][i] : 0.0f;
-                largest = fmaxf(largest, fabsf(x[st][i]));
-                nan |= x[st][i] != x[st][i];
-            }
-        }
-        largest = nan ? INFINITY : largest;
+        for (int st = 0; st < STEPS; ++st)
+            q[t][st] = valid ? load_row8(p + 2 * (64 * (st / 2) + 16 * g + 8 * (st % 2)), a.wide) : make_uint4(0, 0, 0, 0);
+        float largest = largest_of<T, STEPS>(q[t]);
         largest = fmaxf(largest, __shfl_xor(largest, 16));
         largest = fmaxf(largest, __shfl_xor(largest, 32));
         const RowScale r = row_scale(largest);
         cq[t] = r.up * (a.scale * 1.44269504088896341f);
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[st][i] *= r.down;
-            q[t][st] = make_uint4(pack_f16(x[st][0], x[st][1]), pack_f16(x[st][2], x[st][3]), pack_f16(x[st][4], x[st][5]), pack_f16(x[st][6], x[st][7]));
-        }
+        scale_to_f16<T, STEPS>(q[t], r.down);
     }
     // tiles of keys that every row sees need no mask; keys that none sees have their codes cleared
     const int every_from = a.window > 0 ? max(span.length - a.window, 0) : 0;
@@ -158,10 +143,10 @@ __global__ void __launch_bounds__(256) attention_kv8_few_kernel(AttentionArgs a)
                     high = fmaxf(high, w[h][i]);
                 }
             }
-            if (__ballot(high > top[t] + LAZY) != 0) {
+            if (__ballot(high > top[t] + MOST) != 0) {
                 high = fmaxf(high, __shfl_xor(high, 16));
                 high = fmaxf(high, __shfl_xor(high, 32));
-                const float to = fmaxf(top[t], high), fade = __builtin_amdgcn_exp2f(top[t] - to);
+                const float to = fmaxf(top[t], high - SET_TO), fade = __builtin_amdgcn_exp2f(top[t] - to);
                 top[t] = to;
                 sum[t] *= fade;
 #pragma unroll
@@ -180,13 +165,13 @@ __global__ void __launch_bounds__(256) attention_kv8_few_kernel(AttentionArgs a)
             }
             p[t] = make_uint4(pack_f16(w[0][0], w[0][1]), pack_f16(w[0][2], w[0][3]), pack_f16(w[1][0], w[1][1]), pack_f16(w[1][2], w[1][3]));
         }
-        if (key < any_from || key + 32 > span.length) {  // a weight of zero does not undo a NaN code
+        if (key < any_from || key + 32 > span.length || tile.vs[0] < LEAST_SCALE || tile.vs[1] < LEAST_SCALE) {  // a weight of zero does not undo a NaN code
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int at = key + 16 * (j / 4) + 4 * g + j % 4;
 #pragma unroll
                 for (int w = 0; w < VW; ++w)
-                    tile.v[j][w] = at >= any_from && at < span.length ? tile.v[j][w] : 0u;
+                    tile.v[j][w] = at < any_from || at >= span.length || tile.vs[j / 4] < LEAST_SCALE ? 0u : tile.v[j][w];
             }
         }
         static_for<VW>([&](auto w_) {

@@ -39,13 +39,18 @@ struct alignas(sizeof(T) * VEC) RopeVec {
     T e[VEC];
 };
 
+constexpr int ROPE_TOKENS = 2;
+
 // A unit is VEC pairs of one head: two vectors of VEC elements, half a rotation apart or, interleaved, next to each other.  A thread
-// has the same unit of TOKENS consecutive tokens, their loads all in flight before the first is used.  A token's rotations are read
-// again for every head, from the L1 after the first.  Products and sums in f32, one rounding.
-template <typename T, int VEC, bool INTERLEAVED, int TOKENS>
+// has the same unit of two consecutive tokens, all loads of both in flight before the first is used (8192 tokens of 40 heads of 128, bf16:
+// one token a thread 36.3 us, two 33.3, four, whose registers take waves off the CUs, 38.2).  A token's rotations are read again for every head,
+// from the L1 after the first.  Products and sums in f32, one rounding.
+// Bound: HBM, what is turned in once and out once: 172 MB in 33.3 us, 5.2 TB/s, as a large copy.
+template <typename T, int VEC, bool INTERLEAVED>
 __global__ void __launch_bounds__(512) rope_kernel(RopeArgs a)
 {
     typedef RopeVec<T, VEC> Vec;
+    constexpr int TOKENS = ROPE_TOKENS;
     const int unit = blockIdx.y * blockDim.x + threadIdx.x;
     const int first = blockIdx.x * TOKENS;
     if (unit >= a.units * a.heads)
@@ -57,27 +62,35 @@ __global__ void __launch_bounds__(512) rope_kernel(RopeArgs a)
     const int end = turns && !INTERLEAVED ? pair + a.half : lo + VEC;
     const int hi = VEC == 1 && end == a.head_dim ? lo : end;  // (an odd element is left over after the pairs: it is its own neighbour)
     Vec x[TOKENS][2];
+    float cosine[TOKENS][VEC], sine[TOKENS][VEC];
     int at[TOKENS];
 #pragma unroll
-    for (int k = 0; k < TOKENS; ++k) {
-        const int t = min(first + k, a.tokens - 1);
-        const T* row = reinterpret_cast<const T*>(a.x + (int64_t)t * a.x_token + (int64_t)head * a.x_head);
-        x[k][0] = *reinterpret_cast<const Vec*>(row + lo);
-        x[k][1] = *reinterpret_cast<const Vec*>(row + hi);
-        at[k] = a.positions[t];
-    }
+    for (int k = 0; k < TOKENS; ++k)
+        at[k] = a.positions[min(first + k, a.tokens - 1)];
 #pragma unroll
     for (int k = 0; k < TOKENS; ++k) {
-        if (first + k >= a.tokens)
-            break;
-        T* row = reinterpret_cast<T*>(a.out + (int64_t)(first + k) * a.out_token + (int64_t)head * a.out_head);
-        if (turns) {
+        const T* row = reinterpret_cast<const T*>(a.x + (int64_t)min(first + k, a.tokens - 1) * a.x_token + (int64_t)head * a.x_head);
+        x[k][0] = *reinterpret_cast<const Vec*>(row + lo);
+        x[k][1] = *reinterpret_cast<const Vec*>(row + hi);
+    }
+    if (turns) {
+#pragma unroll
+        for (int k = 0; k < TOKENS; ++k) {
             const bool known = (unsigned)at[k] < (unsigned)a.table_rows;
             const float* turn = a.table + (int64_t)(known ? at[k] : 0) * 2 * a.half + pair;
+#pragma unroll
+            for (int j = 0; j < VEC; ++j) {
+                cosine[k][j] = turn[j];
+                sine[k][j] = turn[a.half + j];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < TOKENS; ++k) {
+            const float unknown = (unsigned)at[k] < (unsigned)a.table_rows ? 0.0f : NAN;
             Vec y[2];
 #pragma unroll
             for (int j = 0; j < VEC; ++j) {
-                const float c = known ? turn[j] : NAN, s = known ? turn[a.half + j] * a.sign : NAN;
+                const float c = cosine[k][j] + unknown, s = fmaf(sine[k][j], a.sign, unknown);
                 // the pair's two elements: the j-th of both vectors, or neighbours
                 const int v0 = INTERLEAVED ? (2 * j) / VEC : 0, e0 = INTERLEAVED ? (2 * j) % VEC : j;
                 const int v1 = INTERLEAVED ? (2 * j + 1) / VEC : 1, e1 = INTERLEAVED ? (2 * j + 1) % VEC : j;
@@ -88,6 +101,12 @@ __global__ void __launch_bounds__(512) rope_kernel(RopeArgs a)
             x[k][0] = y[0];
             x[k][1] = y[1];
         }
+    }
+#pragma unroll
+    for (int k = 0; k < TOKENS; ++k) {
+        if (first + k >= a.tokens)
+            break;
+        T* row = reinterpret_cast<T*>(a.out + (int64_t)(first + k) * a.out_token + (int64_t)head * a.out_head);
         *reinterpret_cast<Vec*>(row + lo) = x[k][0];
         *reinterpret_cast<Vec*>(row + hi) = x[k][1];
     }
@@ -99,7 +118,7 @@ static int launch_rope(const RopeArgs& a, hipStream_t stream)
     const long units = (long)a.units * a.heads;
     const long wide = (units + 511) / 512;
     const int block = (int)(((units + wide - 1) / wide + 63) / 64 * 64);
-    hipLaunchKernelGGL((rope_kernel<T, VEC, INTERLEAVED, 1>), dim3((unsigned)a.tokens, (unsigned)wide), dim3(block), 0, stream, a);
+    hipLaunchKernelGGL((rope_kernel<T, VEC, INTERLEAVED>), dim3((unsigned)((a.tokens + ROPE_TOKENS - 1) / ROPE_TOKENS), (unsigned)wide), dim3(block), 0, stream, a);
     PTOAMD_HIP_CHECK(hipGetLastError());
     set_last_kernel("rope");
     return PTOAMD_OK;

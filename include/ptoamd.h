@@ -408,8 +408,8 @@ typedef struct ptoamd_kv8_cache {
  *   cu_tokens  : [sequences + 1] int32: rows cu_tokens[s] .. cu_tokens[s + 1] - 1 of k and v are sequence s's; they become its tokens
  *                lengths[s] - n .. lengths[s] - 1.  NULL: every sequence has max_tokens of them (tokens = sequences * max_tokens).
  *   max_tokens : at least every sequence's n
- * For each page that gets tokens, each head, K and V:  a = max |x| of the new ones;  s1 = max(s0, a / Q), s0 being the page's scale if
- * it holds older tokens of the sequence and else 0, Q = 127 (int8) or 448 (E4M3);  where s1 > s0 the older codes become
+ * For each page that gets tokens, each head, K and V:  a = max |x| of the new ones;  s1 = max(s0, a * (1 / Q)) in f32, s0 being the page's
+ * scale if it holds older tokens of the sequence and else 0, Q = 127 (int8) or 448 (E4M3), 1 / Q rounded to f32;  where s1 > s0 the older codes become
  * round(code * (s0 / s1));  new codes are round(x * (1 / s1)), ties to even, clamped.  The scale grows and never shrinks while a page
  * fills, and an append repeated changes nothing.  A scale below 2^-126 is taken as 0, its codes as 0.  If a new value is infinite or NaN,
  * the scale of its page and head is NaN from then on (and the new codes are 0): what sees it gets NaN instead of a wrong number.
@@ -425,15 +425,16 @@ int ptoamd_kvcache_append(const ptoamd_kv8_cache* cache, const void* k, const vo
  * 0 <= j < L, j <= p (causal != 0) and j > p - window (window > 0):
  *   s_j = scale * (q . k_j);  out = sum_j e^(s_j) v_j / sum_j e^(s_j);  lse = log sum_j e^(s_j)
  * heads is a multiple of kv_heads; query heads h * heads / kv_heads and on share key head h.  A query that sees no key gets zeros and
- * lse = -infinity.  Codes of keys that a query does not see have no influence, NaN codes included.
+ * lse = -infinity.  What a query does not see has no influence on it; codes that no query of the sequence sees may be NaN codes.
  *   lse        : [tokens][heads] f32, or NULL
  *   max_length : at least every length; 0: max_pages * page_size is taken.  It sets how the work is split, so a tight bound helps.
  *   scale      : positive and finite
  *   workspace  : ptoamd_attention_kv8_workspace_bytes(...) bytes, 16-byte aligned, for work that is split over the keys of a sequence and
  *                joined (few queries, many keys).  Nothing in it is kept from one call to the next.  NULL: not split, slower for such calls.
  * Sums of a softmax, of scores and of values are held in f32; the scores' products take q as f16 scaled by a power of two for each row
- * (bf16 and f16 queries lose nothing that is within 2^-14 of their row's largest element), the values' products take each weight rounded to
- * f16, relative to the largest weight times scale so far.
+ * (bf16 and f16 queries lose nothing that is within 2^-14 of their row's largest element), the values' products take each weight, times its
+ * page's value scale, rounded to f16 relative to the largest such so far: full f16 precision down to 2^-25 of that, nothing below 2^-36.  A
+ * value scale below 2^-64 counts as 0.  (Head sizes other than 64, 128 and 256 run on a kernel that is in f32 throughout, and slow.)
  */
 size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window);
 int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, const void* q, int type, int heads, int tokens,

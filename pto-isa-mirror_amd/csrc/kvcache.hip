@@ -133,7 +133,7 @@ __global__ void __launch_bounds__(256) kvcache_append_kernel(AppendArgs a)
     __syncthreads();  // (the scale has been read by all before one writes it)
     largest = max(max(wave_largest[0], wave_largest[1]), max(wave_largest[2], wave_largest[3]));
     const bool finite = largest < 0x7F800000u;
-    float after = u2f(largest) / (CODE == PTOAMD_I8 ? 127.0f : 448.0f);
+    float after = u2f(largest) * (CODE == PTOAMD_I8 ? 1.0f / 127.0f : 1.0f / 448.0f);
     after = before > after ? before : after;
     after = after < 0x1p-126f ? 0.0f : after;
     if (!finite || before != before)

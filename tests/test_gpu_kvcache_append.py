@@ -28,7 +28,7 @@ def nearest(codes, want, code):
 
 
 def check(cache, before, k, v, counts):
-    """Scales by their formula to one rounding, codes nearest in units of the scale that is there, everything else untouched."""
+    """Scales by their formula in f32, bit for bit, codes nearest in units of the scale that is there, everything else untouched."""
     for name, x in (("k", k), ("v", v)):
         codes, scales = getattr(cache, name), getattr(cache, name + "_scale")
         old_codes, old_scales = before[name], before[name + "_scale"]
@@ -41,11 +41,11 @@ def check(cache, before, k, v, counts):
             for b in range(start // cache.page, -(-length // cache.page) if n else 0):
                 lo, hi, page = max(start, b * cache.page), min(length, (b + 1) * cache.page), table[b]
                 older, rows = lo - b * cache.page, x[at + lo - start:at + hi - start].double().transpose(0, 1)
-                unit = rows.abs().amax(dim=(1, 2)) / ref.LARGEST[cache.code]
+                unit = rows.abs().amax(dim=(1, 2)).float() * torch.tensor(1.0 / ref.LARGEST[cache.code], device="cuda")  # (both in f32)
                 if older:
-                    unit = torch.maximum(unit, old_scales[page].double())
+                    unit = torch.maximum(unit, old_scales[page])
                 now = scales[page].double()
-                assert bool(((now - unit).abs() <= 2.0 ** -24 * unit).all()), (name, s, b)
+                assert torch.equal(scales[page], torch.where(unit < 2.0 ** -126, 0.0, unit)), (name, s, b)
                 per = torch.where(now > 0, now, 1.0)[:, None, None]
                 assert nearest(codes[page, :, older:older + hi - lo].contiguous(), rows / per, cache.code), (name, s, b)
                 if older:

@@ -89,10 +89,14 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 }
 
 // Which kernel runs and how the keys are split, from sizes alone: the same for the workspace's size as for the call.
-//   few  : at most 32 rows (new tokens of a sequence times the query heads that share a key head)
+//   few  : at most 96 rows (new tokens of a sequence times the query heads that share a key head), 16 or 32 of them a workgroup.
+//          8 sequences of 6000 keys, 8 key heads of 128, int8, us, few / many: 16 rows 24 / 80, 64 52 / 85, 96 74 / 89, 128 95 / 92.
 //   many : more rows, 256 of them a workgroup (128 for heads of 256 elements)
-// Parts of the keys: few rows get enough for two workgroups a CU over sequences and key heads, none below 256 keys (two tiles a wave: below,
-// a part's start and the join cost more than its keys); many rows where they leave CUs without a workgroup, none below 1024 keys.
+// Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
+// (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
+// heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.
+// Many rows: where they leave CUs without a workgroup, none below 1024 keys.
+constexpr long FEW_ROWS = 96;
 struct AttentionPlan {
     enum { GENERIC, FEW, MANY } kernel;
     int splits, chunk;
@@ -103,22 +107,31 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int ma
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
         return p;
     const long rows = (long)max_tokens * (heads / c->kv_heads);
-    p.kernel = rows <= 32 ? AttentionPlan::FEW : AttentionPlan::MANY;
+    p.kernel = rows <= FEW_ROWS ? AttentionPlan::FEW : AttentionPlan::MANY;
     long keys = (long)c->max_pages * c->page_size;
     if (max_length > 0 && max_length < keys)
         keys = max_length;
     if (window > 0 && (long)window + max_tokens + 31 < keys)
         keys = (long)window + max_tokens + 31;
-    long items = (long)c->sequences * c->kv_heads, wanted = 2 * device_compute_units(), least = 256, step = 128;
-    if (p.kernel == AttentionPlan::MANY) {
+    const long cus = device_compute_units();
+    long items = (long)c->sequences * c->kv_heads, splits, step;
+    if (p.kernel == AttentionPlan::FEW) {
+        step = 32 * few_waves(c->head_dim, rows);  // the keys that a workgroup's waves have at a time
+        const long turns = (keys + step - 1) / step;
+        splits = (cus + items - 1) / items;
+        splits = splits < turns / 2 ? splits : turns / 2;
+        if (turns <= (c->head_dim == 256 ? 4 : 6))
+            splits = 1;
+        const long even = (keys + 4095) / 4096;
+        splits = splits > even ? splits : even;
+    } else {
         const int tile = c->head_dim == 256 ? 128 : 256;
         items *= (rows + tile - 1) / tile;
-        wanted = items < device_compute_units() ? 2 * device_compute_units() : 0;
-        least = 1024;
+        step = 64;
+        splits = items < cus ? (2 * cus + items - 1) / items : 1;
+        const long most = (keys + 1023) / 1024;
+        splits = splits < most ? splits : most;
     }
-    long splits = (wanted + items - 1) / items;
-    const long most = (keys + least - 1) / least;
-    splits = splits < most ? splits : most;
     if (splits <= 1)
         return p;
     p.chunk = (int)(((keys + splits - 1) / splits + step - 1) / step * step);
@@ -191,7 +204,11 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
     PTOAMD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, PTOAMD_E_ALIGNMENT, "%s: the workspace must be 16-byte aligned", what);
     const uint64_t cache_bits = (uint64_t)(uintptr_t)cache->k | (uint64_t)(uintptr_t)cache->v | (uint64_t)cache->k_page_stride | (uint64_t)cache->k_head_stride |
                                 (uint64_t)cache->k_token_stride | (uint64_t)cache->v_page_stride | (uint64_t)cache->v_head_stride | (uint64_t)cache->v_token_stride;
-    if (plan.kernel != AttentionPlan::GENERIC && cache_bits % 16 == 0 && !options().force_generic) {
+    // (what the kernels hold in 32 bits: strides of pages in units of 8 bytes, of the tokens of a page in bytes, places of scales)
+    const bool addressable = cache->k_page_stride >= 0 && cache->k_page_stride < 1LL << 34 && cache->v_page_stride >= 0 && cache->v_page_stride < 1LL << 34 &&
+                             cache->k_token_stride >= 0 && cache->k_token_stride < 1 << 22 && cache->v_token_stride >= 0 && cache->v_token_stride < 1 << 22 &&
+                             (long)cache->pages * cache->kv_heads < 1L << 30;
+    if (plan.kernel != AttentionPlan::GENERIC && cache_bits % 16 == 0 && addressable && !options().force_generic) {
         a.wide = ((uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)out | (uint64_t)a.q_token | (uint64_t)a.q_head | (uint64_t)a.out_token | (uint64_t)a.out_head) % 16 == 0;
         a.splits = workspace != nullptr ? plan.splits : 1;
         a.chunk = plan.chunk;

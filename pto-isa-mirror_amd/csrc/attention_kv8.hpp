@@ -23,6 +23,8 @@ struct AttentionArgs {
     float2* part_sum;
 };
 
+// The waves of a few-rows workgroup: eight where two fit a SIMD's registers (heads up to 128 elements, 16 rows), else four.
+constexpr int few_waves(int head_dim, long rows) { return head_dim <= 128 && rows <= 16 ? 8 : 4; }
 int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_many(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_join(const AttentionArgs& a, bool f16, int sequences, hipStream_t stream);
@@ -78,6 +80,18 @@ __device__ __forceinline__ uint32_t kv8_pair_to_f16(uint32_t w)
         return __builtin_bit_cast(uint32_t, biased - bias);
     }
     return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8((int)w, 1.0f, HIGH));
+}
+// Two dwords' bytes number B side by side, as f16: B of `even` low, B of `odd` high.
+// int8: the turned code c + 128 alone is the f16 (c + 128) 2^-24, a subnormal one, exactly, and the matrix instructions take it as that: one
+// permutation of bytes.  The 128 goes with products of a constant (UNBIAS), the 2^24 into what the sums are scaled with.  E4M3: two codes side by
+// side are converted together.
+constexpr uint32_t UNBIAS = 0x80808080u;  // two f16 of -128 2^-24
+template <int CODE>
+constexpr float KV8_UNIT = CODE == PTOAMD_I8 ? 16777216.0f : 1.0f;
+// (dwords of int8 come turned)
+__device__ __forceinline__ uint32_t bytes_to_f16(uint32_t even, uint32_t odd, int b)
+{
+    return __builtin_amdgcn_perm(odd, even, 0x0C000C00u | (uint32_t)b | (uint32_t)(4 + b) << 16);
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b)
 {

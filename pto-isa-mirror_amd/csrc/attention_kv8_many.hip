@@ -163,21 +163,37 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_many_kernel(Attentio
             }
         }
         const bool whole = key >= every_from && key + KEYS <= every_to;
-        float4 sc[KEYS / 16];
-        float high = -INFINITY;
+        float4 sc[KEYS / 16];  // of 16 keys, 8 of them this lane's
+        float scale[KEYS / 16], high = -INFINITY;
+        // (the largest of a group's scores times its scale: the scale is not negative)
 #pragma unroll
-        for (int x = 0; x < KEYS / 16; ++x) {  // 16 keys, 8 of them this lane's
+        for (int x = 0; x < KEYS / 16; ++x) {
             sc[x] = scales[buffer][x];
-            const float scale = cq * sc[x].x;
+            scale[x] = cq * sc[x].x;
+        }
+        if (whole) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                float& w = reinterpret_cast<float*>(&s[x / 2])[8 * (x % 2) + i];
-                w = fmaf(w, scale, sc[x].y);
-                if (!whole) {
-                    const int at = key + 16 * x + 8 * (i / 4) + 4 * hf + i % 4;
-                    w = at >= seen.x && at < seen.y ? w : -INFINITY;
+            for (int x = 0; x < KEYS / 16; ++x) {
+                float eight = s[x / 2][8 * (x % 2)];
+#pragma unroll
+                for (int i = 1; i < 8; ++i)
+                    eight = fmaxf(eight, s[x / 2][8 * (x % 2) + i]);
+                high = fmaxf(high, fmaf(eight, scale[x], sc[x].y));
+            }
+        } else {
+            const uint32_t first = (uint32_t)(key + 4 * hf - seen.x), count = (uint32_t)(seen.y - seen.x);
+#pragma unroll
+            for (int x = 0; x < KEYS / 16; ++x)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float w = fmaf(s[x / 2][8 * (x % 2) + i], scale[x], sc[x].y);
+                    s[x / 2][8 * (x % 2) + i] = first + (16 * x + 8 * (i / 4) + i % 4) < count ? w : -INFINITY;
+                    high = fmaxf(high, s[x / 2][8 * (x % 2) + i]);
                 }
-                high = fmaxf(high, w);
+#pragma unroll
+            for (int x = 0; x < KEYS / 16; ++x) {  // (these are scores already)
+                scale[x] = 1.0f;
+                sc[x].y = 0.0f;
             }
         }
         if (__ballot(high > top + MOST) != 0) {
@@ -194,9 +210,10 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_many_kernel(Attentio
 #pragma unroll
         for (int x = 0; x < KEYS / 16; ++x) {
             float w[8], eight = 0.0f;
+            const float less = sc[x].y - top;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                w[i] = __builtin_amdgcn_exp2f(s[x / 2][8 * (x % 2) + i] - top);
+                w[i] = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x % 2) + i], scale[x], less));
                 eight += w[i];
             }
             sum = eight == 0.0f ? sum : fmaf(eight, sc[x].z, sum);  // (a NaN scale that the row does not see)

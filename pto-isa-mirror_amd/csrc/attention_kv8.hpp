@@ -1,5 +1,7 @@
 // Attention over a cache held in 8 bits: what its kernels share.
 #pragma once
+#include <stddef.h>
+
 #include "common_host.hpp"
 #include "kv8.hpp"
 #include "lds_dma.hpp"
@@ -37,6 +39,24 @@ __device__ __forceinline__ T load_uniform(const T* p)
     typedef const __attribute__((address_space(4))) T* constant_ptr;
     return *(constant_ptr)(uintptr_t)p;
 }
+
+// A field of the arguments (a kernel's only parameter), read from memory where it is asked for: what only the end of a kernel needs would else
+// sit in scalar registers all through its loop.
+struct ArgumentsAgain {
+    uint64_t at;
+    __device__ __forceinline__ ArgumentsAgain() : at((uint64_t)(uintptr_t)__builtin_amdgcn_kernarg_segment_ptr()) { asm volatile("" : "+s"(at)); }
+    template <typename T>
+    __device__ __forceinline__ T field(size_t offset) const
+    {
+        return *(const __attribute__((address_space(4))) T*)(at + offset);
+    }
+    template <typename T>
+    __device__ __forceinline__ T* global(size_t offset) const  // (through an integer the compiler no longer knows what memory)
+    {
+        return (T*)(__attribute__((address_space(1))) T*)(uintptr_t)field<uint64_t>(offset);
+    }
+};
+#define ARGUMENT(again, name) (again).template field<decltype(AttentionArgs::name)>(offsetof(AttentionArgs, name))
 
 // A sequence's place in the call: its rows of q, its length, the keys that any of its queries sees (aligned down to 32 tokens at the start).
 struct Span {
@@ -121,19 +141,23 @@ __device__ __forceinline__ void widen_row8(uint4 raw, float* x)
     for (int i = 0; i < 8; ++i)
         x[i] = (float)v.e[i];
 }
+// Eight results.  (The packed dwords are what both ways store: given elements, the compiler makes one of the two, then of the narrow stores.)
 template <typename T>
 __device__ __forceinline__ void store_row8(uint8_t* p, bool wide, const float* x)
 {
-    struct alignas(16) V { T e[8]; } v;
+    uint32_t w[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-        v.e[i] = (T)x[i];
+    for (int i = 0; i < 4; ++i)
+        w[i] = sizeof(T) == 2 && __is_same(T, _Float16) ? pack_f16(x[2 * i], x[2 * i + 1]) : f32x2_to_bf16x2_bits(x[2 * i], x[2 * i + 1]);
     if (wide) {
-        *reinterpret_cast<V*>(p) = v;
+        *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
     } else {
+        uint16_t* e = reinterpret_cast<uint16_t*>(p);
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
-            reinterpret_cast<T*>(p)[i] = v.e[i];
+        for (int i = 0; i < 4; ++i) {
+            e[2 * i] = (uint16_t)w[i];
+            e[2 * i + 1] = (uint16_t)(w[i] >> 16);
+        }
     }
 }
 
@@ -142,32 +166,31 @@ __device__ __forceinline__ void store_row8(uint8_t* p, bool wide, const float* x
 struct RowScale {
     float down, up;
 };
-__device__ __forceinline__ RowScale row_scale(float largest)
+template <typename T>
+__device__ __forceinline__ RowScale row_scale(uint32_t largest)
 {
-    const uint32_t bits = f2u(largest) & 0x7FFFFFFFu;
+    const uint32_t bits = f2u((float)__builtin_bit_cast(T, (uint16_t)largest));
     if (bits >= 0x7F800000u)
         return RowScale{1.0f, NAN};
     const uint32_t e = min(max(bits >> 23, 1u), 253u);
     return RowScale{u2f((254u - e) << 23), u2f(e << 23)};
 }
 
-// The largest magnitude among a lane's elements of its row; infinity where one is a NaN.
-template <typename T, int STEPS>
-__device__ __forceinline__ float largest_of(const uint4* q)
+// The largest magnitude among a lane's elements of its row, as the bits of its 16-bit type without the sign (in order, an infinity above every
+// number and a NaN above that).
+template <int STEPS>
+__device__ __forceinline__ uint32_t largest_of(const uint4* q)
 {
-    float largest = 0.0f;
-    bool nan = false;
+    typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+    u16x2 largest = {0, 0};
 #pragma unroll
     for (int st = 0; st < STEPS; ++st) {
-        float x[8];
-        widen_row8<T>(q[st], x);
+        const uint32_t w[4] = {q[st].x, q[st].y, q[st].z, q[st].w};
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            largest = fmaxf(largest, fabsf(x[i]));
-            nan |= x[i] != x[i];
-        }
+        for (int i = 0; i < 4; ++i)
+            largest = __builtin_elementwise_max(largest, __builtin_bit_cast(u16x2, w[i] & 0x7FFF7FFFu));
     }
-    return nan ? INFINITY : largest;
+    return max((uint32_t)largest[0], (uint32_t)largest[1]);
 }
 template <typename T, int STEPS>
 __device__ __forceinline__ void scale_to_f16(uint4* q, float by)

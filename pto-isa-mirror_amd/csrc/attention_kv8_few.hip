@@ -113,10 +113,10 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
     f32x4 start[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        float largest = largest_of<T, STEPS>(q[t]);
-        largest = fmaxf(largest, __shfl_xor(largest, 16));
-        largest = fmaxf(largest, __shfl_xor(largest, 32));
-        const RowScale r = row_scale(largest);
+        uint32_t largest = largest_of<STEPS>(q[t]);
+        largest = max(largest, (uint32_t)__shfl_xor((int)largest, 16));
+        largest = max(largest, (uint32_t)__shfl_xor((int)largest, 32));
+        const RowScale r = row_scale<T>(largest);
         cq[t] = r.up * (a.scale * 1.44269504088896341f) * KV8_UNIT<CODE>;
         scale_to_f16<T, STEPS>(q[t], r.down);
         // where the products' sums start: without the 128 that int8 codes carry

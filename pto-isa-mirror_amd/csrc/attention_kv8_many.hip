@@ -28,13 +28,14 @@ struct ManyTile {
 };
 
 template <typename T, int CODE, int D, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES) attention_kv8_many_kernel(AttentionArgs a)
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) attention_kv8_many_kernel(AttentionArgs args)
 {
     typedef ManyTile<D> Tile;
     constexpr int THREADS = 64 * WAVES, KEYS = Tile::KEYS, STEPS = D / 16, DT = D / 32;
     constexpr int SIDE_UNITS = KEYS * D / 16, UNITS = 2 * SIDE_UNITS / THREADS;  // 16 codes each; a thread's
-    extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];                   // [2][keys, values]
+    extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];                   // two of keys, two of values
     __shared__ float4 scales[2][KEYS / 16];                                                   // of 16 keys: key scale, value scale's log2 and inverse
+    const AttentionArgs& a = args;
     const Kv8& c = a.cache;
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 32, hf = lane / 32;
     const int kv_head = blockIdx.x % c.kv_heads, part = blockIdx.y, seq = blockIdx.z;
@@ -67,59 +68,62 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_many_kernel(Attentio
 #pragma unroll
         for (int st = 0; st < STEPS; ++st)
             q[st] = valid ? load_row8(p + 2 * (16 * st + 8 * hf), a.wide) : make_uint4(0, 0, 0, 0);
-        float largest = largest_of<T, STEPS>(q);
-        largest = fmaxf(largest, __shfl_xor(largest, 32));
-        const RowScale r = row_scale(largest);
+        uint32_t largest = largest_of<STEPS>(q);
+        largest = max(largest, (uint32_t)__shfl_xor((int)largest, 32));
+        const RowScale r = row_scale<T>(largest);
         cq = r.up * (a.scale * 1.44269504088896341f);
         scale_to_f16<T, STEPS>(q, r.down);
     }
-    // of the wave's rows: keys that any sees, and that every one sees
+    // the keys that every row of the wave sees
     const int wave_row = row0 + 32 * wave, wave_first = place0 + min(wave_row, rows - 1) / a.group, wave_last = place0 + (min(wave_row + 32, rows) - 1) / a.group;
-    const bool working = wave_row < rows;
-    const int any_from = visible_keys(a, wave_first, span.length).x, any_to = working ? visible_keys(a, wave_last, span.length).y : 0;
-    const int every_from = visible_keys(a, wave_last, span.length).x, every_to = working ? visible_keys(a, wave_first, span.length).y : 0;
+    const int every_from = visible_keys(a, wave_last, span.length).x, every_to = visible_keys(a, wave_first, span.length).y;
 
-    // what a thread stages: units of 16 codes; unit u of the tile's: side, key, 16 elements of it
+    // What a thread stages: units of 16 codes; a unit's side, key and 16 elements are the same for every tile.  A wave's units of a kind are keys of
+    // one group of 16, so of one page: its id, scale and address are the scalar unit's work.  Values go one tile behind the keys, as they are used:
+    // stage i is the keys of tile i and the values of tile i - 1.
     const int last_key = max(span.length - 1, 0), slot_mask = (1 << c.page_shift) - 1;
     const int32_t* table = c.table + (int64_t)seq * c.max_pages;
     int ids[UNITS], scale_id = 0;
     uint4 raw[UNITS];
     float2 raw_scale = make_float2(0, 0);
     float unit_scale[UNITS];  // of values: the scale of their page
-    auto unit_key = [&](int u) { return ((tid + u * THREADS) % SIDE_UNITS) / (D / 16); };
-    auto find = [&](int key) {  // page ids of a tile
+    uint32_t source[UNITS], target[UNITS][2];
+    static_assert(SIDE_UNITS % THREADS == 0 || THREADS == 2 * SIDE_UNITS, "a unit is keys or values for all waves, or for half of them");
+    auto is_value = [&](int u) { return SIDE_UNITS < THREADS ? wave >= WAVES / 2 : u * THREADS >= SIDE_UNITS; };
+    const int wave_key = wave % (SIDE_UNITS < THREADS ? WAVES / 2 : WAVES) * (1024 / D);
+    auto unit_key = [&](int u, int stage) { return begin + (stage - (is_value(u) ? 1 : 0)) * KEYS + u * THREADS % SIDE_UNITS / (D / 16) + wave_key; };
+#pragma unroll
+    for (int u = 0; u < UNITS; ++u) {
+        const int k = (tid + u * THREADS) % SIDE_UNITS / (D / 16), chunk = lane % (D / 16) * 2;
+        source[u] = (uint32_t)(lane / (D / 16)) * (uint32_t)(is_value(u) ? c.v.token : c.k.token) + lane % (D / 16) * 16;
+        target[u][0] = is_value(u) ? Tile::value_at(k, chunk / 2) : Tile::key_at(k, chunk);
+        target[u][1] = is_value(u) ? Tile::value_at(k, chunk / 2) + 16 : Tile::key_at(k, chunk + 1);
+    }
+    auto find = [&](int stage) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u)
-            ids[u] = table[min(key + unit_key(u), last_key) >> c.page_shift];
-        if (tid < KEYS / 16)
-            scale_id = table[min(key + 16 * tid, last_key) >> c.page_shift];
+            ids[u] = load_uniform(table + (min(max(unit_key(u, stage), 0), last_key) >> c.page_shift));
     };
-    auto fetch = [&](int key) {
+    auto fetch = [&](int stage) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            const Kv8Side side = (tid + u * THREADS) / SIDE_UNITS ? c.v : c.k;
-            const int64_t page = (unsigned)ids[u] < (unsigned)c.pages ? ids[u] : 0;
-            const int slot = min(key + unit_key(u), last_key) & slot_mask;
-            unit_scale[u] = side.scales[page * c.kv_heads + kv_head];
-            raw[u] = *reinterpret_cast<const uint4*>(side.codes + page * side.page + kv_head * side.head + slot * side.token + (tid + u * THREADS) % (D / 16) * 16);
-        }
-        if (tid < KEYS / 16) {
-            const bool known = (unsigned)scale_id < (unsigned)c.pages;
-            const int64_t at = (int64_t)(known ? scale_id : 0) * c.kv_heads + kv_head;
-            raw_scale = make_float2(known ? c.k.scales[at] : NAN, known ? c.v.scales[at] : NAN);
+            const Kv8Side& side = is_value(u) ? c.v : c.k;
+            const uint32_t page = (unsigned)ids[u] < (unsigned)c.pages ? ids[u] : 0, slot = unit_key(u, stage) & slot_mask;
+            const uint8_t* at = side.codes + ((uint64_t)page * (uint32_t)(side.page >> 3) * 8 + kv_head * side.head + slot * (uint32_t)side.token);
+            raw[u] = *reinterpret_cast<const uint4*>(at + source[u]);
+            unit_scale[u] = side.scales[page * (uint32_t)c.kv_heads + kv_head];
         }
     };
-    auto stage = [&](int key, int buffer) {
-        uint8_t* to_tile = tiles + buffer * 2 * Tile::BYTES;
+    auto stage = [&](int stage) __attribute__((always_inline)) {
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            const bool value = (tid + u * THREADS) / SIDE_UNITS;
-            const int k = unit_key(u), chunk = (tid + u * THREADS) % (D / 16) * 2;
             uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
-            if (value && (key + k < from || key + k >= to || unit_scale[u] < LEAST_SCALE)) {  // a weight of zero does not undo a NaN code that no row sees
+            if (is_value(u)) {  // a weight of zero does not undo a NaN code that no row sees
+                const int own = unit_key(u, stage) + lane / (D / 16);
+                const bool seen_by_some = own >= from && own < to && !(unit_scale[u] < LEAST_SCALE);
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    w[i] = 0u;
+                    w[i] = seen_by_some ? w[i] : 0u;
             }
             uint32_t f[8];
 #pragma unroll
@@ -128,14 +132,20 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_many_kernel(Attentio
                 f[2 * i] = kv8_pair_to_f16<CODE, false>(x);
                 f[2 * i + 1] = kv8_pair_to_f16<CODE, true>(x);
             }
-            uint4* at0 = reinterpret_cast<uint4*>(value ? to_tile + Tile::BYTES + Tile::value_at(k, chunk / 2) : to_tile + Tile::key_at(k, chunk));
-            uint4* at1 = reinterpret_cast<uint4*>(value ? to_tile + Tile::BYTES + Tile::value_at(k, chunk / 2) + 16 : to_tile + Tile::key_at(k, chunk + 1));
-            *at0 = make_uint4(f[0], f[1], f[2], f[3]);
-            *at1 = make_uint4(f[4], f[5], f[6], f[7]);
+            uint8_t* to_tile = tiles + (is_value(u) ? 2 + ((stage - 1) & 1) : stage & 1) * Tile::BYTES;
+            *reinterpret_cast<uint4*>(to_tile + target[u][0]) = make_uint4(f[0], f[1], f[2], f[3]);
+            *reinterpret_cast<uint4*>(to_tile + target[u][1]) = make_uint4(f[4], f[5], f[6], f[7]);
         }
+    };
+    // the scales of 16 keys each, by the first lanes of the first wave: a tile's are read two turns ahead and written one ahead
+    auto stage_scales = [&](int stage) {
         if (tid < KEYS / 16) {
             const ValueScale v = value_scale(raw_scale.y);
-            scales[buffer][tid] = make_float4(raw_scale.x, v.log2, v.inverse, 0.0f);
+            scales[stage & 1][tid] = make_float4(raw_scale.x, v.log2, v.inverse, 0.0f);
+            const bool known = (unsigned)scale_id < (unsigned)c.pages;
+            const uint32_t at = (known ? scale_id : 0) * (uint32_t)c.kv_heads + kv_head;
+            raw_scale = make_float2(known ? c.k.scales[at] : NAN, known ? c.v.scales[at] : NAN);
+            scale_id = table[min(begin + (stage + 2) * KEYS + 16 * tid, last_key) >> c.page_shift];
         }
     };
 
@@ -147,30 +157,79 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_many_kernel(Attentio
         for (int i = 0; i < 16; ++i)
             o[m][i] = 0.0f;
 
-    auto compute = [&](int key, int buffer) {
-        const uint8_t* keys = tiles + buffer * 2 * Tile::BYTES;
-        const uint8_t* values = keys + Tile::BYTES;
-        f32x16 s[KEYS / 32];
+    f32x16 s[KEYS / 32];
+    uint4 p[KEYS / 16];  // the weights of 16 keys, 8 of them this lane's
 #pragma unroll
-        for (int kt = 0; kt < KEYS / 32; ++kt) {
+    for (int x = 0; x < KEYS / 16; ++x)
+        p[x] = make_uint4(0, 0, 0, 0);
+    // the matrix part of turn `tile`: the sums of the tile before, the scores of this one
+    constexpr int PV = KEYS / 16 * DT, QK = KEYS / 32 * STEPS;  // their products
+    auto add_values = [&](int tile) __attribute__((always_inline)) {
+        const uint8_t* values = tiles + (2 + (tile & 1)) * Tile::BYTES;
+#pragma unroll
+        for (int x = 0; x < KEYS / 16; ++x)
+#pragma unroll
+            for (int m = 0; m < DT; ++m) {
+                // a group of 16 lanes: four keys of 16 elements; each lane names 8 bytes and gets its own element of the four
+                const int l16 = lane % 16, k = 16 * x + 4 * hf + l16 / 4, piece = 2 * m + (lane / 16) % 2;
+                const uint4 f = read_transposed_16(values + Tile::value_at(k, piece) + l16 % 4 * 8, values + Tile::value_at(k + 8, piece) + l16 % 4 * 8);
+                o[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f), __builtin_bit_cast(f16x8, p[x]), o[m], 0, 0, 0);
+            }
+    };
+    auto score = [&](int tile) __attribute__((always_inline)) {
+        const uint8_t* keys = tiles + (tile & 1) * Tile::BYTES;
+#pragma unroll
+        for (int kt = 0; kt < KEYS / 32; ++kt)
 #pragma unroll
             for (int i = 0; i < 16; ++i)
                 s[kt][i] = 0.0f;
 #pragma unroll
-            for (int st = 0; st < STEPS; ++st) {
+        for (int st = 0; st < STEPS; ++st) {
+#pragma unroll
+            for (int kt = 0; kt < KEYS / 32; ++kt) {
                 const uint4 f = *reinterpret_cast<const uint4*>(keys + Tile::key_at(32 * kt + col, 2 * st + hf));
                 s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f), __builtin_bit_cast(f16x8, q[st]), s[kt], 0, 0, 0);
             }
         }
+    };
+    // In between the matrix instructions, which a SIMD has 32 clocks for and a wave issues in 4: what is staged.  Fragments are read AHEAD products
+    // before theirs (by itself the compiler reads each right before it is used).
+    constexpr int AHEAD = 4, MFMA = 0x008, DS_READ = 0x100, VALU = 0x002;
+    auto multiply = [&](int tile) __attribute__((always_inline)) {
+        add_values(tile - 1);  // (before the first tile: weights and values of zero)
+        score(tile);
+        stage(tile + 1);
+        fetch(tile + 2);
+        if constexpr (D < 256) {  // (heads of 256 have no registers for it)
+            __builtin_amdgcn_sched_group_barrier(DS_READ, 2 * AHEAD, 0);
+            static_for<PV - AHEAD>([&](auto) __attribute__((always_inline)) {
+                __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(DS_READ, 2, 0);
+                __builtin_amdgcn_sched_group_barrier(VALU, 4, 0);
+            });
+            static_for<QK>([&](auto) __attribute__((always_inline)) {
+                __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(VALU, 4, 0);
+            });
+            __builtin_amdgcn_sched_group_barrier(MFMA, AHEAD, 0);
+        }
+    };
+    // the vector part: scores to weights
+    auto weigh = [&](int tile) __attribute__((always_inline)) {
+        const int key = begin + tile * KEYS, buffer = tile & 1;
         const bool whole = key >= every_from && key + KEYS <= every_to;
         float4 sc[KEYS / 16];  // of 16 keys, 8 of them this lane's
         float scale[KEYS / 16], high = -INFINITY;
+        const uint32_t first = (uint32_t)(key + 4 * hf - seen.x), visible = (uint32_t)(seen.y - seen.x);
         // (the largest of a group's scores times its scale: the scale is not negative)
 #pragma unroll
         for (int x = 0; x < KEYS / 16; ++x) {
             sc[x] = scales[buffer][x];
             scale[x] = cq * sc[x].x;
         }
+        find(tile + 3);
+        stage_scales(tile + 1);
         if (whole) {
 #pragma unroll
             for (int x = 0; x < KEYS / 16; ++x) {
@@ -181,21 +240,16 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_many_kernel(Attentio
                 high = fmaxf(high, fmaf(eight, scale[x], sc[x].y));
             }
         } else {
-            const uint32_t first = (uint32_t)(key + 4 * hf - seen.x), count = (uint32_t)(seen.y - seen.x);
 #pragma unroll
             for (int x = 0; x < KEYS / 16; ++x)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float w = fmaf(s[x / 2][8 * (x % 2) + i], scale[x], sc[x].y);
-                    s[x / 2][8 * (x % 2) + i] = first + (16 * x + 8 * (i / 4) + i % 4) < count ? w : -INFINITY;
-                    high = fmaxf(high, s[x / 2][8 * (x % 2) + i]);
+                    high = fmaxf(high, first + (16 * x + 8 * (i / 4) + i % 4) < visible ? w : -INFINITY);
                 }
-#pragma unroll
-            for (int x = 0; x < KEYS / 16; ++x) {  // (these are scores already)
-                scale[x] = 1.0f;
-                sc[x].y = 0.0f;
-            }
         }
+        uint32_t first_again = first;  // (or the compiler keeps all 32 comparisons, 64 scalar registers)
+        asm("" : "+v"(first_again));
         if (__ballot(high > top + MOST) != 0) {
             high = fmaxf(high, __shfl_xor(high, 32));
             const float next = fmaxf(top, high - SET_TO), fade = __builtin_amdgcn_exp2f(top - next);
@@ -209,81 +263,97 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_many_kernel(Attentio
         }
 #pragma unroll
         for (int x = 0; x < KEYS / 16; ++x) {
-            float w[8], eight = 0.0f;
+            float w[8], eight;
             const float less = sc[x].y - top;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 w[i] = __builtin_amdgcn_exp2f(fmaf(s[x / 2][8 * (x % 2) + i], scale[x], less));
-                eight += w[i];
             }
-            sum = eight == 0.0f ? sum : fmaf(eight, sc[x].z, sum);  // (a NaN scale that the row does not see)
-            const uint4 p = make_uint4(pack_f16(w[0], w[1]), pack_f16(w[2], w[3]), pack_f16(w[4], w[5]), pack_f16(w[6], w[7]));
+            if (!whole) {
 #pragma unroll
-            for (int m = 0; m < DT; ++m) {
-                // a group of 16 lanes: four keys of 16 elements; each lane names 8 bytes and gets its own element of the four
-                const int l16 = lane % 16, k = 16 * x + 4 * hf + l16 / 4, piece = 2 * m + (lane / 16) % 2;
-                const uint4 f = read_transposed_16(values + Tile::value_at(k, piece) + l16 % 4 * 8, values + Tile::value_at(k + 8, piece) + l16 % 4 * 8);
-                o[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f), __builtin_bit_cast(f16x8, p), o[m], 0, 0, 0);
+                for (int i = 0; i < 8; ++i)
+                    w[i] = first_again + (16 * x + 8 * (i / 4) + i % 4) < visible ? w[i] : 0.0f;
             }
+            eight = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+            sum = eight == 0.0f ? sum : fmaf(eight, sc[x].z, sum);  // (a NaN scale that the row does not see)
+            p[x] = make_uint4(pack_f16(w[0], w[1]), pack_f16(w[2], w[3]), pack_f16(w[4], w[5]), pack_f16(w[6], w[7]));
         }
     };
 
-    if (begin < end) {
-        find(begin);
-        fetch(begin);
-        find(begin + KEYS);
-        stage(begin, 0);
+    // Where there are two waves a SIMD, the second four go one segment behind the first: one wave of a SIMD multiplies while the other weighs.  Keys
+    // and values have two buffers each; what multiply(j) writes, stage j + 1, was last read in multiply(j - 1), the segment before at the latest,
+    // and is next read in multiply(j + 1), the segment after at the earliest.
+    const int count = begin < end ? (end - begin + KEYS - 1) / KEYS : 0;
+    const bool behind = WAVES == 8 && wave >= 4;
+    if (count > 0) {
+        find(0);
+        fetch(0);
+        if (tid < KEYS / 16)
+            scale_id = table[min(begin + 16 * tid, last_key) >> c.page_shift];
+        stage(0);
+        find(1);
+        fetch(1);
+        find(2);
+        stage_scales(-1);  // (tile 0's are read here; what is written is written again)
+        stage_scales(0);
         __syncthreads();
-        int buffer = 0;
-        for (int key = begin; key < end; key += KEYS, buffer ^= 1) {
-            if (key + KEYS < end) {
-                fetch(key + KEYS);
-                find(key + 2 * KEYS);
-            }
-            if (key < any_to && key + KEYS > any_from)
-                compute(key, buffer);
-            if (key + KEYS < end)
-                stage(key + KEYS, buffer ^ 1);
+        if (behind)
+            __syncthreads();
+        for (int tile = 0; tile <= count; ++tile) {
+            multiply(tile);
+            if (WAVES == 8)
+                __syncthreads();
+            if (tile < count)
+                weigh(tile);
             __syncthreads();
         }
+        if (WAVES == 8 && !behind)
+            __syncthreads();
     }
 
     sum += __shfl_xor(sum, 32);
-    if (!valid)
-        return;
-    const int64_t at = (int64_t)(span.first + token) * a.heads + head;
-    if (a.splits > 1) {
-        float* out = a.part_out + ((int64_t)part * c.tokens * a.heads + at) * D + 4 * hf;
-#pragma unroll
-        for (int m = 0; m < DT; ++m)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4)
-                *reinterpret_cast<f32x4*>(out + 32 * m + 2 * i) = f32x4{o[m][i], o[m][i + 1], o[m][i + 2], o[m][i + 3]};
-        if (hf == 0)
-            a.part_sum[(int64_t)part * c.tokens * a.heads + at] = make_float2(top, sum);
-        return;
+    const ArgumentsAgain e;
+    const int splits = ARGUMENT(e, splits);
+    const int64_t part_row = (int64_t)part * c.tokens * a.heads;
+    if (valid && hf == 0) {
+        const int64_t at = (int64_t)(span.first + token) * a.heads + head;
+        float* lse = e.global<float>(offsetof(AttentionArgs, lse));
+        if (splits > 1)
+            e.global<float2>(offsetof(AttentionArgs, part_sum))[part_row + at] = make_float2(top, sum);
+        else if (lse != nullptr)
+            lse[at] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
     }
-    const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
-    T* out = reinterpret_cast<T*>(a.out + (int64_t)(span.first + token) * a.out_token + (int64_t)head * a.out_head) + 4 * hf;
-    struct alignas(8) Four { T e[4]; };
+    // A lane's elements are four in a row here and there: 32 of every row at a time go through LDS, where the tiles were (behind the last barrier
+    // nobody reads those), so that two lanes have a row's and store 16 each.
+    const float inverse = splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    uint8_t* mine = tiles + wave * 4096;
+    static_assert(WAVES * 4096 <= 4 * Tile::BYTES, "a wave's rows of 32 f32 lie in the tiles' room");
+    const int own = lane / 2, own_row = row0 + 32 * wave + own, own_token = own_row / a.group, own_head = kv_head * a.group + own_row - own_token * a.group;
+    float* part_out = e.global<float>(offsetof(AttentionArgs, part_out)) + (part_row + (int64_t)(span.first + own_token) * a.heads + own_head) * D + 16 * (lane % 2);
+    uint8_t* out = e.global<uint8_t>(offsetof(AttentionArgs, out)) + (int64_t)(span.first + own_token) * ARGUMENT(e, out_token) + (int64_t)own_head * ARGUMENT(e, out_head) + 32 * (lane % 2);
+    const bool wide = ARGUMENT(e, wide);
 #pragma unroll
-    for (int m = 0; m < DT; ++m)
+    for (int m = 0; m < DT; ++m) {
 #pragma unroll
-        for (int i = 0; i < 16; i += 4) {
-            Four x;
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<f32x4*>(mine + col * 128 + ((2 * i + hf) ^ (col & 7)) * 16) =
+                f32x4{o[m][4 * i] * inverse, o[m][4 * i + 1] * inverse, o[m][4 * i + 2] * inverse, o[m][4 * i + 3] * inverse};
+        f32x4 x[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                x.e[j] = (T)(sum == 0.0f ? 0.0f : o[m][i + j] * inverse);
-            if (a.wide) {
-                *reinterpret_cast<Four*>(out + 32 * m + 2 * i) = x;
-            } else {
+        for (int i = 0; i < 4; ++i)
+            x[i] = *reinterpret_cast<const f32x4*>(mine + own * 128 + ((4 * (lane % 2) + i) ^ (own & 7)) * 16);
+        if (own_row >= rows)
+            continue;
+        if (splits > 1) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    out[32 * m + 2 * i + j] = x.e[j];
-            }
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<f32x4*>(part_out + 32 * m + 4 * i) = x[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                store_row8<T>(out + 64 * m + 16 * i, wide, reinterpret_cast<const float*>(&x[2 * i]));
         }
-    if (a.lse != nullptr && hf == 0)
-        a.lse[at] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
+    }
 }
 
 template <typename T, int CODE, int D, int WAVES>

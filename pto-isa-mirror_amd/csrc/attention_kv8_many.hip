@@ -87,7 +87,8 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
     uint4 raw[UNITS];
     float2 raw_scale = make_float2(0, 0);
     float unit_scale[UNITS];  // of values: the scale of their page
-    uint32_t source[UNITS], target[UNITS][2];
+    uint32_t source[UNITS], target[UNITS][2], none = 0;
+    asm("" : "+v"(none));  // (a vector register's zero: a scale that is not read through the scalar cache, for which a barrier would wait)
     static_assert(SIDE_UNITS % THREADS == 0 || THREADS == 2 * SIDE_UNITS, "a unit is keys or values for all waves, or for half of them");
     auto is_value = [&](int u) { return SIDE_UNITS < THREADS ? wave >= WAVES / 2 : u * THREADS >= SIDE_UNITS; };
     const int wave_key = wave % (SIDE_UNITS < THREADS ? WAVES / 2 : WAVES) * (1024 / D);
@@ -104,39 +105,40 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         for (int u = 0; u < UNITS; ++u)
             ids[u] = load_uniform(table + (min(max(unit_key(u, stage), 0), last_key) >> c.page_shift));
     };
-    auto fetch = [&](int stage) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            const Kv8Side& side = is_value(u) ? c.v : c.k;
-            const uint32_t page = (unsigned)ids[u] < (unsigned)c.pages ? ids[u] : 0, slot = unit_key(u, stage) & slot_mask;
-            const uint8_t* at = side.codes + ((uint64_t)page * (uint32_t)(side.page >> 3) * 8 + kv_head * side.head + slot * (uint32_t)side.token);
-            raw[u] = *reinterpret_cast<const uint4*>(at + source[u]);
-            unit_scale[u] = side.scales[page * (uint32_t)c.kv_heads + kv_head];
-        }
+    auto fetch = [&](int u, int stage) __attribute__((always_inline)) {
+        const Kv8Side& side = is_value(u) ? c.v : c.k;
+        const uint32_t page = (unsigned)ids[u] < (unsigned)c.pages ? ids[u] : 0, slot = unit_key(u, stage) & slot_mask;
+        const uint8_t* at = side.codes + ((uint64_t)page * (uint32_t)(side.page >> 3) * 8 + kv_head * side.head + slot * (uint32_t)side.token);
+        raw[u] = *reinterpret_cast<const uint4*>(at + source[u]);
+        unit_scale[u] = side.scales[page * (uint32_t)c.kv_heads + kv_head + none];
     };
-    auto stage = [&](int stage) __attribute__((always_inline)) {
-#pragma unroll
-        for (int u = 0; u < UNITS; ++u) {
-            uint32_t w[4] = {raw[u].x, raw[u].y, raw[u].z, raw[u].w};
+    // the seven pieces of a unit's way from codes to LDS, and the eighth that reads the next one
+    constexpr int PIECES = 8;
+    uint32_t staged[8];
+    auto piece = [&](auto u_, auto piece_, int stage) __attribute__((always_inline)) {
+        constexpr int u = decltype(u_)::value, which = decltype(piece_)::value;
+        if constexpr (which == 0) {
             if (is_value(u)) {  // a weight of zero does not undo a NaN code that no row sees
                 const int own = unit_key(u, stage) + lane / (D / 16);
-                const bool seen_by_some = own >= from && own < to && !(unit_scale[u] < LEAST_SCALE);
-#pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    w[i] = seen_by_some ? w[i] : 0u;
+                const bool seen_by_some = (own >= from) & (own < to) & !(unit_scale[u] < LEAST_SCALE);
+                raw[u].x = seen_by_some ? raw[u].x : 0u;
+                raw[u].y = seen_by_some ? raw[u].y : 0u;
+                raw[u].z = seen_by_some ? raw[u].z : 0u;
+                raw[u].w = seen_by_some ? raw[u].w : 0u;
             }
-            uint32_t f[8];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t x = kv8_turn<CODE>(w[i]);
-                f[2 * i] = kv8_pair_to_f16<CODE, false>(x);
-                f[2 * i + 1] = kv8_pair_to_f16<CODE, true>(x);
-            }
+        } else if constexpr (which < 5) {
+            const uint32_t x = kv8_turn<CODE>(which == 1 ? raw[u].x : which == 2 ? raw[u].y : which == 3 ? raw[u].z : raw[u].w);
+            staged[2 * which - 2] = kv8_pair_to_f16<CODE, false>(x);
+            staged[2 * which - 1] = kv8_pair_to_f16<CODE, true>(x);
+        } else if constexpr (which < 7) {
             uint8_t* to_tile = tiles + (is_value(u) ? 2 + ((stage - 1) & 1) : stage & 1) * Tile::BYTES;
-            *reinterpret_cast<uint4*>(to_tile + target[u][0]) = make_uint4(f[0], f[1], f[2], f[3]);
-            *reinterpret_cast<uint4*>(to_tile + target[u][1]) = make_uint4(f[4], f[5], f[6], f[7]);
+            *reinterpret_cast<uint4*>(to_tile + target[u][which - 5]) =
+                make_uint4(staged[4 * (which - 5)], staged[4 * (which - 5) + 1], staged[4 * (which - 5) + 2], staged[4 * (which - 5) + 3]);
+        } else {
+            fetch(u, stage + 1);
         }
     };
+
     // the scales of 16 keys each, by the first lanes of the first wave: a tile's are read two turns ahead and written one ahead
     auto stage_scales = [&](int stage) {
         if (tid < KEYS / 16) {
@@ -162,58 +164,46 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
     for (int x = 0; x < KEYS / 16; ++x)
         p[x] = make_uint4(0, 0, 0, 0);
-    // the matrix part of turn `tile`: the sums of the tile before, the scores of this one
-    constexpr int PV = KEYS / 16 * DT, QK = KEYS / 32 * STEPS;  // their products
-    auto add_values = [&](int tile) __attribute__((always_inline)) {
-        const uint8_t* values = tiles + (2 + (tile & 1)) * Tile::BYTES;
-#pragma unroll
-        for (int x = 0; x < KEYS / 16; ++x)
-#pragma unroll
-            for (int m = 0; m < DT; ++m) {
-                // a group of 16 lanes: four keys of 16 elements; each lane names 8 bytes and gets its own element of the four
-                const int l16 = lane % 16, k = 16 * x + 4 * hf + l16 / 4, piece = 2 * m + (lane / 16) % 2;
-                const uint4 f = read_transposed_16(values + Tile::value_at(k, piece) + l16 % 4 * 8, values + Tile::value_at(k + 8, piece) + l16 % 4 * 8);
-                o[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f), __builtin_bit_cast(f16x8, p[x]), o[m], 0, 0, 0);
-            }
-    };
-    auto score = [&](int tile) __attribute__((always_inline)) {
-        const uint8_t* keys = tiles + (tile & 1) * Tile::BYTES;
-#pragma unroll
-        for (int kt = 0; kt < KEYS / 32; ++kt)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                s[kt][i] = 0.0f;
-#pragma unroll
-        for (int st = 0; st < STEPS; ++st) {
-#pragma unroll
-            for (int kt = 0; kt < KEYS / 32; ++kt) {
-                const uint4 f = *reinterpret_cast<const uint4*>(keys + Tile::key_at(32 * kt + col, 2 * st + hf));
-                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, f), __builtin_bit_cast(f16x8, q[st]), s[kt], 0, 0, 0);
-            }
-        }
-    };
-    // In between the matrix instructions, which a SIMD has 32 clocks for and a wave issues in 4: what is staged.  Fragments are read AHEAD products
-    // before theirs (by itself the compiler reads each right before it is used).
-    constexpr int AHEAD = 4, MFMA = 0x008, DS_READ = 0x100, VALU = 0x002;
+    // The matrix part of turn `tile`: the sums of the tile before, the scores of this one.  A SIMD has 32 clocks for a product that a wave issues in
+    // four: in between go the reads of the fragment AHEAD products on, and a piece of the staging.  (The order is fixed by barriers for the
+    // compiler, which would by itself read each fragment right before it is used.)
+    constexpr int PV = KEYS / 16 * DT, QK = KEYS / 32 * STEPS, AHEAD = 4;
     auto multiply = [&](int tile) __attribute__((always_inline)) {
-        add_values(tile - 1);  // (before the first tile: weights and values of zero)
-        score(tile);
-        stage(tile + 1);
-        fetch(tile + 2);
-        if constexpr (D < 256) {  // (heads of 256 have no registers for it)
-            __builtin_amdgcn_sched_group_barrier(DS_READ, 2 * AHEAD, 0);
-            static_for<PV - AHEAD>([&](auto) __attribute__((always_inline)) {
-                __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(DS_READ, 2, 0);
-                __builtin_amdgcn_sched_group_barrier(VALU, 4, 0);
+        const uint8_t* values = tiles + (2 + ((tile - 1) & 1)) * Tile::BYTES;
+        const uint8_t* keys = tiles + (tile & 1) * Tile::BYTES;
+        uint4 fragments[AHEAD];
+        auto read = [&](auto i_) __attribute__((always_inline)) {
+            constexpr int i = decltype(i_)::value;
+            if constexpr (i < PV) {
+                // a group of 16 lanes: four keys of 16 elements; each lane names 8 bytes and gets its own element of the four
+                constexpr int x = i / DT, m = i % DT;
+                const int l16 = lane % 16, k = 16 * x + 4 * hf + l16 / 4, part = 2 * m + (lane / 16) % 2;
+                fragments[i % AHEAD] = read_transposed_16(values + Tile::value_at(k, part) + l16 % 4 * 8, values + Tile::value_at(k + 8, part) + l16 % 4 * 8);
+            } else if constexpr (i < PV + QK) {
+                constexpr int st = (i - PV) / (KEYS / 32), kt = (i - PV) % (KEYS / 32);
+                fragments[i % AHEAD] = *reinterpret_cast<const uint4*>(keys + Tile::key_at(32 * kt + col, 2 * st + hf));
+            }
+        };
+        static_for<AHEAD>(read);
+        __builtin_amdgcn_sched_barrier(0);
+        static_for<PV + QK>([&](auto i_) __attribute__((always_inline)) {
+            constexpr int i = decltype(i_)::value;
+            const f16x8 f = __builtin_bit_cast(f16x8, fragments[i % AHEAD]);
+            if constexpr (i < PV) {
+                constexpr int x = i / DT, m = i % DT;  // (before the first tile: weights and values of zero)
+                o[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, __builtin_bit_cast(f16x8, p[x]), o[m], 0, 0, 0);
+            } else {
+                constexpr int st = (i - PV) / (KEYS / 32), kt = (i - PV) % (KEYS / 32);
+                const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, __builtin_bit_cast(f16x8, q[st]), st == 0 ? zero : s[kt], 0, 0, 0);
+            }
+            read(std::integral_constant<int, i + AHEAD>{});
+            static_for<(i + 1) * UNITS * PIECES / (PV + QK) - i * UNITS * PIECES / (PV + QK)>([&](auto n_) __attribute__((always_inline)) {
+                constexpr int n = i * UNITS * PIECES / (PV + QK) + decltype(n_)::value;
+                piece(std::integral_constant<int, n / PIECES>{}, std::integral_constant<int, n % PIECES>{}, tile + 1);
             });
-            static_for<QK>([&](auto) __attribute__((always_inline)) {
-                __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(DS_READ, 1, 0);
-                __builtin_amdgcn_sched_group_barrier(VALU, 4, 0);
-            });
-            __builtin_amdgcn_sched_group_barrier(MFMA, AHEAD, 0);
-        }
+            __builtin_amdgcn_sched_barrier(0);
+        });
     };
     // the vector part: scores to weights
     auto weigh = [&](int tile) __attribute__((always_inline)) {
@@ -287,12 +277,16 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
     const bool behind = WAVES == 8 && wave >= 4;
     if (count > 0) {
         find(0);
-        fetch(0);
+#pragma unroll
+        for (int u = 0; u < UNITS; ++u)
+            fetch(u, 0);
         if (tid < KEYS / 16)
             scale_id = table[min(begin + 16 * tid, last_key) >> c.page_shift];
-        stage(0);
         find(1);
-        fetch(1);
+        static_for<UNITS * PIECES>([&](auto n_) __attribute__((always_inline)) {
+            constexpr int n = decltype(n_)::value;
+            piece(std::integral_constant<int, n / PIECES>{}, std::integral_constant<int, n % PIECES>{}, 0);
+        });
         find(2);
         stage_scales(-1);  // (tile 0's are read here; what is written is written again)
         stage_scales(0);
@@ -300,9 +294,13 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         if (behind)
             __syncthreads();
         for (int tile = 0; tile <= count; ++tile) {
-            multiply(tile);
             if (WAVES == 8)
+                __builtin_amdgcn_s_setprio(1);  // (ahead of the SIMD's other wave, whatever its age)
+            multiply(tile);
+            if (WAVES == 8) {
+                __builtin_amdgcn_s_setprio(0);
                 __syncthreads();
+            }
             if (tile < count)
                 weigh(tile);
             __syncthreads();

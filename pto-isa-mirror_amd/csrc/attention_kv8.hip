@@ -95,13 +95,17 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 // Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
 // (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
 // heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.
-// Many rows: where they leave CUs without a workgroup, none below 1024 keys.
+// Many rows: where they leave CUs without a workgroup, the number that costs least, none below 1024 keys.  The cost of n parts is the turns that the
+// CUs take, a workgroup each, times a part's keys and 440 more (its start and end: 14 us, 64 keys take 2), and n > 1's join; the host does not
+// know the lengths but the largest, so several sequences count as half full and as full.  32 / 8 heads of 128, us, in 1, 2, 3, 4, 6, 8 parts:
+//   512 tokens over 16384 keys 453, 245, 184, [163], 201, 179; 3 x 512 over 6000 each 175, [210], 217, 199, 236; 421, 376 and 512 over 6104, 4383 and
+//   512 167, [106], 149, 123, 143; 4 x 128 over 8192 220, 133, 104, [97], 124, 115  (chosen in brackets)
 constexpr long FEW_ROWS = 96;
 struct AttentionPlan {
     enum { GENERIC, FEW, MANY } kernel;
     int splits, chunk;
 };
-static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int max_tokens, int max_length, int window)
+static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int tokens, int max_tokens, int max_length, int window)
 {
     AttentionPlan p{AttentionPlan::GENERIC, 1, 0};
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
@@ -127,10 +131,20 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int ma
     } else {
         const int tile = c->head_dim == 256 ? 128 : 256;
         items *= (rows + tile - 1) / tile;
+        // (of the workgroups of max_tokens new tokens each, what the tokens fill)
+        items = (long)((double)items * tokens / ((double)c->sequences * max_tokens) + 0.5);
+        const long fewer = c->sequences > 1 ? items / 2 : items;  // (sequences are of several lengths)
+        const double join = 5.4e-5 * tokens * heads * c->head_dim;
         step = 64;
-        splits = items < cus ? (2 * cus + items - 1) / items : 1;
-        const long most = (keys + 1023) / 1024;
-        splits = splits < most ? splits : most;
+        splits = 1;
+        double least = 0;
+        for (long n = 1; items < cus && n <= (keys + 1023) / 1024; ++n) {
+            const double cost = (double)((items * n + cus - 1) / cus + (fewer * n + cus - 1) / cus) * (440 + (double)keys / n) + (n > 1 ? 2 * (n * join + 150) : 0);
+            if (n == 1 || cost < least) {
+                least = cost;
+                splits = n;
+            }
+        }
     }
     if (splits <= 1)
         return p;
@@ -154,7 +168,7 @@ size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache* cache, int h
     if (cache == nullptr || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads != 0 || tokens <= 0 || max_tokens <= 0 || cache->sequences <= 0 ||
         cache->max_pages <= 0 || cache->page_size <= 0)
         return 0;
-    return part_bytes(plan_attention(cache, heads, max_tokens, max_length, window), heads, tokens, cache->head_dim);
+    return part_bytes(plan_attention(cache, heads, tokens, max_tokens, max_length, window), heads, tokens, cache->head_dim);
 }
 
 int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, const void* q, int type, int heads, int tokens,
@@ -198,7 +212,7 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
     a.scale = scale;
     hipStream_t s = as_stream(stream);
     const bool i8 = cache->code_type == PTOAMD_I8, f16 = type == PTOAMD_F16;
-    const AttentionPlan plan = plan_attention(cache, heads, max_tokens, max_length, window);
+    const AttentionPlan plan = plan_attention(cache, heads, tokens, max_tokens, max_length, window);
     const size_t need = part_bytes(plan, heads, tokens, cache->head_dim);
     PTOAMD_REQUIRE(workspace == nullptr || workspace_bytes >= need, PTOAMD_E_INVALID, "%s: a workspace of %zu bytes is needed (%zu)", what, need, workspace_bytes);
     PTOAMD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, PTOAMD_E_ALIGNMENT, "%s: the workspace must be 16-byte aligned", what);

@@ -76,6 +76,8 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, int seq)
     s.begin = a.window > 0 ? max(s.length - s.count + 1 - a.window, 0) & ~31 : 0;
     return s;
 }
+// Whether a sequence's keys are in several parts, which are joined; else its workgroups write what the call returns.
+__device__ __forceinline__ bool several_parts(const AttentionArgs& a, const Span& s) { return a.splits > 1 && s.length - s.begin > a.chunk; }
 // The keys that a query at `place` of a sequence of `length` tokens sees: [x, y).
 __device__ __forceinline__ int2 visible_keys(const AttentionArgs& a, int place, int length)
 {
@@ -112,6 +114,12 @@ constexpr float KV8_UNIT = CODE == PTOAMD_I8 ? 16777216.0f : 1.0f;
 __device__ __forceinline__ uint32_t bytes_to_f16(uint32_t even, uint32_t odd, int b)
 {
     return __builtin_amdgcn_perm(odd, even, 0x0C000C00u | (uint32_t)b | (uint32_t)(4 + b) << 16);
+}
+// Two codes side by side, of keys whose products start at UNBIAS's: int8 comes turned and stays c + 128, as above.
+template <int CODE, bool HIGH>
+__device__ __forceinline__ uint32_t kv8_key_pair(uint32_t w)
+{
+    return CODE == PTOAMD_I8 ? __builtin_amdgcn_perm(w, w, HIGH ? 0x0C030C02u : 0x0C010C00u) : kv8_pair_to_f16<CODE, HIGH>(w);
 }
 __device__ __forceinline__ uint32_t pack_f16(float a, float b)
 {

@@ -49,6 +49,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
     const int from = visible_keys(a, place0 + row0 / a.group, span.length).x;
     const int to = visible_keys(a, place0 + (min(row0 + 32 * WAVES, rows) - 1) / a.group, span.length).y;
     int begin = from & ~31, end = to;
+    const bool parts = several_parts(a, span);
     if (a.splits > 1) {
         begin = max(begin, span.begin + part * a.chunk);
         if (part + 1 < a.splits)
@@ -71,8 +72,16 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         uint32_t largest = largest_of<STEPS>(q);
         largest = max(largest, (uint32_t)__shfl_xor((int)largest, 32));
         const RowScale r = row_scale<T>(largest);
-        cq = r.up * (a.scale * 1.44269504088896341f);
+        cq = r.up * (a.scale * 1.44269504088896341f) * KV8_UNIT<CODE>;
         scale_to_f16<T, STEPS>(q, r.down);
+    }
+    // where a row's scores start: without the 128 that the keys' int8 codes carry
+    f32x16 start = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+    if (CODE == PTOAMD_I8) {
+        const uint4 unbias = make_uint4(UNBIAS, UNBIAS, UNBIAS, UNBIAS);
+#pragma unroll
+        for (int st = 0; st < STEPS; ++st)
+            start = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, unbias), __builtin_bit_cast(f16x8, q[st]), start, 0, 0, 0);
     }
     // the keys that every row of the wave sees
     const int wave_row = row0 + 32 * wave, wave_first = place0 + min(wave_row, rows - 1) / a.group, wave_last = place0 + (min(wave_row + 32, rows) - 1) / a.group;
@@ -128,8 +137,8 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             }
         } else if constexpr (which < 5) {
             const uint32_t x = kv8_turn<CODE>(which == 1 ? raw[u].x : which == 2 ? raw[u].y : which == 3 ? raw[u].z : raw[u].w);
-            staged[2 * which - 2] = kv8_pair_to_f16<CODE, false>(x);
-            staged[2 * which - 1] = kv8_pair_to_f16<CODE, true>(x);
+            staged[2 * which - 2] = is_value(u) ? kv8_pair_to_f16<CODE, false>(x) : kv8_key_pair<CODE, false>(x);
+            staged[2 * which - 1] = is_value(u) ? kv8_pair_to_f16<CODE, true>(x) : kv8_key_pair<CODE, true>(x);
         } else if constexpr (which < 7) {
             uint8_t* to_tile = tiles + (is_value(u) ? 2 + ((stage - 1) & 1) : stage & 1) * Tile::BYTES;
             *reinterpret_cast<uint4*>(to_tile + target[u][which - 5]) =
@@ -143,7 +152,8 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
     auto stage_scales = [&](int stage) {
         if (tid < KEYS / 16) {
             const ValueScale v = value_scale(raw_scale.y);
-            scales[stage & 1][tid] = make_float4(raw_scale.x, v.log2, v.inverse, 0.0f);
+            // (a NaN scale of a page that a row does not see: its weights are 0, and so is their share of the sum)
+            scales[stage & 1][tid] = make_float4(raw_scale.x, v.log2, isnan(v.inverse) ? 0.0f : v.inverse, 0.0f);
             const bool known = (unsigned)scale_id < (unsigned)c.pages;
             const uint32_t at = (known ? scale_id : 0) * (uint32_t)c.kv_heads + kv_head;
             raw_scale = make_float2(known ? c.k.scales[at] : NAN, known ? c.v.scales[at] : NAN);
@@ -194,8 +204,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
                 o[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, __builtin_bit_cast(f16x8, p[x]), o[m], 0, 0, 0);
             } else {
                 constexpr int st = (i - PV) / (KEYS / 32), kt = (i - PV) % (KEYS / 32);
-                const f32x16 zero = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, __builtin_bit_cast(f16x8, q[st]), st == 0 ? zero : s[kt], 0, 0, 0);
+                s[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f, __builtin_bit_cast(f16x8, q[st]), st == 0 ? start : s[kt], 0, 0, 0);
             }
             read(std::integral_constant<int, i + AHEAD>{});
             static_for<(i + 1) * UNITS * PIECES / (PV + QK) - i * UNITS * PIECES / (PV + QK)>([&](auto n_) __attribute__((always_inline)) {
@@ -264,9 +273,9 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
                 for (int i = 0; i < 8; ++i)
                     w[i] = first_again + (16 * x + 8 * (i / 4) + i % 4) < visible ? w[i] : 0.0f;
             }
-            eight = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
-            sum = eight == 0.0f ? sum : fmaf(eight, sc[x].z, sum);  // (a NaN scale that the row does not see)
             p[x] = make_uint4(pack_f16(w[0], w[1]), pack_f16(w[2], w[3]), pack_f16(w[4], w[5]), pack_f16(w[6], w[7]));
+            eight = ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));  // (before they are rounded: the log-sum keeps f32's bits)
+            sum = fmaf(eight, sc[x].z, sum);
         }
     };
 
@@ -311,19 +320,18 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
 
     sum += __shfl_xor(sum, 32);
     const ArgumentsAgain e;
-    const int splits = ARGUMENT(e, splits);
     const int64_t part_row = (int64_t)part * c.tokens * a.heads;
     if (valid && hf == 0) {
         const int64_t at = (int64_t)(span.first + token) * a.heads + head;
         float* lse = e.global<float>(offsetof(AttentionArgs, lse));
-        if (splits > 1)
+        if (parts)
             e.global<float2>(offsetof(AttentionArgs, part_sum))[part_row + at] = make_float2(top, sum);
         else if (lse != nullptr)
             lse[at] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
     }
     // A lane's elements are four in a row here and there: 32 of every row at a time go through LDS, where the tiles were (behind the last barrier
     // nobody reads those), so that two lanes have a row's and store 16 each.
-    const float inverse = splits > 1 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
+    const float inverse = parts ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
     uint8_t* mine = tiles + wave * 4096;
     static_assert(WAVES * 4096 <= 4 * Tile::BYTES, "a wave's rows of 32 f32 lie in the tiles' room");
     const int own = lane / 2, own_row = row0 + 32 * wave + own, own_token = own_row / a.group, own_head = kv_head * a.group + own_row - own_token * a.group;
@@ -342,7 +350,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             x[i] = *reinterpret_cast<const f32x4*>(mine + own * 128 + ((4 * (lane % 2) + i) ^ (own & 7)) * 16);
         if (own_row >= rows)
             continue;
-        if (splits > 1) {
+        if (parts) {
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 *reinterpret_cast<f32x4*>(part_out + 32 * m + 4 * i) = x[i];

@@ -95,19 +95,20 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 // Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
 // (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
 // heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.
-// Many rows: where they leave CUs without a workgroup, the number that costs least, none below 1024 keys.  The cost of n parts is the turns that the
-// CUs take, a workgroup each, times a part's keys and 440 more (its start and end: 14 us, 64 keys take 2), and n > 1's join; the host does not
-// know the lengths but the largest, so several sequences count as half full and as full.  32 / 8 heads of 128, us, in 1, 2, 3, 4, 6, 8 parts:
-//   512 tokens over 16384 keys 453, 245, 184, [163], 201, 179; 3 x 512 over 6000 each 175, [210], 217, 199, 236; 421, 376 and 512 over 6104, 4383 and
-//   512 167, [106], 149, 123, 143; 4 x 128 over 8192 220, 133, 104, [97], 124, 115  (chosen in brackets)
+// Many rows: in equal stretches (Cuts) where tiles of rows leave CUs without a workgroup, and for several sequences, whose lengths the host does
+// not know, up to two a CU; not where all keys are at most 1024.  32 / 8 heads of 128, us, whole / cut: 512 tokens over 16384 keys 448 / 172; 421, 376
+// and 512 over 6104, 4383 and 512 170 / 106; 3 x 512 over 6000 200 / 192; 200, 512, 30 and 400 over 9000, 1200, 400 and 16000 440 / 213;
+// 2 x 1024 over 8192 268 / 296; 2048 over 2048 71 / 81; 4 x 128 over 8192 229 / 103.  (The same number of parts for every sequence, the
+// best number for each of these calls: 163, 106, 175, 204, 268, 71, 97, but no rule on what the host knows came within 10% of that on average.)
+// Parts have room for a sequence that is the only long one, within 256 MB.
 constexpr long FEW_ROWS = 96;
 struct AttentionPlan {
     enum { GENERIC, FEW, MANY } kernel;
-    int splits, chunk;
+    int splits, chunk, row_tiles;
 };
 static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int tokens, int max_tokens, int max_length, int window)
 {
-    AttentionPlan p{AttentionPlan::GENERIC, 1, 0};
+    AttentionPlan p{AttentionPlan::GENERIC, 1, 0, 0};
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
         return p;
     const long rows = (long)max_tokens * (heads / c->kv_heads);
@@ -118,43 +119,37 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     if (window > 0 && (long)window + max_tokens + 31 < keys)
         keys = (long)window + max_tokens + 31;
     const long cus = device_compute_units();
-    long items = (long)c->sequences * c->kv_heads, splits, step;
+    const long items = (long)c->sequences * c->kv_heads;
     if (p.kernel == AttentionPlan::FEW) {
-        step = 32 * few_waves(c->head_dim, rows);  // the keys that a workgroup's waves have at a time
+        const long step = 32 * few_waves(c->head_dim, rows);  // the keys that a workgroup's waves have at a time
         const long turns = (keys + step - 1) / step;
-        splits = (cus + items - 1) / items;
+        long splits = (cus + items - 1) / items;
         splits = splits < turns / 2 ? splits : turns / 2;
         if (turns <= (c->head_dim == 256 ? 4 : 6))
             splits = 1;
         const long even = (keys + 4095) / 4096;
         splits = splits > even ? splits : even;
-    } else {
-        const int tile = c->head_dim == 256 ? 128 : 256;
-        items *= (rows + tile - 1) / tile;
-        // (of the workgroups of max_tokens new tokens each, what the tokens fill)
-        items = (long)((double)items * tokens / ((double)c->sequences * max_tokens) + 0.5);
-        const long fewer = c->sequences > 1 ? items / 2 : items;  // (sequences are of several lengths)
-        const double join = 5.4e-5 * tokens * heads * c->head_dim;
-        step = 64;
-        splits = 1;
-        double least = 0;
-        for (long n = 1; items < cus && n <= (keys + 1023) / 1024; ++n) {
-            const double cost = (double)((items * n + cus - 1) / cus + (fewer * n + cus - 1) / cus) * (440 + (double)keys / n) + (n > 1 ? 2 * (n * join + 150) : 0);
-            if (n == 1 || cost < least) {
-                least = cost;
-                splits = n;
-            }
+        if (splits > 1) {
+            p.chunk = (int)(((keys + splits - 1) / splits + step - 1) / step * step);
+            p.splits = (int)((keys + p.chunk - 1) / p.chunk);
         }
-    }
-    if (splits <= 1)
         return p;
-    p.chunk = (int)(((keys + splits - 1) / splits + step - 1) / step * step);
-    p.splits = (int)((keys + p.chunk - 1) / p.chunk);
+    }
+    p.row_tiles = (int)((rows + many_rows(c->head_dim) - 1) / many_rows(c->head_dim));
+    const long tiles = p.row_tiles * items;  // of rows, a workgroup's each if no keys are cut
+    const bool countable = (long)p.row_tiles * c->sequences <= Cuts::MOST && (double)tiles * c->max_pages * c->page_size < 1e9;
+    if (countable && keys > 1024 && tiles < (c->sequences > 1 ? 2 * cus : cus)) {
+        const long room = (256L << 20) / ((long)tokens * heads * (c->head_dim * 4 + 8)), least = 2 * cus / tiles + 3;
+        const long most = cus / c->kv_heads + 2;
+        p.splits = (int)(most < least || room < least ? least : most < room ? most : room);
+    }
     return p;
 }
 static size_t part_bytes(const AttentionPlan& p, int heads, int tokens, int head_dim)
 {
-    return p.splits > 1 ? (size_t)p.splits * tokens * heads * (head_dim * sizeof(float) + sizeof(float2)) : 0;
+    if (p.splits <= 1)
+        return 0;
+    return (p.kernel == AttentionPlan::MANY ? Cuts::BYTES : 0) + (size_t)p.splits * tokens * heads * (head_dim * sizeof(float) + sizeof(float2));
 }
 
 }  // namespace ptoamd
@@ -226,7 +221,10 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
         a.wide = ((uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)out | (uint64_t)a.q_token | (uint64_t)a.q_head | (uint64_t)a.out_token | (uint64_t)a.out_head) % 16 == 0;
         a.splits = workspace != nullptr ? plan.splits : 1;
         a.chunk = plan.chunk;
-        a.part_out = static_cast<float*>(workspace);
+        a.row_tiles = plan.row_tiles;
+        a.sequences = cache->sequences;
+        a.cuts = plan.kernel == AttentionPlan::MANY && a.splits > 1 ? static_cast<int*>(workspace) : nullptr;
+        a.part_out = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (a.cuts != nullptr ? Cuts::BYTES : 0));
         a.part_sum = reinterpret_cast<float2*>(a.part_out + (size_t)plan.splits * tokens * heads * cache->head_dim);
         const bool few = plan.kernel == AttentionPlan::FEW;
         const int rc = few ? launch_attention_few(a, cache->code_type, f16, cache->sequences, s) : launch_attention_many(a, cache->code_type, f16, cache->sequences, s);

@@ -18,12 +18,27 @@ struct AttentionArgs {
     int causal, window;
     float scale;
     int wide;  // rows of q and out allow 16-byte accesses
-    // The keys of a sequence in parts of `chunk` tokens, each a workgroup's, where splits > 1: every part leaves its sums of a row (unscaled)
-    // and the row's reference and sum, [split][token][head]; a second kernel joins them in the order of the parts.
-    int splits, chunk;
+    // The keys of a row in parts, where splits > 1 (at most so many): every part leaves its sums of a row (unscaled) and the row's reference and
+    // sum, [split][token][head]; a second kernel joins them in the order of the parts.
+    // Few rows: parts of `chunk` tokens, each a workgroup's.  Many: `cuts`, of the rows in row_tiles tiles a sequence (Cuts).
+    int splits, chunk, row_tiles, sequences;
+    int* cuts;
     float* part_out;
     float2* part_sum;
 };
+
+// Many rows, keys in parts: all (key head, tile of rows, tile of keys) that there are, in this order, in equal stretches, one for a workgroup a CU.
+// What the host does not know, how long the sequences are, is counted by each workgroup at its start.  A tile of rows counts for as many tiles
+// of keys more, before its first, as its start and end cost: 448 keys' (12 to 14 us; 64 keys take 2).
+struct Cuts {
+    static constexpr int MOST = 256;                                       // tiles of rows of all sequences
+    static constexpr int HEAD = 0, STRETCH = 1, FIRST = 2, SIZE = MOST + 3;  // tiles of keys: a key head's, a workgroup's, those before a tile of rows
+    static constexpr size_t BYTES = 2048;
+    static_assert(SIZE * sizeof(int) <= BYTES, "the join finds them at the workspace's start");
+};
+constexpr int many_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }  // a tile's
+constexpr int many_keys(int head_dim) { return head_dim == 256 ? 32 : 64; }
+constexpr int many_start(int head_dim) { return 448 / many_keys(head_dim); }
 
 // The waves of a few-rows workgroup: eight where two fit a SIMD's registers (heads up to 128 elements, 16 rows), else four.
 constexpr int few_waves(int head_dim, long rows) { return head_dim <= 128 && rows <= 16 ? 8 : 4; }
@@ -54,6 +69,10 @@ struct ArgumentsAgain {
     __device__ __forceinline__ T* global(size_t offset) const  // (through an integer the compiler no longer knows what memory)
     {
         return (T*)(__attribute__((address_space(1))) T*)(uintptr_t)field<uint64_t>(offset);
+    }
+    __device__ __forceinline__ const AttentionArgs* all() const
+    {
+        return (const AttentionArgs*)(const __attribute__((address_space(4))) AttentionArgs*)at;
     }
 };
 #define ARGUMENT(again, name) (again).template field<decltype(AttentionArgs::name)>(offsetof(AttentionArgs, name))

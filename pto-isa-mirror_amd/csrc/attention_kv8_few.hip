@@ -368,12 +368,24 @@ __global__ void __launch_bounds__(256) attention_kv8_join_kernel(AttentionArgs a
     const int i = threadIdx.x % LANES, group = threadIdx.x / LANES, seq = blockIdx.z;
     const int row = blockIdx.x * ROWS + (ROWS == 1 ? 0 : group), nth = row / a.heads, head = row - nth * a.heads;  // (rows: tokens times heads)
     const Span span = span_of(a, seq);
-    if (nth >= span.count || !several_parts(a, span))
+    if (nth >= span.count)
         return;
     const int64_t at = (int64_t)(span.first + nth) * a.heads + head, stride = (int64_t)a.cache.tokens * a.heads;
-    const int2 keys = visible_keys(a, span.length - span.count + nth, span.length);
-    const int from = min((keys.x - span.begin) / a.chunk, a.splits - 1);
-    const int to = keys.y > keys.x ? min((keys.y - 1 - span.begin) / a.chunk, a.splits - 1) + 1 : from;
+    int from = 0, to;
+    if (a.cuts != nullptr) {  // (rows of one part are written already)
+        const int kv_head = head / a.group, tile = seq * a.row_tiles + (nth * a.group + head - kv_head * a.group) / many_rows(D);
+        const int stretch = a.cuts[Cuts::STRETCH], first = kv_head * a.cuts[Cuts::HEAD] + a.cuts[Cuts::FIRST + tile] + many_start(D);
+        const int last = kv_head * a.cuts[Cuts::HEAD] + a.cuts[Cuts::FIRST + tile + 1] - 1;
+        to = last / stretch - first / stretch + 1;
+        if (to == 1)
+            return;
+    } else {
+        if (!several_parts(a, span))
+            return;
+        const int2 keys = visible_keys(a, span.length - span.count + nth, span.length);
+        from = min((keys.x - span.begin) / a.chunk, a.splits - 1);
+        to = keys.y > keys.x ? min((keys.y - 1 - span.begin) / a.chunk, a.splits - 1) + 1 : from;
+    }
     float top = NO_REFERENCE, sum = 0.0f;
     float4 o = make_float4(0, 0, 0, 0);
     for (int part = from + (ROWS == 1 ? group : 0); part < to; part += STEP)

@@ -63,6 +63,15 @@ def test_long_sequences_are_split_and_joined(pa, tokens):  # noqa: F811
     run(pa, "i8", [9000, 33], [tokens, min(tokens, 33)], 4, 1, 128, 16, window=700)
 
 
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("kw", [{}, {"causal": False}, {"window": 1500}])
+def test_chunks_over_sequences_of_very_different_lengths(pa, code, dim, kw):  # noqa: F811
+    # keys in equal stretches: tiles of rows cut in many parts, whole ones, some without keys, sequences without rows; queries before the first key
+    run(pa, code, [5104, 0, 130, 3000, 77, 40], [321, 5, 130, 1, 0, 60], 8, 2, dim, 32, **kw)
+    run(pa, code, [20, 12011], [20, 70], 8, 2, dim, 16, dtype=torch.float16, **kw)
+
+
 @pytest.mark.parametrize("tokens", [1, 40])
 def test_without_room_to_split_the_result_is_the_same_to_rounding(pa, tokens):  # noqa: F811
     cache = ref.Cache("i8", [5000, 700], 2, 128, 64, 3)

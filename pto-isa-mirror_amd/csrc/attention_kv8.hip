@@ -152,6 +152,25 @@ static size_t part_bytes(const AttentionPlan& p, int heads, int tokens, int head
     return (p.kernel == AttentionPlan::MANY ? Cuts::BYTES : 0) + (size_t)p.splits * tokens * heads * (head_dim * sizeof(float) + sizeof(float2));
 }
 
+int prepare_attention_kernels()
+{
+    for (int code : {PTOAMD_I8, PTOAMD_E4M3})
+        for (bool f16 : {false, true})
+            for (int dim : {64, 128, 256})
+                for (int rows : {16, 32}) {
+                    AttentionArgs a{};  // (of no heads: nothing is launched)
+                    a.cache.head_dim = dim;
+                    a.cache.max_tokens = rows;
+                    a.group = 1;
+                    int rc = launch_attention_few(a, code, f16, 1, nullptr);
+                    if (rc == PTOAMD_OK)
+                        rc = launch_attention_many(a, code, f16, 1, nullptr);
+                    if (rc != PTOAMD_OK)
+                        return rc;
+                }
+    return PTOAMD_OK;
+}
+
 }  // namespace ptoamd
 
 using namespace ptoamd;

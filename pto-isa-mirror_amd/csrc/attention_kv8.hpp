@@ -45,7 +45,7 @@ constexpr int few_waves(int head_dim, long rows) { return head_dim <= 128 && row
 int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_many(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_join(const AttentionArgs& a, bool f16, int sequences, hipStream_t stream);
-int prepare_attention_kernels();
+int prepare_attention_kernels();  // the launch attributes of all of them, for the current device
 
 // Wave-uniform reads of what no kernel writes (tables, lengths, scales) through the scalar cache.
 template <typename T>

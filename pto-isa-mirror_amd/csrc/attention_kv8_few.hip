@@ -444,6 +444,8 @@ static int launch_few(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
     constexpr int bytes = WAVES / 2 * 16 * NT * (D + 4) * 4;
     PTOAMD_HIP_CHECK((ensure_dynamic_lds<&attention_kv8_few_kernel<T, CODE, D, NT, WAVES>>(bytes)));
+    if (a.heads == 0)  // (prepare_attention_kernels)
+        return PTOAMD_OK;
     const int row_groups = (a.cache.max_tokens * a.group + 16 * NT - 1) / (16 * NT);
     hipLaunchKernelGGL((attention_kv8_few_kernel<T, CODE, D, NT, WAVES>), dim3((unsigned)(a.cache.kv_heads * row_groups), (unsigned)sequences, (unsigned)a.splits),
                        dim3(64 * WAVES), bytes, stream, a);

@@ -455,6 +455,8 @@ static int launch_many(const AttentionArgs& a, int sequences, hipStream_t stream
 {
     constexpr int bytes = 4 * ManyTile<D>::BYTES;
     PTOAMD_HIP_CHECK((ensure_dynamic_lds<&attention_kv8_many_kernel<T, CODE, D, WAVES>>(bytes)));
+    if (a.heads == 0)  // (prepare_attention_kernels)
+        return PTOAMD_OK;
     static_assert(32 * WAVES == many_rows(D), "the tiles of rows that the cuts count");
     const dim3 grid = a.splits > 1 ? dim3(device_compute_units()) : dim3((unsigned)(a.row_tiles * a.cache.kv_heads), (unsigned)sequences);
     hipLaunchKernelGGL((attention_kv8_many_kernel<T, CODE, D, WAVES>), grid, dim3(64 * WAVES), bytes, stream, a);

@@ -12,6 +12,8 @@
 #include "common_host.hpp"
 
 namespace ptoamd {
+
+int prepare_attention_kernels();
 static thread_local char g_error[512] = "";
 static thread_local char g_kernel[64] = "";
 
@@ -254,6 +256,8 @@ int ptoamd_init(int device)
     int rc = prepare_gemm_kernels();
     if (rc == PTOAMD_OK)
         rc = prepare_gemv_kernels();
+    if (rc == PTOAMD_OK)
+        rc = prepare_attention_kernels();
     if (rc == PTOAMD_OK && device < 64)
         prepared[device].store(true, std::memory_order_release);
     return rc;

@@ -95,12 +95,13 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 // Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
 // (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
 // heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.
-// Many rows: in equal stretches (Cuts) where that is less than a tile of rows' keys by more than the second start and the join cost (800 keys; 400
-// of heads of 256); several sequences, whose lengths the host does not know, count as half of the longest.  us, whole / cut, 32 / 8 heads of 128:
+// Many rows: in equal stretches (Cuts) where that is less than a tile of rows' keys by more than the second start and the join cost (800 keys of
+// heads of 128, 1600 of 64, 400 of 256); several sequences, whose lengths the host does not know, count as half of the longest.  us, whole / cut, 32 / 8 heads of 128:
 //   128 tokens over 700, 1024, 1500 keys 30 / 35, 38 / 37, 52 / 39; 512 over 700, 1024, 1500, 2500, 16384 30 / 38, 38 / 42, 52 / 47, 78 / 55, 441 / 174;
 //   1024 over 1500, 2500 53 / 54, 80 / 71; 421, 376 and 512 over 6104, 4383 and 512 170 / 109; 3 x 512 over 6000 181 / 186; 4 x 256 over 1024, 512,
 //   341 and 146 39 / 43, over four times as many 117 / 70; 200, 512, 30 and 400 over 9000, 1200, 400 and 16000 440 / 213; 2 x 1024 over 8192 268 / 296;
-//   4 / 1 heads, 47, 114 and 166 over 8642 234 / 39.  (The same number of parts for every sequence instead, the best for each call: of these 512 over
+//   4 / 1 heads, 47, 114 and 166 over 8642 234 / 39; heads of 64, 4 x 100 over 1024, 2000 33 / 43, 56 / 49; 8 / 2 of 256, over 512, 1024 40 / 39,
+//   68 / 43.  (The same number of parts for every sequence instead, the best for each call: of these 512 over
 //   16384 163, the three of 6104 106, the four of 16000 204; but what the host knows did not tell which number, by a factor of up to 1.7.)
 // Parts have room for a sequence that is the only long one, within 256 MB.
 constexpr long FEW_ROWS = 96;
@@ -141,10 +142,12 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     const long tiles = p.row_tiles * items;  // of rows, a workgroup's each if no keys are cut
     const bool countable = (long)p.row_tiles * c->sequences <= Cuts::MOST && (double)tiles * c->max_pages * c->page_size < 1e9;
     const double full = (double)tiles / cus / (c->sequences > 1 ? 2 : 1);
-    if (countable && keys * (1 - full) > 448 * full + (c->head_dim == 256 ? 400 : 800)) {
-        const long room = (256L << 20) / ((long)tokens * heads * (c->head_dim * 4 + 8)), least = 2 * cus / tiles + 3;
-        const long most = cus / c->kv_heads + 2;
-        p.splits = (int)(most < least || room < least ? least : most < room ? most : room);
+    if (countable && keys * (1 - full) > 448 * full + 102400.0 / c->head_dim) {
+        // (a tile's parts: its keys, at most twice the mean of one sequence's, in stretches of the mean; of several up to all stretches of a key head)
+        const long mean = 2 * cus / tiles + 3, most = c->sequences > 1 ? cus / c->kv_heads + 2 : mean;
+        const long room = (256L << 20) / ((long)tokens * heads * (c->head_dim * 4 + 8));
+        const long parts = most < room ? most : room;
+        p.splits = (int)(parts > mean ? parts : mean);
     }
     return p;
 }

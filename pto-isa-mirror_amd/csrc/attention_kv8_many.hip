@@ -5,12 +5,18 @@ namespace ptoamd {
 
 // A workgroup has 32 rows a wave of one sequence and key head (rows: new tokens times the query heads that share the key head, token-major,
 // so those heads share what is staged) and walks the keys that its rows see in tiles of 64 (32 of heads of 256).  A tile's codes are read while the tile before
-// is computed, become f16, exactly, once for all waves, and go to LDS in one of two buffers; one barrier a tile.
+// is computed, become f16, exactly, once for all waves, and go to LDS in one of two buffers.
 //   S^T = K q^T (32x32x16): a fragment is 8 elements of one key, q's fragments stay in registers.
 //   o^T = V^T p^T : a lane has the scores of keys 8 (i / 4) + 4 (lane / 32) + i % 4 of 32 for its row; with eight of them as its share of a
 //                 product's 16 keys the weights are the fragment as they stand, and V's fragment (the same keys of one element) comes from
 //                 two transposing LDS reads of four keys each.
 // Scores, references and sums are f32; a page's value scale goes into the weight (ValueScale).
+// Bound: the matrix and the vector unit by turns.  A tile of 64 keys of heads of 128 takes a SIMD and its two waves 2048 clocks of products and some
+// 2900 of vector instructions (an exponential of a score takes 16), which overlap to 4160.  A prompt of 8192 tokens, 32 / 8 heads of 128, E4M3: 550
+// to 580 us with the card's clock, 950 to 1000 TFLOP/s (a bf16 product of 8192 x 8192 x 8192: 1407).  On the way there: both waves
+// of a SIMD in step 666 us, one a segment behind 606, fragments and staging in a fixed order between the products 574, NaN kept out of the sum where
+// scales are staged instead of at every sum 550.  The card clocks it at 2.05 GHz (of 2.4): looking for the largest score only where a weight
+// overflows spares a sixth of a score's vector instructions and no time; table entries asked for later in a turn cost 1%.
 template <int D>
 struct ManyTile {
     static constexpr int KEYS = many_keys(D);  // (heads of 256: the registers hold no scores of 64 keys beside q and the sums)

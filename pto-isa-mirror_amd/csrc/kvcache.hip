@@ -92,7 +92,10 @@ __device__ __forceinline__ void load8(const T* p, float* x)
 // One workgroup a page of a sequence, head, and side (keys or values).  The new tokens' largest magnitude gives the page's scale, which
 // only grows; where it grows, the older tokens' codes are rounded again to the new one.  A thread has 8 elements of a row at a time.
 // Magnitudes are compared as integers, so that an infinity or a NaN among them is the largest, whatever the order.
-// Bound: HBM (values read once, a byte a value written; the second read of a page's values comes from the L2).
+// Bound: HBM (values read once, a byte a value written; the second read of a page's values comes from the L2) and the chain of loads of a
+// workgroup that has 12 KB to move (lengths, values, page, scale).  Seven ragged prompts of up to 2048 tokens, 8 heads of 128, pages of 32,
+// bf16 to E4M3: 48.5 MB in 13.9 us, 3.5 TB/s; one token of 48 sequences 7 us, a launch.  (Keys and values in one workgroup: 16.4 us
+// where this took 14.8, one token 4.6 instead of 3.6 in a graph; values kept in registers between the passes: no faster.)
 template <typename T, int CODE, bool WIDE>
 __global__ void __launch_bounds__(256) kvcache_append_kernel(AppendArgs a)
 {

@@ -112,7 +112,8 @@ struct AttentionPlan {
 static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int tokens, int max_tokens, int max_length, int window)
 {
     AttentionPlan p{AttentionPlan::GENERIC, 1, 0, 0};
-    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+    const int dim = built_head(c->head_dim);
+    if (dim == 0)
         return p;
     const long rows = (long)max_tokens * (heads / c->kv_heads);
     p.kernel = rows <= FEW_ROWS ? AttentionPlan::FEW : AttentionPlan::MANY;
@@ -124,11 +125,11 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     const long cus = device_compute_units();
     const long items = (long)c->sequences * c->kv_heads;
     if (p.kernel == AttentionPlan::FEW) {
-        const long step = 32 * few_waves(c->head_dim, rows);  // the keys that a workgroup's waves have at a time
+        const long step = 32 * few_waves(dim, rows);  // the keys that a workgroup's waves have at a time
         const long turns = (keys + step - 1) / step;
         long splits = (cus + items - 1) / items;
         splits = splits < turns / 2 ? splits : turns / 2;
-        if (turns <= (c->head_dim == 256 ? 4 : 6))
+        if (turns <= (dim == 256 ? 4 : 6))
             splits = 1;
         const long even = (keys + 4095) / 4096;
         splits = splits > even ? splits : even;
@@ -138,14 +139,14 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
         }
         return p;
     }
-    p.row_tiles = (int)((rows + many_rows(c->head_dim) - 1) / many_rows(c->head_dim));
+    p.row_tiles = (int)((rows + many_rows(dim) - 1) / many_rows(dim));
     const long tiles = p.row_tiles * items;  // of rows, a workgroup's each if no keys are cut
     const bool countable = (long)p.row_tiles * c->sequences <= Cuts::MOST && (double)tiles * c->max_pages * c->page_size < 1e9;
     const double full = (double)tiles / cus / (c->sequences > 1 ? 2 : 1);
-    if (countable && keys * (1 - full) > 448 * full + 102400.0 / c->head_dim) {
+    if (countable && keys * (1 - full) > 448 * full + 102400.0 / dim) {
         // (a tile's parts: its keys, at most twice the mean of one sequence's, in stretches of the mean; of several up to all stretches of a key head)
         const long mean = 2 * cus / tiles + 3, most = c->sequences > 1 ? cus / c->kv_heads + 2 : mean;
-        const long room = (256L << 20) / ((long)tokens * heads * (c->head_dim * 4 + 8));
+        const long room = (256L << 20) / ((long)tokens * heads * (dim * 4 + 8));
         const long parts = most < room ? most : room;
         p.splits = (int)(parts > mean ? parts : mean);
     }
@@ -188,7 +189,7 @@ size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache* cache, int h
     if (cache == nullptr || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads != 0 || tokens <= 0 || max_tokens <= 0 || cache->sequences <= 0 ||
         cache->max_pages <= 0 || cache->page_size <= 0)
         return 0;
-    return part_bytes(plan_attention(cache, heads, tokens, max_tokens, max_length, window), heads, tokens, cache->head_dim);
+    return part_bytes(plan_attention(cache, heads, tokens, max_tokens, max_length, window), heads, tokens, built_head(cache->head_dim));
 }
 
 int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, const void* q, int type, int heads, int tokens,
@@ -233,7 +234,7 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
     hipStream_t s = as_stream(stream);
     const bool i8 = cache->code_type == PTOAMD_I8, f16 = type == PTOAMD_F16;
     const AttentionPlan plan = plan_attention(cache, heads, tokens, max_tokens, max_length, window);
-    const size_t need = part_bytes(plan, heads, tokens, cache->head_dim);
+    const size_t need = part_bytes(plan, heads, tokens, built_head(cache->head_dim));
     PTOAMD_REQUIRE(workspace == nullptr || workspace_bytes >= need, PTOAMD_E_INVALID, "%s: a workspace of %zu bytes is needed (%zu)", what, need, workspace_bytes);
     PTOAMD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, PTOAMD_E_ALIGNMENT, "%s: the workspace must be 16-byte aligned", what);
     const uint64_t cache_bits = (uint64_t)(uintptr_t)cache->k | (uint64_t)(uintptr_t)cache->v | (uint64_t)cache->k_page_stride | (uint64_t)cache->k_head_stride |
@@ -250,7 +251,7 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
         a.sequences = cache->sequences;
         a.cuts = plan.kernel == AttentionPlan::MANY && a.splits > 1 ? static_cast<int*>(workspace) : nullptr;
         a.part_out = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (a.cuts != nullptr ? Cuts::BYTES : 0));
-        a.part_sum = reinterpret_cast<float2*>(a.part_out + (size_t)plan.splits * tokens * heads * cache->head_dim);
+        a.part_sum = reinterpret_cast<float2*>(a.part_out + (size_t)plan.splits * tokens * heads * built_head(cache->head_dim));
         const bool few = plan.kernel == AttentionPlan::FEW;
         const int rc = few ? launch_attention_few(a, cache->code_type, f16, cache->sequences, s) : launch_attention_many(a, cache->code_type, f16, cache->sequences, s);
         if (rc != PTOAMD_OK)

@@ -36,6 +36,9 @@ struct Cuts {
     static constexpr size_t BYTES = 2048;
     static_assert(SIZE * sizeof(int) <= BYTES, "the join finds them at the workspace's start");
 };
+// The heads that the few and many kernels are built for; a smaller head takes the next of them: lanes beyond its elements read its first ones again,
+// which the queries' zeros there take out of the scores, and whose results are not stored.  0: only the generic kernel.
+constexpr int built_head(int head_dim) { return head_dim % 16 != 0 || head_dim > 256 ? 0 : head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 constexpr int many_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }  // a tile's
 constexpr int many_keys(int head_dim) { return head_dim == 256 ? 32 : 64; }
 constexpr int many_start(int head_dim) { return 448 / many_keys(head_dim); }

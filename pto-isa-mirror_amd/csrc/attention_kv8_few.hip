@@ -50,7 +50,11 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
     const int first = begin + 32 * wave;
     const int32_t* table = c.table + (int64_t)seq * c.max_pages;
     auto find = [&](int key) { return table[min((key + 16 * (lane & 1)) >> c.page_shift, c.max_pages - 1)]; };  // even lanes: of the first half, odd: the second
-    const uint32_t k_lane = (uint32_t)(col * (int)c.k.token + 16 * g), v_lane = (uint32_t)(4 * g * (int)c.v.token + col * (D / 16));
+    uint32_t k_lane[D / 64];  // (beyond the head: its first elements)
+#pragma unroll
+    for (int cc = 0; cc < D / 64; ++cc)
+        k_lane[cc] = (uint32_t)(col * (int)c.k.token + (64 * cc + 16 * g < c.head_dim ? 64 * cc + 16 * g : 0));
+    const uint32_t v_lane = (uint32_t)(4 * g * (int)c.v.token + (col * (D / 16) < c.head_dim ? col * (D / 16) : 0));
     const uint8_t *k_head = c.k.codes + kv_head * c.k.head, *v_head = c.v.codes + kv_head * c.v.head;
     const uint32_t k_page = (uint32_t)(c.k.page >> 3), v_page = (uint32_t)(c.v.page >> 3);  // (pages start on 8 bytes)
     const float* scales = lane & 2 ? c.v.scales : c.k.scales;
@@ -65,7 +69,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
             const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(v_head + ((uint64_t)page * v_page * 8 + slot * (uint32_t)c.v.token)), 0, bytes, 0x20000);
 #pragma unroll
             for (int cc = 0; cc < D / 64; ++cc)
-                tile.k[h][cc] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane + 64 * cc, 0, 0));
+                tile.k[h][cc] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane[cc], 0, 0));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = i * (int)c.v.token;
@@ -101,7 +105,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
         const uint8_t* p = a.q + (int64_t)(span.first + (valid ? token : 0)) * a.q_token + (int64_t)(kv_head * a.group + (valid ? row - token * a.group : 0)) * a.q_head;
 #pragma unroll
         for (int st = 0; st < STEPS; ++st)
-            q[t][st] = valid ? load_row8(p + 2 * (64 * (st / 2) + 16 * g + 8 * (st % 2)), a.wide) : make_uint4(0, 0, 0, 0);
+            q[t][st] = valid && 64 * (st / 2) + 16 * g < c.head_dim ? load_row8(p + 2 * (64 * (st / 2) + 16 * g + 8 * (st % 2)), a.wide) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int s = 0; s < RING; ++s) {
@@ -317,6 +321,8 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
     __syncthreads();
     for (int u = threadIdx.x; u < min(rows - row0, 16 * NT) * (D / 8); u += 64 * WAVES) {
         const int row = u / (D / 8), piece = u % (D / 8) * 8, token = (row0 + row) / a.group, head = kv_head * a.group + row0 + row - token * a.group;
+        if (piece >= c.head_dim)
+            continue;
         float to = wave_top[0][row];
 #pragma unroll
         for (int w = 1; w < WAVES; ++w)
@@ -421,6 +427,8 @@ __global__ void __launch_bounds__(256) attention_kv8_join_kernel(AttentionArgs a
             o = make_float4(o.x + x.x * by, o.y + x.y * by, o.z + x.z * by, o.w + x.w * by);
         }
     }
+    if (4 * i >= a.cache.head_dim)
+        return;
     const float inverse = sum == 0.0f ? 0.0f : 1.0f / sum;
     T* out = reinterpret_cast<T*>(a.out + (int64_t)(span.first + nth) * a.out_token + (int64_t)head * a.out_head) + 4 * i;
     const float x[4] = {sum == 0.0f ? 0.0f : o.x * inverse, sum == 0.0f ? 0.0f : o.y * inverse, sum == 0.0f ? 0.0f : o.z * inverse, sum == 0.0f ? 0.0f : o.w * inverse};
@@ -465,7 +473,7 @@ static int choose_tiles(const AttentionArgs& a, int sequences, hipStream_t strea
 template <typename T, int CODE>
 static int choose_size(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
-    switch (a.cache.head_dim) {
+    switch (built_head(a.cache.head_dim)) {
         case 64: return choose_tiles<T, CODE, 64>(a, sequences, stream);
         case 128: return choose_tiles<T, CODE, 128>(a, sequences, stream);
         default: return choose_tiles<T, CODE, 256>(a, sequences, stream);
@@ -492,7 +500,7 @@ static void launch_join(const AttentionArgs& a, int sequences, hipStream_t strea
 template <typename T>
 static void choose_join(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
-    switch (a.cache.head_dim) {
+    switch (built_head(a.cache.head_dim)) {
         case 64: launch_join<T, 64>(a, sequences, stream); break;
         case 128: launch_join<T, 128>(a, sequences, stream); break;
         default: launch_join<T, 256>(a, sequences, stream); break;

@@ -159,7 +159,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             const uint8_t* p = a.q + (int64_t)(span.first + (valid ? token : 0)) * a.q_token + (int64_t)head * a.q_head;
 #pragma unroll
             for (int st = 0; st < STEPS; ++st)
-                q[st] = valid ? load_row8(p + 2 * (16 * st + 8 * hf), a.wide) : make_uint4(0, 0, 0, 0);
+                q[st] = valid && 16 * st < c.head_dim ? load_row8(p + 2 * (16 * st + 8 * hf), a.wide) : make_uint4(0, 0, 0, 0);
             uint32_t largest = largest_of<STEPS>(q);
             largest = max(largest, (uint32_t)__shfl_xor((int)largest, 32));
             const RowScale r = row_scale<T>(largest);
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             const int k = (tid + u * THREADS) % SIDE_UNITS / (D / 16), chunk = lane % (D / 16) * 2;
-            source[u] = (uint32_t)(lane / (D / 16)) * (uint32_t)(is_value(u) ? c.v.token : c.k.token) + lane % (D / 16) * 16;
+            source[u] = (uint32_t)(lane / (D / 16)) * (uint32_t)(is_value(u) ? c.v.token : c.k.token) + (lane % (D / 16) * 16 < c.head_dim ? lane % (D / 16) * 16 : 0);
             target[u][0] = is_value(u) ? Tile::value_at(k, chunk / 2) : Tile::key_at(k, chunk);
             target[u][1] = is_value(u) ? Tile::value_at(k, chunk / 2) + 16 : Tile::key_at(k, chunk + 1);
         }
@@ -429,6 +429,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         float* part_out = e.global<float>(offsetof(AttentionArgs, part_out)) + (part_row + (int64_t)(span.first + own_token) * a.heads + own_head) * D + 16 * (lane % 2);
         uint8_t* out = e.global<uint8_t>(offsetof(AttentionArgs, out)) + (int64_t)(span.first + own_token) * ARGUMENT(e, out_token) + (int64_t)own_head * ARGUMENT(e, out_head) + 32 * (lane % 2);
         const bool wide = ARGUMENT(e, wide);
+        const int head_dim = e.field<int>(offsetof(AttentionArgs, cache) + offsetof(Kv8, head_dim));
 #pragma unroll
         for (int m = 0; m < DT; ++m) {
 #pragma unroll
@@ -439,7 +440,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
             for (int i = 0; i < 4; ++i)
                 x[i] = *reinterpret_cast<const f32x4*>(mine + own * 128 + ((4 * (lane % 2) + i) ^ (own & 7)) * 16);
-            if (own_row >= rows)
+            if (own_row >= rows || 32 * m + 16 * (lane % 2) >= head_dim)
                 continue;
             if (part >= 0) {
 #pragma unroll
@@ -472,7 +473,7 @@ static int launch_many(const AttentionArgs& a, int sequences, hipStream_t stream
 template <typename T, int CODE>
 static int choose_size(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
-    switch (a.cache.head_dim) {
+    switch (built_head(a.cache.head_dim)) {
         case 64: return launch_many<T, CODE, 64, 8>(a, sequences, stream);
         case 128: return launch_many<T, CODE, 128, 8>(a, sequences, stream);
         default: return launch_many<T, CODE, 256, 4>(a, sequences, stream);

@@ -50,6 +50,25 @@ def test_chunks_and_prompts(pa, code, dim, causal, window):  # noqa: F811
     run(pa, code, lengths, counts, 6, 2, dim, 16 if dim == 64 else 64, causal=causal, window=window, strided=True)
 
 
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [16, 48, 80, 96, 112, 192, 240])
+@pytest.mark.parametrize("token_major", [False, True])
+def test_heads_of_other_sizes(pa, code, dim, token_major):  # noqa: F811
+    run(pa, code, [1, 300, 0, 2077], [1] * 4, 8, 2, dim, 16, token_major=token_major)
+    assert not pa.last_kernel().startswith("attention_kv8_generic")
+    run(pa, code, [9, 300, 40, 2077], [9, 5, 17, 2], 12, 2, dim, 32, dtype=torch.float16, token_major=token_major, strided=True, window=77)
+    run(pa, code, [90, 300, 0, 3001], [90, 55, 0, 70], 6, 2, dim, 64, token_major=token_major)
+    assert not pa.last_kernel().startswith("attention_kv8_generic")
+
+
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [8, 72, 320, 512])
+def test_heads_that_only_the_generic_kernel_takes(pa, code, dim):  # noqa: F811
+    run(pa, code, [1, 300, 0, 1077], [1] * 4, 8, 2, dim, 16, strided=True)
+    assert pa.last_kernel() == "attention_kv8_generic"
+    run(pa, code, [90, 200], [90, 35], 4, 4, dim, 32, dtype=torch.float16, window=50)
+
+
 @pytest.mark.parametrize("page", [16, 32, 64, 128, 256])
 def test_every_page_size(pa, page):  # noqa: F811
     run(pa, "i8", [700, 255, 256, 257], [1] * 4, 8, 2, 128, page)

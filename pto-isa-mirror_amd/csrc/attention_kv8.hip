@@ -89,9 +89,14 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 }
 
 // Which kernel runs and how the keys are split, from sizes alone: the same for the workspace's size as for the call.
-//   few  : at most 96 rows (new tokens of a sequence times the query heads that share a key head), 16 or 32 of them a workgroup.
-//          8 sequences of 6000 keys, 8 key heads of 128, int8, us, few / many: 16 rows 24 / 80, 64 52 / 85, 96 74 / 89, 128 95 / 92.
+//   few  : at most 96 rows (new tokens of a sequence times the query heads that share a key head), or 64 (48 of heads of 256) where the keys of
+//          all heads and sequences are more than 64 KB a CU.  us, few / many, heads of 128: 8 sequences of 6000 keys, 8 key heads, 16 rows 24 / 62,
+//          48 38 / 63, 64 46 / 65, 80 65 / 69; 32 of 8000 128 rows 353 / 278; one of 2000 48 rows 13 / 23, 96 15 / 25.  Of 256, 32 of 8000, 2 key heads:
+//          48 130 / 145, 64 168 / 147; 8 of 6000 64 59 / 49.
 //   many : more rows, 256 of them a workgroup (128 for heads of 256 elements)
+// Few rows are 16, 32, or, where the keys are that many, up to 48 a workgroup and 64 of heads of 128: codes are converted once for all of them.
+// 32 sequences of 8000 keys, 8 key heads of 128, us, 32 / 48 / 64 rows a workgroup: 32 rows 128 / 153 / 181, 48 226 / 156 / 183, 64 229 / 277 / 188;
+// of 64: 48 rows 114 / 85 / 135, 64 105 / 131 / 125; one sequence of 2000 keys, 48 rows 13.4 / 15.7 / 17.7.
 // Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
 // (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
 // heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.
@@ -104,7 +109,6 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 //   68 / 43.  (The same number of parts for every sequence instead, the best for each call: of these 512 over
 //   16384 163, the three of 6104 106, the four of 16000 204; but what the host knows did not tell which number, by a factor of up to 1.7.)
 // Parts have room for a sequence that is the only long one, within 256 MB.
-constexpr long FEW_ROWS = 96;
 struct AttentionPlan {
     enum { GENERIC, FEW, MANY } kernel;
     int splits, chunk, row_tiles;
@@ -116,7 +120,6 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     if (dim == 0)
         return p;
     const long rows = (long)max_tokens * (heads / c->kv_heads);
-    p.kernel = rows <= FEW_ROWS ? AttentionPlan::FEW : AttentionPlan::MANY;
     long keys = (long)c->max_pages * c->page_size;
     if (max_length > 0 && max_length < keys)
         keys = max_length;
@@ -124,8 +127,11 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
         keys = (long)window + max_tokens + 31;
     const long cus = device_compute_units();
     const long items = (long)c->sequences * c->kv_heads;
+    const bool busy = items * keys * dim > 65536 * cus;
+    p.kernel = rows <= (!busy ? 96 : dim == 256 ? 48 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
     if (p.kernel == AttentionPlan::FEW) {
-        const long step = 32 * few_waves(dim, rows);  // the keys that a workgroup's waves have at a time
+        p.row_tiles = rows <= 16 || dim == 256 ? 1 : rows <= 32 || !busy ? 2 : rows <= 48 ? 3 : dim == 128 ? 4 : 2;
+        const long step = 32 * few_waves(dim, p.row_tiles);  // the keys that a workgroup's waves have at a time
         const long turns = (keys + step - 1) / step;
         long splits = (cus + items - 1) / items;
         splits = splits < turns / 2 ? splits : turns / 2;
@@ -164,11 +170,12 @@ int prepare_attention_kernels()
     for (int code : {PTOAMD_I8, PTOAMD_E4M3})
         for (bool f16 : {false, true})
             for (int dim : {64, 128, 256})
-                for (int rows : {16, 32}) {
+                for (int tiles : {1, 2, 3, 4}) {
+                    if (tiles > (dim == 64 ? 3 : dim == 128 ? 4 : 1))
+                        continue;
                     AttentionArgs a{};  // (of no heads: nothing is launched)
                     a.cache.head_dim = dim;
-                    a.cache.max_tokens = rows;
-                    a.group = 1;
+                    a.row_tiles = tiles;
                     int rc = launch_attention_few(a, code, f16, 1, nullptr);
                     if (rc == PTOAMD_OK)
                         rc = launch_attention_many(a, code, f16, 1, nullptr);

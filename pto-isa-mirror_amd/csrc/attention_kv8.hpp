@@ -20,7 +20,7 @@ struct AttentionArgs {
     int wide;  // rows of q and out allow 16-byte accesses
     // The keys of a row in parts, where splits > 1 (at most so many): every part leaves its sums of a row (unscaled) and the row's reference and
     // sum, [split][token][head]; a second kernel joins them in the order of the parts.
-    // Few rows: parts of `chunk` tokens, each a workgroup's.  Many: `cuts`, of the rows in row_tiles tiles a sequence (Cuts).
+    // Few rows, row_tiles of 16 a workgroup: parts of `chunk` tokens, each a workgroup's.  Many: `cuts`, of the rows in row_tiles tiles a sequence (Cuts).
     int splits, chunk, row_tiles, sequences;
     int* cuts;
     float* part_out;
@@ -43,8 +43,8 @@ constexpr int many_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }  /
 constexpr int many_keys(int head_dim) { return head_dim == 256 ? 32 : 64; }
 constexpr int many_start(int head_dim) { return 448 / many_keys(head_dim); }
 
-// The waves of a few-rows workgroup: eight where two fit a SIMD's registers (heads up to 128 elements, 16 rows), else four.
-constexpr int few_waves(int head_dim, long rows) { return head_dim <= 128 && rows <= 16 ? 8 : 4; }
+// The waves of a few-rows workgroup of so many tiles of 16 rows: eight where two fit a SIMD's registers (heads up to 128 elements, one tile), else four.
+constexpr int few_waves(int head_dim, int row_tiles) { return head_dim <= 128 && row_tiles == 1 ? 8 : 4; }
 int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_many(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_join(const AttentionArgs& a, bool f16, int sequences, hipStream_t stream);

@@ -463,12 +463,14 @@ static int launch_few(const AttentionArgs& a, int sequences, hipStream_t stream)
 template <typename T, int CODE, int D>
 static int choose_tiles(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
-    // (two tiles of 256 columns' sums and fragments do not fit the registers: those rows go 16 a workgroup)
-    if constexpr (D < 256) {
-        if (a.cache.max_tokens * a.group > 16)
-            return launch_few<T, CODE, D, 2, few_waves(D, 32)>(a, sequences, stream);
+    // (two tiles of 256 columns' sums and fragments do not fit the registers, nor four of 128 columns more than one wave a SIMD)
+    switch (a.row_tiles) {
+        case 1: return launch_few<T, CODE, D, 1, few_waves(D, 1)>(a, sequences, stream);
+        case 2: if constexpr (D < 256) return launch_few<T, CODE, D, 2, few_waves(D, 2)>(a, sequences, stream); break;
+        case 3: if constexpr (D < 256) return launch_few<T, CODE, D, 3, few_waves(D, 3)>(a, sequences, stream); break;
+        case 4: if constexpr (D == 128) return launch_few<T, CODE, D, 4, few_waves(D, 4)>(a, sequences, stream); break;
     }
-    return launch_few<T, CODE, D, 1, few_waves(D, 16)>(a, sequences, stream);
+    return PTOAMD_E_INVALID;  // (no plan has it)
 }
 template <typename T, int CODE>
 static int choose_size(const AttentionArgs& a, int sequences, hipStream_t stream)

@@ -83,6 +83,16 @@ def test_long_sequences_are_split_and_joined(pa, tokens):  # noqa: F811
 
 
 @pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 112, 128, 256])
+@pytest.mark.parametrize("tokens", [5, 6, 7, 8, 9])
+def test_several_tokens_over_many_keys(pa, code, dim, tokens):  # noqa: F811
+    # 40 to 72 rows over more than 64 KB of keys a compute unit: one to three, or four, tiles of 16 rows a workgroup
+    kv_heads = 4 if dim == 64 else 2
+    run(pa, code, [22030, 5, 1200], [tokens, 2, tokens], 8 * kv_heads, kv_heads, dim, 64)
+    run(pa, code, [30, 24100, 0], [tokens, tokens, 0], 7 * kv_heads, kv_heads, dim, 128, window=23000)
+
+
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("kw", [{}, {"causal": False}, {"window": 1500}])
 def test_chunks_over_sequences_of_very_different_lengths(pa, code, dim, kw):  # noqa: F811

@@ -94,10 +94,10 @@ __device__ __forceinline__ void load8(const T* p, float* x)
 // Magnitudes are compared as integers, so that an infinity or a NaN among them is the largest, whatever the order.
 // Bound: HBM (values read once, a byte a value written; the second read of a page's values comes from the L2) and the chain of loads of a
 // workgroup that has 12 KB to move (lengths, values, page, scale).  Seven ragged prompts of up to 2048 tokens, 8 heads of 128, pages of 32,
-// bf16 to E4M3: 48.5 MB in 13.9 us, 3.5 TB/s; one token of 48 sequences 7 us, a launch.  (Keys and values in one workgroup: 16.4 us
-// where this took 14.8, one token 4.6 instead of 3.6 in a graph; values kept in registers between the passes: no faster.)
-template <typename T, int CODE, bool WIDE>
-__global__ void __launch_bounds__(256) kvcache_append_kernel(AppendArgs a)
+// bf16 to E4M3: 48.5 MB in 13.5 us, 3.6 TB/s; one token of 48 sequences 7 us, a launch.  (Keys and values in one workgroup, their values in
+// registers between the passes: 16.4 us in a graph where one side's without took 14.8, and one side's with 15.9.)
+template <typename T, int CODE, bool WIDE, int THREADS>
+__global__ void __launch_bounds__(THREADS) kvcache_append_kernel(AppendArgs a)
 {
     const Kv8& c = a.cache;
     const int seq = blockIdx.x / a.blocks, nth = blockIdx.x - seq * a.blocks, head = blockIdx.y;
@@ -118,14 +118,14 @@ __global__ void __launch_bounds__(256) kvcache_append_kernel(AppendArgs a)
     const int chunks = c.head_dim / 8, units = fresh * chunks;
     const uint8_t* src = a.src[values] + (int64_t)(first + lo - start) * a.token[values] + (int64_t)head * a.head[values];
     uint32_t largest = 0;
-    for (int u = threadIdx.x; u < units; u += 256) {
+    for (int u = threadIdx.x; u < units; u += THREADS) {
         float x[8];
         load8<T, WIDE>(reinterpret_cast<const T*>(src + (int64_t)(u / chunks) * a.token[values]) + (u % chunks) * 8, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             largest = max(largest, f2u(x[i]) & 0x7FFFFFFFu);
     }
-    __shared__ uint32_t wave_largest[4];
+    __shared__ uint32_t wave_largest[THREADS / 64];
 #pragma unroll
     for (int d = 32; d > 0; d >>= 1)
         largest = max(largest, (uint32_t)__shfl_xor((int)largest, d));
@@ -134,7 +134,9 @@ __global__ void __launch_bounds__(256) kvcache_append_kernel(AppendArgs a)
     float* scale = side.scales + (int64_t)page * c.kv_heads + head;
     const float before = older > 0 ? *scale : 0.0f;
     __syncthreads();  // (the scale has been read by all before one writes it)
-    largest = max(max(wave_largest[0], wave_largest[1]), max(wave_largest[2], wave_largest[3]));
+#pragma unroll
+    for (int w = 0; w < THREADS / 64; ++w)
+        largest = max(largest, wave_largest[w]);
     const bool finite = largest < 0x7F800000u;
     float after = u2f(largest) * (CODE == PTOAMD_I8 ? 1.0f / 127.0f : 1.0f / 448.0f);
     after = before > after ? before : after;
@@ -146,7 +148,7 @@ __global__ void __launch_bounds__(256) kvcache_append_kernel(AppendArgs a)
     uint8_t* dst = side.codes + (int64_t)page * side.page + (int64_t)head * side.head;
     if (before < after) {  // the older tokens' codes in the new unit
         const float ratio = before / after;
-        for (int u = threadIdx.x; u < older * chunks; u += 256) {
+        for (int u = threadIdx.x; u < older * chunks; u += THREADS) {
             uint2* p = reinterpret_cast<uint2*>(dst + (int64_t)(u / chunks) * side.token + (u % chunks) * 8);
             const uint2 w = *p;
             float x[8];
@@ -157,7 +159,7 @@ __global__ void __launch_bounds__(256) kvcache_append_kernel(AppendArgs a)
         }
     }
     const float inverse = after > 0.0f ? 1.0f / after : 0.0f;
-    for (int u = threadIdx.x; u < units; u += 256) {
+    for (int u = threadIdx.x; u < units; u += THREADS) {
         float x[8];
         load8<T, WIDE>(reinterpret_cast<const T*>(src + (int64_t)(u / chunks) * a.token[values]) + (u % chunks) * 8, x);
 #pragma unroll
@@ -167,17 +169,30 @@ __global__ void __launch_bounds__(256) kvcache_append_kernel(AppendArgs a)
     }
 }
 
-template <typename T, int CODE>
+template <typename T, int CODE, int THREADS>
 static int launch_append(const AppendArgs& a, int sequences, bool wide, hipStream_t stream)
 {
     const dim3 grid((unsigned)((long)sequences * a.blocks), (unsigned)a.cache.kv_heads, 2);
     if (wide)
-        hipLaunchKernelGGL((kvcache_append_kernel<T, CODE, true>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((kvcache_append_kernel<T, CODE, true, THREADS>), grid, dim3(THREADS), 0, stream, a);
     else
-        hipLaunchKernelGGL((kvcache_append_kernel<T, CODE, false>), grid, dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((kvcache_append_kernel<T, CODE, false, THREADS>), grid, dim3(THREADS), 0, stream, a);
     PTOAMD_HIP_CHECK(hipGetLastError());
     set_last_kernel("kvcache_append");
     return PTOAMD_OK;
+}
+// Threads by the bytes that a page's new tokens have of a head: few enough that small pages' workgroups are many on a CU, enough that large ones are
+// loaded at once.  4 sequences of 1024 tokens, 8 heads, us, 128 / 256 / 512 threads: bf16, heads of 64, pages of 16 (2 KB) 6.9 / 8.9 / 13.5; of 128, 32
+// (8 KB) 8.4 / 8.3 / 10.4; 64 (16 KB) 10.0 / 8.6 / 8.5; 128 (32 KB) 12.4 / 9.4 / 9.2; of 256, 128 (64 KB) 31 / 19 / 16; f32, of 256, pages of 16 (16 KB)
+// 24 / 19 / 19, of 32 (32 KB) 23 / 24 / 20; one token of 256 sequences, heads of 128, 5.9 / 7.9 / 12.5.
+template <typename T, int CODE>
+static int choose_threads(const AppendArgs& a, int sequences, bool wide, hipStream_t stream)
+{
+    const int page = 1 << a.cache.page_shift;
+    const long bytes = (long)(a.cache.max_tokens < page ? a.cache.max_tokens : page) * a.cache.head_dim * sizeof(T);
+    if (bytes <= 8192)
+        return launch_append<T, CODE, 128>(a, sequences, wide, stream);
+    return bytes <= 16384 ? launch_append<T, CODE, 256>(a, sequences, wide, stream) : launch_append<T, CODE, 512>(a, sequences, wide, stream);
 }
 template <typename T>
 static int dispatch_append(const AppendArgs& a, int code, int sequences, hipStream_t stream)
@@ -185,8 +200,8 @@ static int dispatch_append(const AppendArgs& a, int code, int sequences, hipStre
     uint64_t bits = 0;
     for (int i = 0; i < 2; ++i)
         bits |= (uint64_t)(uintptr_t)a.src[i] | (uint64_t)a.token[i] | (uint64_t)a.head[i];
-    return code == PTOAMD_I8 ? launch_append<T, PTOAMD_I8>(a, sequences, bits % 16 == 0, stream)
-                             : launch_append<T, PTOAMD_E4M3>(a, sequences, bits % 16 == 0, stream);
+    return code == PTOAMD_I8 ? choose_threads<T, PTOAMD_I8>(a, sequences, bits % 16 == 0, stream)
+                             : choose_threads<T, PTOAMD_E4M3>(a, sequences, bits % 16 == 0, stream);
 }
 
 }  // namespace ptoamd

@@ -89,10 +89,10 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 }
 
 // Which kernel runs and how the keys are split, from sizes alone: the same for the workspace's size as for the call.
-//   few  : at most 96 rows (new tokens of a sequence times the query heads that share a key head), or 64 (48 of heads of 256) where the keys of
+//   few  : at most 96 rows (new tokens of a sequence times the query heads that share a key head), or 64 (32 of heads of 256) where the keys of
 //          all heads and sequences are more than 64 KB a CU.  us, few / many, heads of 128: 8 sequences of 6000 keys, 8 key heads, 16 rows 24 / 62,
-//          48 38 / 63, 64 46 / 65, 80 65 / 69; 32 of 8000 128 rows 353 / 278; one of 2000 48 rows 13 / 23, 96 15 / 25.  Of 256, 32 of 8000, 2 key heads:
-//          48 130 / 145, 64 168 / 147; 8 of 6000 64 59 / 49.
+//          48 38 / 63, 64 46 / 65, 80 65 / 69; 32 of 8000 128 rows 353 / 278; one of 2000 48 rows 13 / 23, 96 15 / 25.  Of 256, 2 key heads, 32 of
+//          8000: 48 130 / 114, 64 168 / 115; 8 of 6000: 40 45 / 42, 64 59 / 45; one of 60000 40 57 / 52.
 //   many : more rows, 256 of them a workgroup (128 for heads of 256 elements)
 // Few rows are 16, 32, or, where the keys are that many, up to 48 a workgroup and 64 of heads of 128: codes are converted once for all of them.
 // 32 sequences of 8000 keys, 8 key heads of 128, us, 32 / 48 / 64 rows a workgroup: 32 rows 128 / 153 / 181, 48 226 / 156 / 183, 64 229 / 277 / 188;
@@ -105,8 +105,8 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 //   128 tokens over 700, 1024, 1500 keys 30 / 35, 38 / 37, 52 / 39; 512 over 700, 1024, 1500, 2500, 16384 30 / 38, 38 / 42, 52 / 47, 78 / 55, 441 / 174;
 //   1024 over 1500, 2500 53 / 54, 80 / 71; 421, 376 and 512 over 6104, 4383 and 512 170 / 109; 3 x 512 over 6000 181 / 186; 4 x 256 over 1024, 512,
 //   341 and 146 39 / 43, over four times as many 117 / 70; 200, 512, 30 and 400 over 9000, 1200, 400 and 16000 440 / 213; 2 x 1024 over 8192 268 / 296;
-//   4 / 1 heads, 47, 114 and 166 over 8642 234 / 39; heads of 64, 4 x 100 over 1024, 2000 33 / 43, 56 / 49; 8 / 2 of 256, over 512, 1024 40 / 39,
-//   68 / 43.  (The same number of parts for every sequence instead, the best for each call: of these 512 over
+//   4 / 1 heads, 47, 114 and 166 over 8642 234 / 39; heads of 64, 4 x 100 over 1024, 2000 33 / 43, 56 / 49; 8 / 2 of 256 (then in tiles of
+//   32 keys), over 512, 1024 40 / 39, 68 / 43.  (The same number of parts for every sequence instead, the best for each call: of these 512 over
 //   16384 163, the three of 6104 106, the four of 16000 204; but what the host knows did not tell which number, by a factor of up to 1.7.)
 // Parts have room for a sequence that is the only long one, within 256 MB.
 struct AttentionPlan {
@@ -128,7 +128,7 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     const long cus = device_compute_units();
     const long items = (long)c->sequences * c->kv_heads;
     const bool busy = items * keys * dim > 65536 * cus;
-    p.kernel = rows <= (!busy ? 96 : dim == 256 ? 48 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
+    p.kernel = rows <= (!busy ? 96 : dim == 256 ? 32 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
     if (p.kernel == AttentionPlan::FEW) {
         p.row_tiles = rows <= 16 || dim == 256 ? 1 : rows <= 32 || !busy ? 2 : rows <= 48 ? 3 : dim == 128 ? 4 : 2;
         const long step = 32 * few_waves(dim, p.row_tiles);  // the keys that a workgroup's waves have at a time

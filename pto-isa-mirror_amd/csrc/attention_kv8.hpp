@@ -40,8 +40,7 @@ struct Cuts {
 // which the queries' zeros there take out of the scores, and whose results are not stored.  0: only the generic kernel.
 constexpr int built_head(int head_dim) { return head_dim % 16 != 0 || head_dim > 256 ? 0 : head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 constexpr int many_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }  // a tile's
-constexpr int many_keys(int head_dim) { return head_dim == 256 ? 32 : 64; }
-constexpr int many_start(int head_dim) { return 448 / many_keys(head_dim); }
+constexpr int MANY_KEYS = 64, MANY_START = 448 / MANY_KEYS;
 
 // The waves of a few-rows workgroup of so many tiles of 16 rows: eight where two fit a SIMD's registers (heads up to 128 elements, one tile), else four.
 constexpr int few_waves(int head_dim, int row_tiles) { return head_dim <= 128 && row_tiles == 1 ? 8 : 4; }

@@ -4,7 +4,7 @@
 namespace ptoamd {
 
 // A workgroup has 32 rows a wave of one sequence and key head (rows: new tokens times the query heads that share the key head, token-major,
-// so those heads share what is staged) and walks the keys that its rows see in tiles of 64 (32 of heads of 256).  A tile's codes are read while the tile before
+// so those heads share what is staged) and walks the keys that its rows see in tiles of 64.  A tile's codes are read while the tile before
 // is computed, become f16, exactly, once for all waves, and go to LDS in one of two buffers.
 //   S^T = K q^T (32x32x16): a fragment is 8 elements of one key, q's fragments stay in registers.
 //   o^T = V^T p^T : a lane has the scores of keys 8 (i / 4) + 4 (lane / 32) + i % 4 of 32 for its row; with eight of them as its share of a
@@ -19,7 +19,7 @@ namespace ptoamd {
 // overflows spares a sixth of a score's vector instructions and no time; table entries asked for later in a turn cost 1%.
 template <int D>
 struct ManyTile {
-    static constexpr int KEYS = many_keys(D);  // (heads of 256: the registers hold no scores of 64 keys beside q and the sums)
+    static constexpr int KEYS = MANY_KEYS;
     static constexpr int BYTES = KEYS * D * 2;       // of the keys, and as many of the values
     // Keys: 16 lanes of a read take one chunk of 16 keys: chunks are permuted so that they fall on different banks.
     static __device__ __forceinline__ int key_at(int key, int chunk)
@@ -38,7 +38,7 @@ struct ManyTile {
 template <int D, int WAVES>
 __device__ __forceinline__ void count_tiles(const AttentionArgs& a, int tiles, int* cuts)
 {
-    constexpr int KEYS = many_keys(D), LEAST = 256 / KEYS;
+    constexpr int KEYS = MANY_KEYS, LEAST = 256 / KEYS;
     static_assert(64 * WAVES >= Cuts::MOST, "a thread counts a tile of rows");
     __shared__ int wave_sum[WAVES], wave_most[WAVES];
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
@@ -50,7 +50,7 @@ __device__ __forceinline__ void count_tiles(const AttentionArgs& a, int tiles, i
         if (row0 < rows) {  // (rows that see no key have a tile too: zeros are written there)
             const int from = visible_keys(a, place0 + row0 / a.group, span.length).x & ~31;
             const int to = visible_keys(a, place0 + (min(row0 + many_rows(D), rows) - 1) / a.group, span.length).y;
-            own = max((to - from + KEYS - 1) / KEYS, 1) + many_start(D);
+            own = max((to - from + KEYS - 1) / KEYS, 1) + MANY_START;
         }
     }
     int sum = own, most = own;
@@ -86,7 +86,8 @@ __device__ __forceinline__ void count_tiles(const AttentionArgs& a, int tiles, i
 }
 
 // Heads of 256: the sums are in accumulator registers, which only the matrix instructions read.  Left to itself the compiler moves all 128 of them out
-// and back in every tile, for the multiplication that few tiles have: 1016 us instead of 815, 8192 tokens of 16 / 4 heads, int8.
+// and back in every tile, for the multiplication that few tiles have: 1016 us instead of 815, 8192 tokens of 16 / 4 heads, int8;
+// with the registers that this leaves, tiles of 64 keys instead of 32: 753.
 __device__ __forceinline__ float scaled_accumulator(float x, float by)
 {
     float t;
@@ -134,14 +135,14 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             const int first = __builtin_amdgcn_readfirstlane(cuts[Cuts::FIRST + tile]), next = __builtin_amdgcn_readfirstlane(cuts[Cuts::FIRST + tile + 1]);
             seq = tile / a.row_tiles;
             row_tile = tile - seq * a.row_tiles;
-            const int until = min(next - rest, unit_end - unit) + rest - first - many_start(D);
-            skip = max(rest - first - many_start(D), 0);
+            const int until = min(next - rest, unit_end - unit) + rest - first - MANY_START;
+            skip = max(rest - first - MANY_START, 0);
             most = until - skip;
             unit += next - rest;
             if (until <= 0)
                 continue;  // (the stretch ends before the first of its keys)
-            if (most < next - first - many_start(D))
-                part = turn - (kv_head * head_tiles + first + many_start(D)) / stretch;
+            if (most < next - first - MANY_START)
+                part = turn - (kv_head * head_tiles + first + MANY_START) / stretch;
         } else {
             const int row_tiles = gridDim.x / c.kv_heads;
             kv_head = blockIdx.x % c.kv_heads;

@@ -484,6 +484,17 @@ def kvcache_append(k, v, k_cache, v_cache, k_scale, v_scale, block_table, length
            "ptoamd_kvcache_append")
 
 
+def _temporary(nbytes, device, stream):
+    """Device memory that a call on `stream` takes and drops.  It is of that stream's pool: dropped, the allocator hands it out again only to what
+    runs behind the call, where a block of the current stream's pool could be another call's while this one still writes it."""
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream.cuda_stream, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+
 def attention_kv8_workspace_bytes(q, k_cache, block_table, max_tokens, max_length=0, window=0):
     """Bytes of workspace that attention_kv8 of these sizes splits its work with (0: not split)."""
     pages, heads, page, dim = k_cache.shape
@@ -496,7 +507,8 @@ def attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, c
     """Attention of q [tokens, heads, head_dim] (f16, bf16) over a cache that kvcache_append fills; query i of a sequence's n stands at
     lengths[s] - n + i.  max_length: a bound on the lengths, where the caller has a tighter one than the block table.  scale: by default
     head_dim ** -0.5.  want_lse: returns (out, lse), lse [tokens, heads] f32.  workspace: a uint8 device tensor of
-    attention_kv8_workspace_bytes(...) bytes; by default one is allocated where the call needs it."""
+    attention_kv8_workspace_bytes(...) bytes; by default one is allocated where the call needs it, from the memory of the stream that it runs on
+    (results are, as in every call here, of the current stream's memory)."""
     what = "attention_kv8"
     _require(q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16), f"{what}: q must be [tokens, heads, head_dim] of f16 or bf16")
     cache = _kv8_cache(what, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type)
@@ -509,7 +521,7 @@ def attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, c
     lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if want_lse else None
     if workspace is None:
         need = _lib.ptoamd_attention_kv8_workspace_bytes(C.byref(cache), heads, tokens, most, max_length, window)
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        workspace = _temporary(need, q.device, stream) if need else None
     _check(_lib.ptoamd_attention_kv8(op, _ptr(lse), C.addressof(cache), qp, _SRC_TYPE[q.dtype], heads, tokens, cu, most, max_length, qt, qh, ot, oh,
                                      dim ** -0.5 if scale is None else scale, int(causal), window, _ptr(workspace),
                                      0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(stream)),

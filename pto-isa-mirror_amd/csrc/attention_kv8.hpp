@@ -4,6 +4,7 @@
 
 #include "common_host.hpp"
 #include "kv8.hpp"
+#include "kv8_places.hpp"
 #include "lds_dma.hpp"
 
 namespace ptoamd {
@@ -94,7 +95,7 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, int seq)
         s.count = min(max(load_uniform(c.cu_tokens + seq + 1), s.first) - s.first, min(c.max_tokens, c.tokens - s.first));
     }
     s.length = min(max(load_uniform(c.lengths + seq), 0), c.max_pages << c.page_shift);
-    s.begin = a.window > 0 ? max(s.length - s.count + 1 - a.window, 0) & ~31 : 0;
+    s.begin = first_key(s.length - s.count, a.window) & ~31;
     return s;
 }
 // Whether a sequence's keys are in several parts, which are joined; else its workgroups write what the call returns.
@@ -102,9 +103,7 @@ __device__ __forceinline__ bool several_parts(const AttentionArgs& a, const Span
 // The keys that a query at `place` of a sequence of `length` tokens sees: [x, y).
 __device__ __forceinline__ int2 visible_keys(const AttentionArgs& a, int place, int length)
 {
-    const int last = a.causal ? min(max(place + 1, 0), length) : length;
-    const int first = a.window > 0 ? max(place - a.window + 1, 0) : 0;
-    return make_int2(first, max(last, first));
+    return keys_of(place, length, a.causal, a.window);
 }
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

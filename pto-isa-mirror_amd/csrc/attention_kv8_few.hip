@@ -133,9 +133,9 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
         }
     }
     // tiles of keys that every row sees need no mask; keys that none sees have their codes cleared
-    const int every_from = a.window > 0 ? max(span.length - a.window, 0) : 0;
+    const int every_from = first_key(span.length - 1, a.window);
     const int every_to = a.causal ? span.length - span.count + 1 : span.length;
-    const int any_from = a.window > 0 ? max(span.length - span.count + 1 - a.window, 0) : 0;
+    const int any_from = first_key(span.length - span.count, a.window);
 
     f32x4 o[NT][MT];
     float top[NT], sum[NT];

@@ -1,0 +1,26 @@
+"""Attention over an 8-bit cache where queries stand before the first key and windows are as long as 32 bits hold."""
+import pytest
+import torch
+
+import kv8_reference as ref
+from test_gpu_attention_kv8 import queries
+from test_gpu_parity import pa  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31 - 40, 2 ** 30])
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("tokens", [3, 20, 300])
+@pytest.mark.parametrize("dim", [64, 128, 256, 72])
+def test_a_window_beyond_every_key_hides_none(pa, dim, tokens, causal, window):  # noqa: F811
+    """As without a window, bit for bit, idle sequences (no key, but queries) and queries before the first key among them."""
+    cache = ref.Cache("e4m3", [0, 2, 700, 5000], 2, dim, 64, 31)
+    counts = [tokens, tokens, tokens, 1]
+    q = queries(sum(counts), 8, dim, torch.bfloat16, 32)
+    print("window", dim, tokens, causal, window, flush=True)
+    kw = dict(cu_tokens=ref.starts(counts), max_tokens=tokens, causal=causal, want_lse=True)
+    plain = pa.attention_kv8(q, *cache.operands(pa), **kw)
+    ref.check_attention(plain[0], ref.attention(q, cache, counts, causal=causal), plain[1])
+    got = pa.attention_kv8(q, *cache.operands(pa), window=window, **kw)
+    assert torch.equal(got[0], plain[0]) and torch.equal(got[1], plain[1])

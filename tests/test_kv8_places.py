@@ -1,0 +1,32 @@
+"""Which keys a query of the attention over an 8-bit cache sees: the arithmetic that its kernels run, compiled for the host."""
+import ctypes
+import os
+
+import pytest
+
+LIB = os.path.join(os.path.dirname(os.path.abspath(__file__)), "pto_kernels", "build", "libkv8places.so")
+MOST = 2 ** 31 - 1
+
+
+@pytest.fixture(scope="module")
+def places():
+    assert os.path.exists(LIB), "build the test libraries first: make -C tests/pto_kernels"
+    return ctypes.CDLL(LIB)
+
+
+@pytest.mark.parametrize("causal", [False, True])
+def test_keys_by_their_definition(places, causal):
+    """0 <= j < length, j <= place (causal), j > place - window (window > 0): lengths, new tokens and windows from none to as many as 32 bits hold,
+    queries before the first key among them."""
+    x, y = ctypes.c_int(), ctypes.c_int()
+    for length in (0, 1, 2, 5, 16, 31, 1000, 2 ** 31 - 2 ** 20):
+        for count in (1, 2, 3, 9, 16, 4097, 2 ** 30, MOST):
+            for nth in {0, 1, count // 2, count - 1}:
+                place = length - count + nth
+                for window in (0, 1, 2, 5, 17, 1000, 2 ** 30, 2 ** 31 - 2 ** 20, MOST - 1, MOST):
+                    first = max(place - window + 1, 0) if window else 0
+                    end = min(length, max(place + 1, 0)) if causal else length
+                    assert places.kv8_first_key(place, window) == first, (length, count, nth, window)
+                    places.kv8_keys_of(place, length, int(causal), window, ctypes.byref(x), ctypes.byref(y))
+                    assert (x.value, y.value) == (first, max(end, first)), (length, count, nth, window)
+                    assert 0 <= x.value <= max(length, place + 1) and x.value <= y.value <= max(length, x.value)

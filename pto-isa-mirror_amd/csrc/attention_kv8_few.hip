@@ -221,13 +221,15 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
             }
             p[t] = make_uint4(pack_f16(w[0][0], w[0][1]), pack_f16(w[0][2], w[0][3]), pack_f16(w[1][0], w[1][1]), pack_f16(w[1][2], w[1][3]));
         }
-        if (key < any_from || key + 32 > span.length || vs[0] < LEAST_SCALE || vs[1] < LEAST_SCALE) {  // a weight of zero does not undo a NaN code
+        // A weight of zero does not undo a NaN code: those of places that no row sees, of pages that count as zeros, and what was read in place of a page
+        // that the table does not name (its scale is NaN, which is what makes the rows that do see it NaN).
+        if (key < any_from || key + 32 > span.length || !(vs[0] >= LEAST_SCALE) || !(vs[1] >= LEAST_SCALE)) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int at = key + 16 * (j / 4) + 4 * g + j % 4;
 #pragma unroll
                 for (int w = 0; w < VW; ++w)
-                    tile.v[j][w] = at < any_from || at >= span.length || vs[j / 4] < LEAST_SCALE ? 0u : tile.v[j][w];
+                    tile.v[j][w] = at < any_from || at >= span.length || !(vs[j / 4] >= LEAST_SCALE) ? 0u : tile.v[j][w];
             }
         }
         static_for<VW>([&](auto w_) {

@@ -197,6 +197,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         uint4 raw[UNITS];
         float2 raw_scale = make_float2(0, 0);
         float unit_scale[UNITS];  // of values: the scale of their page
+        uint32_t no_page = 0;     // bit u: the table names no page for unit u (asked of E4M3 codes, which may be NaN; no int8 code is)
         uint32_t source[UNITS], target[UNITS][2], none = 0;
         asm("" : "+v"(none));  // (a vector register's zero: a scale that is not read through the scalar cache, for which a barrier would wait)
         static_assert(SIDE_UNITS % THREADS == 0 || THREADS == 2 * SIDE_UNITS, "a unit is keys or values for all waves, or for half of them");
@@ -217,7 +218,10 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         };
         auto fetch = [&](int u, int stage) __attribute__((always_inline)) {
             const Kv8Side& side = is_value(u) ? c.v : c.k;
-            const uint32_t page = (unsigned)ids[u] < (unsigned)c.pages ? ids[u] : 0, slot = unit_key(u, stage) & slot_mask;
+            const bool known = (unsigned)ids[u] < (unsigned)c.pages;
+            const uint32_t page = known ? ids[u] : 0, slot = unit_key(u, stage) & slot_mask;
+            if (CODE != PTOAMD_I8)
+                no_page = known ? no_page & ~(1u << u) : no_page | 1u << u;
             const uint8_t* at = side.codes + ((uint64_t)page * (uint32_t)(side.page >> 3) * 8 + kv_head * side.head + slot * (uint32_t)side.token);
             raw[u] = *reinterpret_cast<const uint4*>(at + source[u]);
             unit_scale[u] = side.scales[page * (uint32_t)c.kv_heads + kv_head + none];
@@ -228,9 +232,9 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         auto piece = [&](auto u_, auto piece_, int stage) __attribute__((always_inline)) {
             constexpr int u = decltype(u_)::value, which = decltype(piece_)::value;
             if constexpr (which == 0) {
-                if (is_value(u)) {  // a weight of zero does not undo a NaN code that no row sees
+                if (is_value(u)) {  // a weight of zero does not undo a NaN code: of places that no row sees, or of what stands for a page that is none
                     const int own = unit_key(u, stage) + lane / (D / 16);
-                    const bool seen_by_some = (own >= from) & (own < to) & !(unit_scale[u] < LEAST_SCALE);
+                    const bool seen_by_some = (own >= from) & (own < to) & (unit_scale[u] >= ((no_page >> u & 1) != 0 ? NAN : LEAST_SCALE));
                     raw[u].x = seen_by_some ? raw[u].x : 0u;
                     raw[u].y = seen_by_some ? raw[u].y : 0u;
                     raw[u].z = seen_by_some ? raw[u].z : 0u;

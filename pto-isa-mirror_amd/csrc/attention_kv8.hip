@@ -119,6 +119,8 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     const int dim = built_head(c->head_dim);
     if (dim == 0)
         return p;
+    if (max_tokens > tokens)  // (a loose bound)
+        max_tokens = tokens;
     const long rows = (long)max_tokens * (heads / c->kv_heads);
     long keys = (long)c->max_pages * c->page_size;
     if (max_length > 0 && max_length < keys)

@@ -1,4 +1,4 @@
-// Which keys of a cache a query sees, by places in its sequence: what the attention's kernels index with, and its tests on the host.
+// Which keys of a cache a query sees, by places in its sequence: what the kernels around the cache index with, and their tests on the host.
 #pragma once
 #include <hip/hip_runtime.h>
 
@@ -12,6 +12,12 @@ __host__ __device__ __forceinline__ int2 keys_of(int place, int length, bool cau
 {
     const int behind = place + 1 < 0 ? 0 : place + 1, last = causal && behind < length ? behind : length, first = first_key(place, window);
     return make_int2(first, last > first ? last : first);
+}
+
+// The most pages that so many consecutive tokens lie in, wherever the first is; tokens > 0, up to 2^31 - 1.
+__host__ __device__ __forceinline__ int pages_of(int tokens, int page_shift)
+{
+    return ((tokens - 1) >> page_shift) + (((tokens - 1) & ((1 << page_shift) - 1)) != 0) + 1;
 }
 
 }  // namespace ptoamd

@@ -1,6 +1,7 @@
 // The append to a cache of keys and values held in 8 bits: new tokens are quantised into their pages, one scale a page and head.
 #include "common_host.hpp"
 #include "kv8.hpp"
+#include "kv8_places.hpp"
 #include "lds_dma.hpp"
 
 namespace ptoamd {
@@ -40,7 +41,7 @@ int kv8_from(const char* what, const ptoamd_kv8_cache* c, int tokens, const int3
     out->head_dim = c->head_dim;
     out->max_pages = c->max_pages;
     out->tokens = tokens;
-    out->max_tokens = max_tokens;
+    out->max_tokens = max_tokens < tokens ? max_tokens : tokens;  // (a loose bound: no sequence has more than all of them)
     return PTOAMD_OK;
 }
 
@@ -238,7 +239,7 @@ int ptoamd_kvcache_append(const ptoamd_kv8_cache* cache, const void* k, const vo
     a.token[1] = v_token_stride * size;
     a.head[0] = k_head_stride * size;
     a.head[1] = v_head_stride * size;
-    a.blocks = (max_tokens - 1 + cache->page_size - 1) / cache->page_size + 1;
+    a.blocks = pages_of(a.cache.max_tokens, a.cache.page_shift);
     PTOAMD_REQUIRE((long)cache->sequences * a.blocks <= 0x7FFFFFFF, PTOAMD_E_UNSUPPORTED, "ptoamd_kvcache_append: too many pages for one launch");
     hipStream_t s = as_stream(stream);
     switch (type) {

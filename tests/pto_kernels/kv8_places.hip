@@ -10,3 +10,4 @@ extern "C" void kv8_keys_of(int place, int length, int causal, int window, int* 
     *first = keys.x;
     *end = keys.y;
 }
+extern "C" int kv8_pages_of(int tokens, int page_shift) { return pages_of(tokens, page_shift); }

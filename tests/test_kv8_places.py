@@ -30,3 +30,22 @@ def test_keys_by_their_definition(places, causal):
                     places.kv8_keys_of(place, length, int(causal), window, ctypes.byref(x), ctypes.byref(y))
                     assert (x.value, y.value) == (first, max(end, first)), (length, count, nth, window)
                     assert 0 <= x.value <= max(length, place + 1) and x.value <= y.value <= max(length, x.value)
+
+
+@pytest.mark.parametrize("shift", [4, 5, 6, 7, 8])
+def test_the_most_pages_of_so_many_tokens(places, shift):
+    page = 1 << shift
+    for tokens in (1, 2, page - 1, page, page + 1, page + 2, 10 * page, 10 * page + 1, 2 ** 30 + 3, MOST - page, MOST - 1, MOST):
+        most = max((start + tokens - 1) // page - start // page + 1 for start in (0, 1, 2, page // 2, page - 2, page - 1))
+        assert places.kv8_pages_of(tokens, shift) == most, tokens
+
+
+def test_more_tokens_a_sequence_than_there_are():
+    """max_tokens bounds the sequences' tokens and may be loose; no sequence has more than all tokens, which is what work is planned for."""
+    import __graft_entry__ as ge
+    pa = ge.load_package()
+    lib = pa.lib()
+    for heads, kv_heads, dim, tokens in ((8, 8, 128, 4), (64, 8, 128, 4), (64, 8, 64, 300), (16, 2, 256, 70)):
+        cache = pa._Kv8Cache(pages=4096, kv_heads=kv_heads, page_size=64, head_dim=dim, sequences=2, max_pages=512)
+        need = [lib.ptoamd_attention_kv8_workspace_bytes(ctypes.byref(cache), heads, tokens, most, 0, window) for window in (0, 1000) for most in (tokens, tokens + 1, 2 ** 20, MOST)]
+        assert need[0] > 0 and set(need[:4]) == {need[0]} and set(need[4:]) == {need[4]}, need

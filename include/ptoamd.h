@@ -383,7 +383,7 @@ int ptoamd_rope(void* out, const void* x, int type, const float* table, int tabl
  *                   sees it gets NaN.
  *   lengths       : [sequences] int32, tokens of each sequence with the new ones (those of this step, whose keys are appended and
  *                   whose queries look back).  Taken as at least 0 and at most max_pages * page_size.
- *   page_size     : 16, 32, 64, 128 or 256
+ *   page_size     : 16, 32, 64, 128 or 256; max_pages * page_size is at most 2^31 - 2^16
  */
 typedef struct ptoamd_kv8_cache {
     void* k;

@@ -18,7 +18,8 @@ int kv8_from(const char* what, const ptoamd_kv8_cache* c, int tokens, const int3
     while (shift < 8 && (1 << shift) != c->page_size)
         ++shift;
     PTOAMD_REQUIRE(c->page_size == 1 << shift, PTOAMD_E_UNSUPPORTED, "%s: page_size must be 16, 32, 64, 128 or 256 (%d)", what, c->page_size);
-    PTOAMD_REQUIRE((long)c->max_pages * c->page_size <= 0x7FFFFF00L, PTOAMD_E_UNSUPPORTED, "%s: max_pages pages of %d tokens are too many", what, c->page_size);
+    // (places are held in 32 bits, and the attention's loops step up to 1040 of them past a sequence's last key)
+    PTOAMD_REQUIRE((long)c->max_pages * c->page_size <= 0x7FFF0000L, PTOAMD_E_UNSUPPORTED, "%s: max_pages pages of %d tokens are too many", what, c->page_size);
     PTOAMD_REQUIRE(c->kv_heads <= 65535 && c->sequences <= 65535, PTOAMD_E_UNSUPPORTED, "%s: more than 65535 key heads or sequences (%d, %d)", what, c->kv_heads,
                    c->sequences);
     PTOAMD_REQUIRE(tokens >= 0 && max_tokens >= 0, PTOAMD_E_INVALID, "%s: tokens and max_tokens must not be negative (%d, %d)", what, tokens, max_tokens);

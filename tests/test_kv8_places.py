@@ -49,3 +49,14 @@ def test_more_tokens_a_sequence_than_there_are():
         cache = pa._Kv8Cache(pages=4096, kv_heads=kv_heads, page_size=64, head_dim=dim, sequences=2, max_pages=512)
         need = [lib.ptoamd_attention_kv8_workspace_bytes(ctypes.byref(cache), heads, tokens, most, 0, window) for window in (0, 1000) for most in (tokens, tokens + 1, 2 ** 20, MOST)]
         assert need[0] > 0 and set(need[:4]) == {need[0]} and set(need[4:]) == {need[4]}, need
+
+
+def test_tables_of_nearly_as_many_places_as_32_bits_hold():
+    """Kernels step past a sequence's last key by up to 1040 places; a table whose places leave no room for that is refused."""
+    from test_kv8_refusals import call
+    for name in ("ptoamd_kvcache_append", "ptoamd_attention_kv8"):
+        for page, pages in ((256, 2 ** 23 - 1), (256, 2 ** 23 - 4), (16, 2 ** 27 - 16), (64, 2 ** 25 - 1023)):
+            rc, error = call(name, cache_page_size=page, cache_max_pages=pages, tokens=0, most=0)
+            assert rc == -2 and "too many" in error, (name, page, pages, rc)
+        for page, pages in ((256, 2 ** 23 - 256), (16, 2 ** 27 - 4096)):
+            assert call(name, cache_page_size=page, cache_max_pages=pages, tokens=0, most=0)[0] == 0

@@ -430,7 +430,8 @@ int ptoamd_kvcache_append(const ptoamd_kv8_cache* cache, const void* k, const vo
  *   max_length : at least every length; 0: max_pages * page_size is taken.  It sets how the work is split, so a tight bound helps.
  *   scale      : positive and finite
  *   workspace  : ptoamd_attention_kv8_workspace_bytes(...) bytes, 16-byte aligned, for work that is split over the keys of a sequence and
- *                joined (few rows, or ragged ones, over many keys).  Nothing in it is kept from one call to the next.  NULL: not split, slower for such calls.
+ *                joined (few rows, or ragged ones, over many keys): at most 288 MB.  Nothing in it is kept from one call to the next.  NULL: not split,
+ *                slower for such calls.
  * Sums of a softmax, of scores and of values are held in f32; the scores' products take q as f16 scaled by a power of two for each row
  * (bf16 and f16 queries lose nothing that is within 2^-14 of their row's largest element), the values' products take each weight, times its
  * page's value scale, rounded to f16 relative to the largest such so far: full f16 precision down to 2^-25 of that, nothing below 2^-36.  A

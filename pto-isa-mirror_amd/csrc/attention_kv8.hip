@@ -108,7 +108,9 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 //   4 / 1 heads, 47, 114 and 166 over 8642 234 / 39; heads of 64, 4 x 100 over 1024, 2000 33 / 43, 56 / 49; 8 / 2 of 256 (then in tiles of
 //   32 keys), over 512, 1024 40 / 39, 68 / 43.  (The same number of parts for every sequence instead, the best for each call: of these 512 over
 //   16384 163, the three of 6104 106, the four of 16000 204; but what the host knows did not tell which number, by a factor of up to 1.7.)
-// Parts have room for a sequence that is the only long one, within 256 MB.
+// Parts have room for a sequence that is the only long one, within PART_ROOM: of few rows fewer and longer ones where that is less, of many rows as
+// many as the mean tile of rows needs even so (271 MB at most, over three million sizes: rows that fill the card are not cut).
+constexpr long PART_ROOM = 256L << 20;  // bytes
 struct AttentionPlan {
     enum { GENERIC, FEW, MANY } kernel;
     int splits, chunk, row_tiles;
@@ -129,6 +131,7 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
         keys = (long)window + max_tokens + 31;
     const long cus = device_compute_units();
     const long items = (long)c->sequences * c->kv_heads;
+    const long room = PART_ROOM / ((long)tokens * heads * (dim * 4 + 8));  // parts
     const bool busy = items * keys * dim > 65536 * cus;
     p.kernel = rows <= (!busy ? 96 : dim == 256 ? 32 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
     if (p.kernel == AttentionPlan::FEW) {
@@ -141,6 +144,8 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
             splits = 1;
         const long even = (keys + 4095) / 4096;
         splits = splits > even ? splits : even;
+        const long most = room < 65535 ? room : 65535;  // (parts are a grid's slowest index)
+        splits = splits < most ? splits : most;
         if (splits > 1) {
             p.chunk = (int)(((keys + splits - 1) / splits + step - 1) / step * step);
             p.splits = (int)((keys + p.chunk - 1) / p.chunk);
@@ -154,7 +159,6 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     if (countable && keys * (1 - full) > 448 * full + 102400.0 / dim) {
         // (a tile's parts: its keys, at most twice the mean of one sequence's, in stretches of the mean; of several up to all stretches of a key head)
         const long mean = 2 * cus / tiles + 3, most = c->sequences > 1 ? cus / c->kv_heads + 2 : mean;
-        const long room = (256L << 20) / ((long)tokens * heads * (dim * 4 + 8));
         const long parts = most < room ? most : room;
         p.splits = (int)(parts > mean ? parts : mean);
     }

@@ -229,6 +229,8 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
     PTOAMD_REQUIRE(window >= 0 && max_length >= 0, PTOAMD_E_INVALID, "%s: window and max_length must not be negative (%d, %d)", what, window, max_length);
     if (tokens == 0 || max_tokens == 0)
         return PTOAMD_OK;
+    PTOAMD_REQUIRE((long)a.cache.max_tokens * (heads / cache->kv_heads) <= 0x7FFF0000L, PTOAMD_E_UNSUPPORTED,
+                   "%s: %d tokens of %d heads a key head are too many rows", what, a.cache.max_tokens, heads / cache->kv_heads);
     PTOAMD_REQUIRE(out && q, PTOAMD_E_INVALID, "%s: null operand", what);
     PTOAMD_REQUIRE((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % 2 == 0 && reinterpret_cast<uintptr_t>(lse) % 4 == 0, PTOAMD_E_ALIGNMENT,
                    "%s: q, out and lse must be aligned to their elements", what);

@@ -60,3 +60,12 @@ def test_tables_of_nearly_as_many_places_as_32_bits_hold():
             assert rc == -2 and "too many" in error, (name, page, pages, rc)
         for page, pages in ((256, 2 ** 23 - 256), (16, 2 ** 27 - 4096)):
             assert call(name, cache_page_size=page, cache_max_pages=pages, tokens=0, most=0)[0] == 0
+
+
+def test_more_rows_than_32_bits_number():
+    """A sequence's new tokens times the query heads of a key head are rows, numbered in 32 bits."""
+    from test_kv8_refusals import AT, call
+    for heads, tokens in ((65534, 2 ** 17), (64, 2 ** 28)):
+        for cu in (None, AT):
+            rc, error = call("ptoamd_attention_kv8", heads=heads, tokens=tokens if cu else 2 * tokens, most=tokens, cu=cu)
+            assert rc == -2 and "rows" in error, (rc, error)

@@ -407,7 +407,7 @@ typedef struct ptoamd_kv8_cache {
  * Appends new tokens' keys and values, k and v [tokens][kv_heads][head_dim] of `type` (PTOAMD_F32 | F16 | BF16).
  *   cu_tokens  : [sequences + 1] int32: rows cu_tokens[s] .. cu_tokens[s + 1] - 1 of k and v are sequence s's; they become its tokens
  *                lengths[s] - n .. lengths[s] - 1.  NULL: every sequence has max_tokens of them (tokens = sequences * max_tokens).
- *   max_tokens : at least every sequence's n
+ *   max_tokens : at least every sequence's n.  Rows that no sequence has, as far as cu_tokens and this say, are not read.
  * For each page that gets tokens, each head, K and V:  a = max |x| of the new ones;  s1 = max(s0, a * (1 / Q)) in f32, s0 being the page's
  * scale if it holds older tokens of the sequence and else 0, Q = 127 (int8) or 448 (E4M3), 1 / Q rounded to f32;  where s1 > s0 the older codes become
  * round(code * (s0 / s1));  new codes are round(x * (1 / s1)), ties to even, clamped.  The scale grows and never shrinks while a page
@@ -426,6 +426,8 @@ int ptoamd_kvcache_append(const ptoamd_kv8_cache* cache, const void* k, const vo
  *   s_j = scale * (q . k_j);  out = sum_j e^(s_j) v_j / sum_j e^(s_j);  lse = log sum_j e^(s_j)
  * heads is a multiple of kv_heads; query heads h * heads / kv_heads and on share key head h.  A query that sees no key gets zeros and
  * lse = -infinity.  What a query does not see has no influence on it; codes that no query of the sequence sees may be NaN codes.
+ * Rows of q that no sequence has (before cu_tokens[0], behind cu_tokens[sequences], beyond a sequence's max_tokens: a batch padded to the size of a
+ * captured step) are not read, and those rows of out and lse are not written.
  *   lse        : [tokens][heads] f32, or NULL
  *   max_length : at least every length; 0: max_pages * page_size is taken.  It sets how the work is split, so a tight bound helps.
  *   scale      : positive and finite

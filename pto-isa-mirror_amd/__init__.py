@@ -505,7 +505,8 @@ def attention_kv8_workspace_bytes(q, k_cache, block_table, max_tokens, max_lengt
 def attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, cu_tokens=None, max_tokens=None, max_length=0,
                   scale=None, causal=True, window=0, want_lse=False, stream=None, out=None, workspace=None):
     """Attention of q [tokens, heads, head_dim] (f16, bf16) over a cache that kvcache_append fills; query i of a sequence's n stands at
-    lengths[s] - n + i.  max_length: a bound on the lengths, where the caller has a tighter one than the block table.  scale: by default
+    lengths[s] - n + i.  Rows of a padded batch that cu_tokens gives to no sequence are not written, in `out` as in the log-sums: those of an `out`
+    that is allocated here hold whatever lay there.  max_length: a bound on the lengths, where the caller has a tighter one than the block table.  scale: by default
     head_dim ** -0.5.  want_lse: returns (out, lse), lse [tokens, heads] f32.  workspace: a uint8 device tensor of
     attention_kv8_workspace_bytes(...) bytes; by default one is allocated where the call needs it, from the memory of the stream that it runs on
     (results are, as in every call here, of the current stream's memory)."""

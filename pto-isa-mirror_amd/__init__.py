@@ -423,7 +423,8 @@ def rope_table(rows, rot_dim, base=10000.0, factor=1.0, ramp_low=0.0, ramp_high=
 def rope(x, table, positions, interleaved=False, backward=False, stream=None, out=None):
     """Rotary positions on the first table.shape[1] elements of every head of x [tokens, heads, head_dim] (f32, f16, bf16; tokens and
     heads at any stride, so the queries and keys of a fused product in one call).  table: of rope_table(); positions: [tokens] int32.
-    interleaved: pairs (2 i, 2 i + 1), else (i, i + half).  backward=True turns a gradient back.  out may be x."""
+    interleaved: pairs (2 i, 2 i + 1), else (i, i + half).  backward=True turns a gradient back.  out may be x.  (Autograd records none of the
+    package's calls: where x needs a gradient, the training step's own backward calls this with backward=True.)"""
     _require(x.dim() == 3 and x.dtype in _SRC_TYPE, "rope: x must be [tokens, heads, head_dim] of f32, f16 or bf16")
     tokens, heads, dim = x.shape
     _require(table.is_cuda and table.dim() == 2 and table.dtype == torch.float32 and table.is_contiguous(),

@@ -105,8 +105,8 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 //   128 tokens over 700, 1024, 1500 keys 30 / 35, 38 / 37, 52 / 39; 512 over 700, 1024, 1500, 2500, 16384 30 / 38, 38 / 42, 52 / 47, 78 / 55, 441 / 174;
 //   1024 over 1500, 2500 53 / 54, 80 / 71; 421, 376 and 512 over 6104, 4383 and 512 170 / 109; 3 x 512 over 6000 181 / 186; 4 x 256 over 1024, 512,
 //   341 and 146 39 / 43, over four times as many 117 / 70; 200, 512, 30 and 400 over 9000, 1200, 400 and 16000 440 / 213; 2 x 1024 over 8192 268 / 296;
-//   4 / 1 heads, 47, 114 and 166 over 8642 234 / 39; heads of 64, 4 x 100 over 1024, 2000 33 / 43, 56 / 49; 8 / 2 of 256 (then in tiles of
-//   32 keys), over 512, 1024 40 / 39, 68 / 43.  (The same number of parts for every sequence instead, the best for each call: of these 512 over
+//   4 / 1 heads, 47, 114 and 166 over 8642 234 / 39; heads of 64, 4 x 100 over 1024, 2000 33 / 43, 56 / 49; 8 / 2 of 256, 512 over 512, 700, 1024
+//   35 / 37, 43 / 38, 55 / 43; 128 over 400, 512, 700 32 / 35, 34 / 35, 42 / 37; 4 x 100 over 512, 1024 36 / 39, 56 / 42.  (The same number of parts for every sequence instead, the best for each call: of these 512 over
 //   16384 163, the three of 6104 106, the four of 16000 204; but what the host knows did not tell which number, by a factor of up to 1.7.)
 // Parts have room for a sequence that is the only long one, within PART_ROOM: of few rows fewer and longer ones where that is less, of many rows as
 // many as the mean tile of rows needs even so (271 MB at most, over three million sizes: rows that fill the card are not cut).

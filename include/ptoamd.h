@@ -15,7 +15,7 @@
  *       kernels/manual/a5/matmul_mxfp8_performance/mxmatmul_performance_kernel.cpp:360-380),
  *      each of which runs one TLOAD -> TMATMUL/TMATMUL_ACC -> TSTORE pipeline (or one TQUANT / TDEQUANT pass)
  *      over whole matrices in HBM;
- *   3. what stands between the products of a decoder layer: rotary positions, a cache of keys and values in 8 bits, attention over it.
+ *   3. what stands between the products of a decoder layer: rotary positions, a cache of keys and values in 8 bits, attention over it, drafted trees.
  */
 #ifndef PTOAMD_H
 #define PTOAMD_H
@@ -447,6 +447,70 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
                          const int32_t* cu_tokens, int max_tokens, int max_length, int64_t q_token_stride, int64_t q_head_stride,
                          int64_t out_token_stride, int64_t out_head_stride, float scale, int causal, int window, void* workspace,
                          size_t workspace_bytes, void* stream);
+
+/*
+ * Drafted trees.  Several continuations of a sequence are drafted as a tree of tokens, run through the model in one step, and one path of them is
+ * kept.  The drafted tokens are the sequence's newest: appended in their order to places lengths[s] - n .. lengths[s] - 1, whatever the tree's shape
+ * (parents before their children).  What a drafted token sees of the others is a row of bits: bit t of tree[token][t / 64] stands for the sequence's
+ * drafted token t.  Rows are tree_words 64-bit words long, 64 * tree_words >= max_tokens; bits of tokens that the sequence does not have are ignored.
+ * At most 256 tokens are drafted for a sequence.
+ *
+ * ptoamd_draft_tree makes the rows from parents: a token sees itself and its ancestors.
+ *   parents : [tokens] int32, the place of a token's parent among its sequence's drafted ones, or -1: the last token that is older.  A parent that
+ *             is neither -1 nor before the token leaves the token's row empty (and its descendants see nothing beyond the token).
+ *   tree    : [tokens][tree_words].  Rows that no sequence has are not written.
+ *   cu_tokens, max_tokens : as for the append below; NULL: tokens = sequences * max_tokens
+ */
+#define PTOAMD_MOST_DRAFTED 256
+int ptoamd_draft_tree(uint64_t* tree, int tree_words, const int32_t* parents, int tokens, int sequences, const int32_t* cu_tokens, int max_tokens,
+                      void* stream);
+
+/*
+ * ptoamd_rope of q and k and ptoamd_kvcache_append of k and v in one launch: queries [tokens][heads][head_dim] are turned into q_out, keys on their way
+ * into the cache, where they are quantised as they come from the rotation, in f32.  The definitions are those of the two calls, with one rounding of a
+ * key where they have two.  heads 0: only keys and values (q and q_out are then not looked at).
+ *   positions  : [tokens] int32, or NULL: a token's place in its sequence, lengths[s] - n + i; with `tree` (only without positions) a drafted token
+ *                stands behind the others that it sees: lengths[s] - n + the number of bits of its row without its own
+ *   type       : of q, k, v and q_out: PTOAMD_F32 | F16 | BF16
+ *   q_out      : may be q (with its strides), and overlap none of the operands in any other way
+ * A token whose position is not in 0 .. table_rows - 1 gets NaN for the rot_dim elements of its queries, and makes its page's key scales NaN.  Queries of
+ * tokens that have no place in the cache are turned as the others are.  Rows that no sequence has are neither read nor written.
+ */
+int ptoamd_kvcache_append_rope(const ptoamd_kv8_cache* cache, void* q_out, const void* q, int heads, const void* k, const void* v, int type, int tokens,
+                               const int32_t* cu_tokens, int max_tokens, const float* table, int table_rows, int rot_dim, int interleaved,
+                               const int32_t* positions, const uint64_t* tree, int tree_words, int64_t q_token_stride, int64_t q_head_stride,
+                               int64_t q_out_token_stride, int64_t q_out_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                               int64_t v_token_stride, int64_t v_head_stride, void* stream);
+
+/*
+ * Attention of drafted tokens: ptoamd_attention_kv8 with, in place of `causal`, rows of bits.  Query i of the n of a sequence of length L sees key j
+ *   where j < L - n and j > L - n + d - window (window > 0; d: the others that it sees among the drafted ones), and
+ *   where j = L - n + t, t >= 0 and bit t of its row is set.
+ * window is 0 or at least max_tokens, so that what a token sees of the tree lies within it.  Any bits are taken, a tree's or not: a query that sees
+ * nothing at all gets zeros and lse = -infinity.  Codes of drafted tokens must be numbers, whether a query sees them or not.
+ *   workspace : ptoamd_attention_kv8_tree_workspace_bytes(...) bytes, as for ptoamd_attention_kv8
+ */
+size_t ptoamd_attention_kv8_tree_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window);
+int ptoamd_attention_kv8_tree(void* out, float* lse, const ptoamd_kv8_cache* cache, const uint64_t* tree, int tree_words, const void* q, int type,
+                              int heads, int tokens, const int32_t* cu_tokens, int max_tokens, int max_length, int64_t q_token_stride,
+                              int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride, float scale, int window, void* workspace,
+                              size_t workspace_bytes, void* stream);
+
+/*
+ * Keeps a path of the drafted tokens: they move together behind the older ones, in the codes that they have.
+ *   kept        : [sequences][max_kept] int32: drafted tokens in ascending order.  A list ends at the first entry that is not above the one before, or
+ *                 is none of 0 .. n - 1 (so -1 fills it up); r entries are kept
+ *   new_lengths : [sequences] int32, gets lengths[s] - n + r.  Must not be lengths.
+ *   cu_tokens   : as for the append: n = cu_tokens[s + 1] - cu_tokens[s], at most max_tokens.  NULL: n = max_tokens
+ * Token kept[i] moves from place lengths[s] - n + kept[i] to lengths[s] - n + i.  Within a page its codes are copied.  Where tokens come into a page
+ * from others, a = max |code| * (scale of their page) of those, the page's scale becomes s1 = max(s0, a * (1 / Q)) as in an append; what was there and
+ * stays becomes round(code * (s0 / s1)) where s1 > s0, and what comes round(code * (scale of its page / s1)).  So a page keeps a scale that the
+ * tokens not kept have raised, until it is begun anew.  If a token comes from a page that the table does not name, or whose scale is NaN, the scale of
+ * the page that it comes to is NaN from then on; a page that the table does not name takes nothing.  Codes behind the kept tokens are left as they are.
+ * A sequence with lengths[s] < n, or beyond max_pages, is left as it is, with its length.
+ */
+int ptoamd_kvcache_keep(const ptoamd_kv8_cache* cache, int32_t* new_lengths, const int32_t* kept, int max_kept, const int32_t* cu_tokens, int max_tokens,
+                        void* stream);
 
 #ifdef __cplusplus
 }

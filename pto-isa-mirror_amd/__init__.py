@@ -40,6 +40,7 @@ _lib.ptoamd_gemm_mx_workspace_bytes_b_nd.restype = C.c_size_t
 _lib.ptoamd_gemm_workspace_bytes.restype = C.c_size_t
 _lib.ptoamd_gemv_mxfp4_packed_bytes.restype = C.c_size_t
 _lib.ptoamd_attention_kv8_workspace_bytes.restype = C.c_size_t
+_lib.ptoamd_attention_kv8_tree_workspace_bytes.restype = C.c_size_t
 
 EXPORTS = [
     "ptoamd_init", "ptoamd_finalize", "ptoamd_last_error", "ptoamd_device_info", "ptoamd_malloc", "ptoamd_free",
@@ -52,6 +53,7 @@ EXPORTS = [
     "ptoamd_tquant_int8_para", "ptoamd_tquant_mx", "ptoamd_tdequant", "ptoamd_tdequant_para", "ptoamd_mx_scale_relayout",
     "ptoamd_last_kernel", "ptoamd_reload_options",
     "ptoamd_rope_table", "ptoamd_rope", "ptoamd_kvcache_append", "ptoamd_attention_kv8_workspace_bytes", "ptoamd_attention_kv8",
+    "ptoamd_draft_tree", "ptoamd_kvcache_append_rope", "ptoamd_attention_kv8_tree_workspace_bytes", "ptoamd_attention_kv8_tree", "ptoamd_kvcache_keep",
 ]
 
 # Argument types of the entry points called below (p: device address or stream, i: int, l: int64_t, z: size_t, f: float, d: double): with them ctypes takes plain
@@ -81,6 +83,10 @@ _SIGNATURES = {
     "ptoamd_rope": "ppipip" + "iiii" + "llll" + "ii" + "p",
     "ptoamd_kvcache_append": "pppiipi" + "llll" + "p",
     "ptoamd_attention_kv8": "ppppiiipii" + "llll" + "fii" + "pzp",
+    "ptoamd_draft_tree": "pipiipi" + "p",
+    "ptoamd_kvcache_append_rope": "pppippiipipiiippi" + "llllllll" + "p",
+    "ptoamd_attention_kv8_tree": "ppppipiiipii" + "llll" + "fi" + "pzp",
+    "ptoamd_kvcache_keep": "pppipi" + "p",
 }
 for _name, _sig in _SIGNATURES.items():
     getattr(_lib, _name).argtypes = [{"p": C.c_void_p, "i": C.c_int, "l": C.c_int64, "z": C.c_size_t, "f": C.c_float, "d": C.c_double}[c]
@@ -531,6 +537,120 @@ def attention_kv8(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, c
     return (out, lse) if want_lse else out
 
 
+# ---- drafted trees over the 8-bit cache --------------------------------------------------------------------------------------
+MOST_DRAFTED = 256  # tokens of a sequence
+
+
+def _tree(t, tokens, what):
+    """(address of the rows, 64-bit words of a row)"""
+    if t is None:
+        return None, 0
+    _require(t.is_cuda and t.dtype == torch.int64 and t.dim() == 2 and t.shape[0] == tokens and t.is_contiguous(),
+             f"{what} must be a contiguous int64 device tensor [tokens, words] of {tokens} tokens")
+    return t.data_ptr(), t.shape[1]
+
+
+def draft_tree(parents, sequences, cu_tokens=None, max_tokens=None, stream=None, out=None):
+    """What each drafted token sees of those drafted with it, itself and its ancestors, as rows of bits: [tokens, ceil(max_tokens / 64)] int64,
+    bit t % 64 of word t / 64 for its sequence's token t.  parents [tokens] int32: a token's parent among its sequence's, before it, or -1 (the
+    last token that is older); any other value leaves the token's row empty.  cu_tokens [sequences + 1]: where each sequence's tokens start (None: equal
+    shares); at most 256 tokens a sequence.  Rows that cu_tokens gives to no sequence are not written."""
+    what = "draft_tree"
+    _require(parents.dim() == 1, f"{what}: parents must be [tokens]")
+    tokens = parents.shape[0]
+    cu, most = _tokens_of(what, tokens, sequences, cu_tokens, max_tokens)
+    if out is None:
+        out = torch.empty((tokens, max(1, (min(most, tokens) + 63) // 64)), dtype=torch.int64, device=parents.device)
+    address, words = _tree(out, tokens, f"{what}: out")
+    _check(_lib.ptoamd_draft_tree(address, words, _int32(parents, (tokens,), f"{what}: parents"), tokens, sequences, cu, most, _stream(stream)),
+           "ptoamd_draft_tree")
+    return out
+
+
+def kvcache_append_rope(q, k, v, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, table, positions=None, tree=None,
+                        interleaved=False, cu_tokens=None, max_tokens=None, stream=None, out=None):
+    """rope() of q and k and kvcache_append() of k and v in one launch: returns the turned queries [tokens, heads, head_dim] (q None: turns keys
+    only, returns None) and changes the caches and scales in place.  A key is rounded once, to its code.  table: of rope_table().  positions
+    [tokens] int32; by default a token's place in its sequence, or with tree (rows of draft_tree()) the place behind the others that it sees.
+    out may be q; rows of a padded batch that no sequence has are not written."""
+    what = "kvcache_append_rope"
+    _require(k.dim() == 3 and k.dtype in _SRC_TYPE, f"{what}: k must be [tokens, kv_heads, head_dim] of f32, f16 or bf16")
+    _require(table.is_cuda and table.dim() == 2 and table.dtype == torch.float32 and table.is_contiguous(),
+             f"{what}: table must be a contiguous f32 device tensor [rows, rot_dim]")
+    _require(positions is None or tree is None, f"{what}: a token's position is given or follows from the tree, not both")
+    cache = _kv8_cache(what, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type)
+    tokens = k.shape[0]
+    kp, kt, kh = _heads(k, (tokens, cache.kv_heads, cache.head_dim), f"{what}: k")
+    vp, vt, vh = _heads(v, k.shape, f"{what}: v", k.dtype)
+    cu, most = _tokens_of(what, tokens, cache.sequences, cu_tokens, max_tokens)
+    at = None if positions is None else _int32(positions, (tokens,), f"{what}: positions")
+    bits, words = _tree(tree, tokens, f"{what}: tree")
+    qp = qt = qh = op = ot = oh = heads = 0
+    if q is None:
+        _require(out is None, f"{what}: out is for queries")
+    else:
+        _require(q.dim() == 3, f"{what}: q must be [tokens, heads, head_dim]")
+        heads = q.shape[1]
+        qp, qt, qh = _heads(q, (tokens, heads, cache.head_dim), f"{what}: q", k.dtype)
+        if out is None:
+            out = torch.empty((tokens, heads, cache.head_dim), dtype=q.dtype, device=q.device)
+        op, ot, oh = _heads(out, q.shape, f"{what}: out", q.dtype)
+    _check(_lib.ptoamd_kvcache_append_rope(C.addressof(cache), op, qp, heads, kp, vp, _SRC_TYPE[k.dtype], tokens, cu, most, table.data_ptr(), table.shape[0],
+                                           table.shape[1], int(interleaved), at, bits, words, qt, qh, ot, oh, kt, kh, vt, vh, _stream(stream)),
+           "ptoamd_kvcache_append_rope")
+    return out
+
+
+def attention_kv8_tree_workspace_bytes(q, k_cache, block_table, max_tokens, max_length=0, window=0):
+    """Bytes of workspace that attention_kv8_tree of these sizes splits its work with (0: not split)."""
+    pages, heads, page, dim = k_cache.shape
+    cache = _Kv8Cache(pages=pages, kv_heads=heads, page_size=page, head_dim=dim, sequences=block_table.shape[0], max_pages=block_table.shape[1])
+    return int(_lib.ptoamd_attention_kv8_tree_workspace_bytes(C.byref(cache), q.shape[1], q.shape[0], max_tokens, max_length, window))
+
+
+def attention_kv8_tree(q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, tree, cu_tokens=None, max_tokens=None, max_length=0,
+                       scale=None, window=0, want_lse=False, stream=None, out=None, workspace=None):
+    """attention_kv8() of drafted tokens, the newest of each sequence, appended in their order: a query sees what is older than the step and, of the
+    step, the tokens whose bits its row of tree has (draft_tree(), or any bits).  window: 0 or at least max_tokens; a query stands behind the
+    others that it sees.  The other arguments are attention_kv8's (workspace: of attention_kv8_tree_workspace_bytes(...) bytes)."""
+    what = "attention_kv8_tree"
+    _require(q.dim() == 3 and q.dtype in (torch.float16, torch.bfloat16), f"{what}: q must be [tokens, heads, head_dim] of f16 or bf16")
+    cache = _kv8_cache(what, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type)
+    tokens, heads, dim = q.shape
+    qp, qt, qh = _heads(q, (tokens, heads, cache.head_dim), f"{what}: q")
+    bits, words = _tree(tree, tokens, f"{what}: tree")
+    cu, most = _tokens_of(what, tokens, cache.sequences, cu_tokens, max_tokens)
+    if out is None:
+        out = torch.empty((tokens, heads, dim), dtype=q.dtype, device=q.device)
+    op, ot, oh = _heads(out, q.shape, f"{what}: out", q.dtype)
+    lse = torch.empty((tokens, heads), dtype=torch.float32, device=q.device) if want_lse else None
+    if workspace is None:
+        need = _lib.ptoamd_attention_kv8_tree_workspace_bytes(C.byref(cache), heads, tokens, most, max_length, window)
+        workspace = _temporary(need, q.device, stream) if need else None
+    _check(_lib.ptoamd_attention_kv8_tree(op, _ptr(lse), C.addressof(cache), bits, words, qp, _SRC_TYPE[q.dtype], heads, tokens, cu, most, max_length, qt, qh,
+                                          ot, oh, dim ** -0.5 if scale is None else scale, window, _ptr(workspace),
+                                          0 if workspace is None else workspace.numel() * workspace.element_size(), _stream(stream)),
+           "ptoamd_attention_kv8_tree")
+    return (out, lse) if want_lse else out
+
+
+def kvcache_keep(kept, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, cu_tokens=None, max_tokens=None, stream=None, out=None):
+    """Keeps a path of each sequence's drafted tokens: kept [sequences, most] int32, ascending, -1 behind the last; they move together behind what is
+    older, in the cache's codes.  Returns the new lengths [sequences] (out: into that tensor, not lengths itself).  A sequence has
+    cu_tokens[s + 1] - cu_tokens[s] drafted tokens, at most max_tokens; without cu_tokens max_tokens each."""
+    what = "kvcache_keep"
+    cache = _kv8_cache(what, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type)
+    _require(kept.dim() == 2, f"{what}: kept must be [sequences, most]")
+    _require(max_tokens is not None, f"{what}: needs max_tokens, the most drafted tokens of a sequence")
+    cu = None if cu_tokens is None else _int32(cu_tokens, (cache.sequences + 1,), f"{what}: cu_tokens")
+    if out is None:
+        out = torch.empty((cache.sequences,), dtype=torch.int32, device=lengths.device)
+    _check(_lib.ptoamd_kvcache_keep(C.addressof(cache), _int32(out, (cache.sequences,), f"{what}: out"),
+                                    _int32(kept, (cache.sequences, kept.shape[1]), f"{what}: kept"), kept.shape[1], cu, max_tokens, _stream(stream)),
+           "ptoamd_kvcache_keep")
+    return out
+
+
 # ---- the entry points above as native callables (binding/entry_points.cpp): they take the plain calls and hand every other one to the
 # function of that name above
 def _native_entry_points():
@@ -551,7 +671,8 @@ def _native_entry_points():
         warnings.warn(f"{path} is not used, calls take the slower way through ctypes: {e}", RuntimeWarning, stacklevel=2)
         return
     binding.set_error(PtoAmdError)
-    for f in (gemm, gemm_w8a8, gemm_mx, gemv_mxfp4, gemv_mxfp4_packed, tquant_int8, tquant_mx, tdequant, rope, kvcache_append, attention_kv8):
+    for f in (gemm, gemm_w8a8, gemm_mx, gemv_mxfp4, gemv_mxfp4_packed, tquant_int8, tquant_mx, tdequant, rope, kvcache_append, attention_kv8,
+              draft_tree, kvcache_append_rope, attention_kv8_tree, kvcache_keep):
         globals()[f.__name__] = binding.entry_point(f)
 
 

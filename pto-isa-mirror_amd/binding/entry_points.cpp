@@ -493,6 +493,169 @@ PyObject* attention_kv8(const Call& c)
     return result;
 }
 
+// rows of drafted tokens' bits, or none
+const uint64_t* tree_of(const Call& c, int at, int tokens, int* words)
+{
+    *words = 0;
+    if (!c.given(at))
+        return nullptr;
+    const at::Tensor& t = c.typed(at, 2, at::kLong);
+    if (t.size(0) != tokens)
+        throw NotPlain{};
+    *words = extent(t.size(1));
+    return address_as<const uint64_t>(t);
+}
+
+// parents, sequences, cu_tokens, max_tokens, stream, out
+PyObject* draft_tree(const Call& c)
+{
+    c.only_default(4);
+    const at::Tensor& parents = c.typed(0, 1, at::kInt);
+    const int tokens = extent(parents.size(0));
+    ptoamd_kv8_cache sequences{};
+    sequences.sequences = c.integer(1);
+    if (sequences.sequences < 0)
+        throw NotPlain{};
+    int most = 0, words = 0;
+    const int32_t* cu = tokens_of(c, 2, tokens, sequences, &most);
+    at::Tensor out;
+    if (c.given(5)) {
+        tree_of(c, 5, tokens, &words);
+        out = c.typed(5, 2, at::kLong);
+    }
+    {
+        Released no_gil;
+        if (!out.defined()) {
+            const int rows = most < tokens ? most : tokens;
+            words = rows > 64 ? (rows + 63) / 64 : 1;
+            out = empty({tokens, words}, at::kLong, parents);
+        }
+        check(ptoamd_draft_tree(address_as<uint64_t>(out), words, address_as<const int32_t>(parents), tokens, sequences.sequences, cu, most, stream()),
+              "ptoamd_draft_tree");
+    }
+    return wrap(std::move(out));
+}
+
+// q, k, v, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, table, positions, tree, interleaved, cu_tokens, max_tokens, stream, out
+PyObject* kvcache_append_rope(const Call& c)
+{
+    c.only_default(16);
+    const at::Tensor &q = c.rows(0, 3), &k = c.rows(1, 3), &v = c.rows(2, 3), &table = c.typed(10, 2, at::kFloat);
+    const ptoamd_kv8_cache cache = kv8_cache(c, 3);
+    const int type = real_type(k), tokens = extent(k.size(0)), heads = extent(q.size(1)), rows = extent(table.size(0)), rot = extent(table.size(1));
+    if (k.size(1) != cache.kv_heads || k.size(2) != cache.head_dim || v.sizes() != k.sizes() || v.scalar_type() != k.scalar_type() || q.size(0) != tokens ||
+        q.size(2) != cache.head_dim || q.scalar_type() != k.scalar_type())
+        throw NotPlain{};
+    const int32_t* positions = nullptr;
+    if (c.given(11)) {
+        const at::Tensor& t = c.typed(11, 1, at::kInt);
+        if (t.size(0) != tokens)
+            throw NotPlain{};
+        positions = address_as<const int32_t>(t);
+    }
+    int most = 0, words = 0;
+    const uint64_t* tree = tree_of(c, 12, tokens, &words);
+    if (positions != nullptr && tree != nullptr)
+        throw NotPlain{};
+    const bool interleaved = c.truth(13, false);
+    const int32_t* cu = tokens_of(c, 14, tokens, cache, &most);
+    at::Tensor out;
+    if (c.given(17))
+        out = c.rows(17, 3);
+    if (out.defined() && (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type()))
+        throw NotPlain{};
+    {
+        Released no_gil;
+        if (!out.defined())
+            out = empty(q.sizes(), q.scalar_type(), q);
+        check(ptoamd_kvcache_append_rope(&cache, address(out), address(q), heads, address(k), address(v), type, tokens, cu, most, address_as<const float>(table),
+                                         rows, rot, interleaved, positions, tree, words, q.stride(0), q.stride(1), out.stride(0), out.stride(1), k.stride(0),
+                                         k.stride(1), v.stride(0), v.stride(1), stream()),
+              "ptoamd_kvcache_append_rope");
+    }
+    return wrap(std::move(out));
+}
+
+// q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, tree, cu_tokens, max_tokens, max_length, scale, window, want_lse, stream, out,
+// workspace
+PyObject* attention_kv8_tree(const Call& c)
+{
+    c.only_default(15);
+    const at::Tensor& q = c.rows(0, 3);
+    const ptoamd_kv8_cache cache = kv8_cache(c, 1);
+    const int type = real_type(q), tokens = extent(q.size(0)), heads = extent(q.size(1));
+    if (type == PTOAMD_F32 || q.size(2) != cache.head_dim || !c.given(8))
+        throw NotPlain{};
+    int most = 0, words = 0;
+    const uint64_t* tree = tree_of(c, 8, tokens, &words);
+    const int32_t* cu = tokens_of(c, 9, tokens, cache, &most);
+    const int max_length = c.integer(11, 0), window = c.integer(13, 0);
+    const double scale = c.given(12) ? c.real(12) : 1.0 / std::sqrt((double)cache.head_dim);
+    const bool want_lse = c.truth(14, false);
+    at::Tensor out, lse, workspace;
+    if (c.given(16))
+        out = c.rows(16, 3);
+    if (c.given(17))
+        workspace = c.tensor(17, 1, false);
+    if (out.defined() && (out.sizes() != q.sizes() || out.scalar_type() != q.scalar_type()))
+        throw NotPlain{};
+    {
+        Released no_gil;
+        if (!out.defined())
+            out = empty(q.sizes(), q.scalar_type(), q);
+        if (want_lse)
+            lse = empty({tokens, heads}, at::kFloat, q);
+        if (!workspace.defined()) {
+            const size_t need = ptoamd_attention_kv8_tree_workspace_bytes(&cache, heads, tokens, most, max_length, window);
+            if (need != 0)
+                workspace = empty({(int64_t)need}, at::kByte, q);
+        }
+        check(ptoamd_attention_kv8_tree(address(out), want_lse ? address_as<float>(lse) : nullptr, &cache, tree, words, address(q), type, heads, tokens, cu,
+                                        most, max_length, q.stride(0), q.stride(1), out.stride(0), out.stride(1), (float)scale, window,
+                                        workspace.defined() ? address(workspace) : nullptr, workspace.defined() ? workspace.nbytes() : 0, stream()),
+              "ptoamd_attention_kv8_tree");
+    }
+    if (!want_lse)
+        return wrap(std::move(out));
+    PyObject* result = PyTuple_New(2);
+    if (result == nullptr)
+        return nullptr;
+    PyTuple_SET_ITEM(result, 0, wrap(std::move(out)));
+    PyTuple_SET_ITEM(result, 1, wrap(std::move(lse)));
+    return result;
+}
+
+// kept, k_cache, v_cache, k_scale, v_scale, block_table, lengths, code_type, cu_tokens, max_tokens, stream, out
+PyObject* kvcache_keep(const Call& c)
+{
+    c.only_default(10);
+    const at::Tensor& kept = c.typed(0, 2, at::kInt);
+    const ptoamd_kv8_cache cache = kv8_cache(c, 1);
+    const int most = c.integer(9);
+    if (kept.size(0) != cache.sequences)
+        throw NotPlain{};
+    const int32_t* cu = nullptr;
+    if (c.given(8)) {
+        const at::Tensor& t = c.typed(8, 1, at::kInt);
+        if (t.size(0) != (int64_t)cache.sequences + 1)
+            throw NotPlain{};
+        cu = address_as<const int32_t>(t);
+    }
+    at::Tensor out;
+    if (c.given(11))
+        out = c.typed(11, 1, at::kInt);
+    if (out.defined() && out.size(0) != cache.sequences)
+        throw NotPlain{};
+    const int max_kept = extent(kept.size(1));
+    {
+        Released no_gil;
+        if (!out.defined())
+            out = empty({cache.sequences}, at::kInt, kept);
+        check(ptoamd_kvcache_keep(&cache, address_as<int32_t>(out), address_as<const int32_t>(kept), max_kept, cu, most, stream()), "ptoamd_kvcache_keep");
+    }
+    return wrap(std::move(out));
+}
+
 struct Native {
     const char* name;
     PyObject* (*run)(const Call&);
@@ -513,6 +676,13 @@ const Native natives[] = {
                                            "max_tokens", "stream"}},
     {"attention_kv8", attention_kv8, 8, {"q", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "lengths", "code_type", "cu_tokens", "max_tokens",
                                          "max_length", "scale", "causal", "window", "want_lse", "stream", "out", "workspace"}},
+    {"draft_tree", draft_tree, 2, {"parents", "sequences", "cu_tokens", "max_tokens", "stream", "out"}},
+    {"kvcache_append_rope", kvcache_append_rope, 11, {"q", "k", "v", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "lengths", "code_type", "table",
+                                                      "positions", "tree", "interleaved", "cu_tokens", "max_tokens", "stream", "out"}},
+    {"attention_kv8_tree", attention_kv8_tree, 9, {"q", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "lengths", "code_type", "tree", "cu_tokens",
+                                                   "max_tokens", "max_length", "scale", "window", "want_lse", "stream", "out", "workspace"}},
+    {"kvcache_keep", kvcache_keep, 8, {"kept", "k_cache", "v_cache", "k_scale", "v_scale", "block_table", "lengths", "code_type", "cu_tokens", "max_tokens",
+                                       "stream", "out"}},
 };
 
 // ---- the callable -------------------------------------------------------------------------------------------------------

@@ -5,8 +5,8 @@ namespace ptoamd {
 
 // One wave a query and head, in f32 throughout: a lane's key of 64 at a time, then a lane's elements of the result.  Any head_dim that
 // is a multiple of 8 up to 512, any number of queries: what the other kernels are checked against, and what head sizes without a kernel
-// of their own run on.
-template <typename T, int CODE>
+// of their own run on.  TREE: of drafted tokens, which see the older keys and the bits of their row.
+template <typename T, int CODE, bool TREE>
 __global__ void __launch_bounds__(64) attention_kv8_generic_kernel(AttentionArgs a)
 {
     const Kv8& c = a.cache;
@@ -15,8 +15,10 @@ __global__ void __launch_bounds__(64) attention_kv8_generic_kernel(AttentionArgs
     if (nth >= count)
         return;
     const int length = c.length(seq), dim = c.head_dim;
-    const int2 keys = visible_keys(a, length - count + nth, length);
-    __shared__ float q[512], weight[64];
+    const int old = length - count;
+    const uint32_t* bits = TREE ? a.tree + (int64_t)(first + nth) * a.tree_words : nullptr;
+    const int2 keys = TREE ? make_int2(first_key(old + others_seen(bits, a.tree_words, count, nth), a.window), length) : visible_keys(a, old + nth, length);
+    __shared__ float q[512], weight[64];  // (weights below 0: of keys that are not seen)
     const T* row = reinterpret_cast<const T*>(a.q + (int64_t)(first + nth) * a.q_token + (int64_t)head * a.q_head);
     for (int i = lane; i < dim; i += 64)
         q[i] = (float)row[i];
@@ -28,7 +30,10 @@ __global__ void __launch_bounds__(64) attention_kv8_generic_kernel(AttentionArgs
         __syncthreads();  // q; the weights of the tile before have been read
         const int key = base + lane;
         float s = -INFINITY;
-        if (key < keys.y) {
+        bool seen = key < keys.y;
+        if (TREE && seen && key >= old)
+            seen = (row_bits(bits, a.tree_words, key - old) & 1u) != 0;
+        if (seen) {
             const int page = c.page_of(seq, key >> c.page_shift), slot = key & ((1 << c.page_shift) - 1);
             const uint8_t* k = c.k.codes + (int64_t)max(page, 0) * c.k.page + (int64_t)kv_head * c.k.head + (int64_t)slot * c.k.token;
             float dot = 0.0f;
@@ -53,13 +58,15 @@ __global__ void __launch_bounds__(64) attention_kv8_generic_kernel(AttentionArgs
         for (int d = 32; d > 0; d >>= 1)
             sum += __shfl_xor(sum, d);
         total = total * fade + sum;
-        weight[lane] = p;
+        weight[lane] = seen ? p : -1.0f;
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             o[i] *= fade;
         for (int j = 0; j < min(64, keys.y - base); ++j) {
             const float w = weight[j];
+            if (TREE && w < 0.0f)
+                continue;
             const int page = c.page_of(seq, (base + j) >> c.page_shift), slot = (base + j) & ((1 << c.page_shift) - 1);
             const uint8_t* v = c.v.codes + (int64_t)max(page, 0) * c.v.page + (int64_t)kv_head * c.v.head + (int64_t)slot * c.v.token;
             const float wv = page < 0 ? NAN : w * c.v.scales[(int64_t)page * c.kv_heads + kv_head];
@@ -82,7 +89,11 @@ __global__ void __launch_bounds__(64) attention_kv8_generic_kernel(AttentionArgs
 template <typename T, int CODE>
 static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
-    hipLaunchKernelGGL((attention_kv8_generic_kernel<T, CODE>), dim3((unsigned)a.cache.max_tokens, (unsigned)a.heads, (unsigned)sequences), dim3(64), 0, stream, a);
+    const dim3 grid((unsigned)a.cache.max_tokens, (unsigned)a.heads, (unsigned)sequences);
+    if (a.tree != nullptr)
+        hipLaunchKernelGGL((attention_kv8_generic_kernel<T, CODE, true>), grid, dim3(64), 0, stream, a);
+    else
+        hipLaunchKernelGGL((attention_kv8_generic_kernel<T, CODE, false>), grid, dim3(64), 0, stream, a);
     PTOAMD_HIP_CHECK(hipGetLastError());
     set_last_kernel("attention_kv8_generic");
     return PTOAMD_OK;
@@ -191,31 +202,17 @@ int prepare_attention_kernels()
     return PTOAMD_OK;
 }
 
-}  // namespace ptoamd
-
-using namespace ptoamd;
-
-extern "C" {
-
-size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window)
+// The call of both entry points: `causal`, or `tree` with rows of tree_words 64-bit words.
+static int attention(const char* what, void* out, float* lse, const ptoamd_kv8_cache* cache, const uint64_t* tree, int tree_words, const void* q, int type,
+                     int heads, int tokens, const int32_t* cu_tokens, int max_tokens, int max_length, int64_t q_token_stride, int64_t q_head_stride,
+                     int64_t out_token_stride, int64_t out_head_stride, float scale, int causal, int window, void* workspace, size_t workspace_bytes,
+                     void* stream)
 {
-    if (cache == nullptr || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads != 0 || tokens <= 0 || max_tokens <= 0 || cache->sequences <= 0 ||
-        cache->max_pages <= 0 || cache->page_size <= 0)
-        return 0;
-    return part_bytes(plan_attention(cache, heads, tokens, max_tokens, max_length, window), heads, tokens, built_head(cache->head_dim));
-}
-
-int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, const void* q, int type, int heads, int tokens,
-                         const int32_t* cu_tokens, int max_tokens, int max_length, int64_t q_token_stride, int64_t q_head_stride,
-                         int64_t out_token_stride, int64_t out_head_stride, float scale, int causal, int window, void* workspace,
-                         size_t workspace_bytes, void* stream)
-{
-    const char* what = "ptoamd_attention_kv8";
     AttentionArgs a{};
     const int checked = kv8_from(what, cache, tokens, cu_tokens, max_tokens, &a.cache);
     if (checked != PTOAMD_OK)
         return checked;
-    TraceScope trace("ATTENTION_KV8", "mix", tokens, heads, cache->head_dim);
+    TraceScope trace(tree != nullptr ? "ATTENTION_KV8_TREE" : "ATTENTION_KV8", "mix", tokens, heads, cache->head_dim);
     trace.in(q, tokens, (long)heads * cache->head_dim, "ND", type)
         .in(cache->k, cache->pages, (long)cache->kv_heads * cache->page_size * cache->head_dim, "ND", cache->code_type)
         .in(cache->v, cache->pages, (long)cache->kv_heads * cache->page_size * cache->head_dim, "ND", cache->code_type)
@@ -246,6 +243,8 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
     a.causal = causal != 0;
     a.window = window;
     a.scale = scale;
+    a.tree = reinterpret_cast<const uint32_t*>(tree);
+    a.tree_words = 2 * tree_words;
     hipStream_t s = as_stream(stream);
     const bool i8 = cache->code_type == PTOAMD_I8, f16 = type == PTOAMD_F16;
     const AttentionPlan plan = plan_attention(cache, heads, tokens, max_tokens, max_length, window);
@@ -258,7 +257,7 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
     const bool addressable = cache->k_page_stride >= 0 && cache->k_page_stride < 1LL << 34 && cache->v_page_stride >= 0 && cache->v_page_stride < 1LL << 34 &&
                              cache->k_token_stride >= 0 && cache->k_token_stride < 1 << 22 && cache->v_token_stride >= 0 && cache->v_token_stride < 1 << 22 &&
                              (long)cache->pages * cache->kv_heads < 1L << 30;
-    if (plan.kernel != AttentionPlan::GENERIC && cache_bits % 16 == 0 && addressable && !options().force_generic) {
+    if (plan.kernel != AttentionPlan::GENERIC && cache_bits % 16 == 0 && addressable && !options().force_generic && tree == nullptr) {
         a.wide = ((uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)out | (uint64_t)a.q_token | (uint64_t)a.q_head | (uint64_t)a.out_token | (uint64_t)a.out_head) % 16 == 0;
         a.splits = workspace != nullptr ? plan.splits : 1;
         a.chunk = plan.chunk;
@@ -277,6 +276,53 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
     if (type == PTOAMD_F16)
         return i8 ? launch_generic<_Float16, PTOAMD_I8>(a, cache->sequences, s) : launch_generic<_Float16, PTOAMD_E4M3>(a, cache->sequences, s);
     return i8 ? launch_generic<__bf16, PTOAMD_I8>(a, cache->sequences, s) : launch_generic<__bf16, PTOAMD_E4M3>(a, cache->sequences, s);
+}
+
+}  // namespace ptoamd
+
+using namespace ptoamd;
+
+extern "C" {
+
+size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window)
+{
+    if (cache == nullptr || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads != 0 || tokens <= 0 || max_tokens <= 0 || cache->sequences <= 0 ||
+        cache->max_pages <= 0 || cache->page_size <= 0)
+        return 0;
+    return part_bytes(plan_attention(cache, heads, tokens, max_tokens, max_length, window), heads, tokens, built_head(cache->head_dim));
+}
+
+int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, const void* q, int type, int heads, int tokens,
+                         const int32_t* cu_tokens, int max_tokens, int max_length, int64_t q_token_stride, int64_t q_head_stride,
+                         int64_t out_token_stride, int64_t out_head_stride, float scale, int causal, int window, void* workspace,
+                         size_t workspace_bytes, void* stream)
+{
+    return attention("ptoamd_attention_kv8", out, lse, cache, nullptr, 0, q, type, heads, tokens, cu_tokens, max_tokens, max_length, q_token_stride, q_head_stride,
+                     out_token_stride, out_head_stride, scale, causal, window, workspace, workspace_bytes, stream);
+}
+
+size_t ptoamd_attention_kv8_tree_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window)
+{
+    return ptoamd_attention_kv8_workspace_bytes(cache, heads, tokens, max_tokens, max_length, window);
+}
+
+int ptoamd_attention_kv8_tree(void* out, float* lse, const ptoamd_kv8_cache* cache, const uint64_t* tree, int tree_words, const void* q, int type,
+                              int heads, int tokens, const int32_t* cu_tokens, int max_tokens, int max_length, int64_t q_token_stride,
+                              int64_t q_head_stride, int64_t out_token_stride, int64_t out_head_stride, float scale, int window, void* workspace,
+                              size_t workspace_bytes, void* stream)
+{
+    const char* what = "ptoamd_attention_kv8_tree";
+    const int most = max_tokens < tokens ? max_tokens : tokens;  // (a loose bound)
+    if (most > 0) {
+        PTOAMD_REQUIRE(tree != nullptr, PTOAMD_E_INVALID, "%s: null operand", what);
+        PTOAMD_REQUIRE(reinterpret_cast<uintptr_t>(tree) % 8 == 0, PTOAMD_E_ALIGNMENT, "%s: the tree must be aligned to its words", what);
+        PTOAMD_REQUIRE(most <= PTOAMD_MOST_DRAFTED, PTOAMD_E_UNSUPPORTED, "%s: at most %d tokens of a sequence are drafted (%d)", what, PTOAMD_MOST_DRAFTED, most);
+        PTOAMD_REQUIRE(tree_words > 0 && tree_words <= PTOAMD_MOST_DRAFTED / 64 && 64 * tree_words >= most, PTOAMD_E_INVALID,
+                       "%s: rows of %d words for %d tokens: one for every 64 is needed, at most %d", what, tree_words, most, PTOAMD_MOST_DRAFTED / 64);
+        PTOAMD_REQUIRE(window <= 0 || window >= most, PTOAMD_E_UNSUPPORTED, "%s: a window of %d does not hold the %d tokens that may be drafted", what, window, most);
+    }
+    return attention(what, out, lse, cache, tree, tree_words, q, type, heads, tokens, cu_tokens, max_tokens, max_length, q_token_stride, q_head_stride,
+                     out_token_stride, out_head_stride, scale, 1, window, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

@@ -3,6 +3,7 @@
 #include <stddef.h>
 
 #include "common_host.hpp"
+#include "drafted.hpp"
 #include "kv8.hpp"
 #include "kv8_places.hpp"
 #include "lds_dma.hpp"
@@ -26,6 +27,9 @@ struct AttentionArgs {
     int* cuts;
     float* part_out;
     float2* part_sum;
+    // of drafted tokens, in place of `causal`: rows of tree_words 32-bit words (seen_keys)
+    const uint32_t* tree;
+    int tree_words;
 };
 
 // Many rows, keys in parts: all (key head, tile of rows, tile of keys) that there are, in this order, in equal stretches, one for a workgroup a CU.

@@ -1,0 +1,48 @@
+// Values to the codes of an 8-bit cache: what the kernels that write one share.
+#pragma once
+#include "kv8.hpp"
+
+namespace ptoamd {
+
+// Eight values in units of their scale -> eight codes.  int8: nearest, ties to even, clamped.  E4M3: the hardware's conversion, which
+// rounds every value inside +-448 to the nearest code, ties to even; values are clamped to that first.
+template <int CODE>
+__device__ __forceinline__ uint2 kv8_codes(const float* x)
+{
+    uint32_t w[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        if (CODE == PTOAMD_I8) {
+            w[h] = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                w[h] |= ((uint32_t)(int)__builtin_amdgcn_fmed3f(rintf(x[4 * h + i]), -127.0f, 127.0f) & 0xFFu) << (8 * i);
+        } else {
+            float c[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                c[i] = __builtin_amdgcn_fmed3f(x[4 * h + i], -448.0f, 448.0f);
+            int pk = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
+            w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], pk, true);
+        }
+    }
+    return make_uint2(w[0], w[1]);
+}
+
+template <int CODE>
+constexpr float KV8_PER_LARGEST = CODE == PTOAMD_I8 ? 1.0f / 127.0f : 1.0f / 448.0f;  // a page's scale over its largest magnitude
+
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T* p, float* x)
+{
+    struct alignas(WIDE ? 16 : sizeof(T)) V { T e[16 / sizeof(T)]; };
+    V v[8 * sizeof(T) / 16];
+#pragma unroll
+    for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
+        v[i] = reinterpret_cast<const V*>(p)[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = (float)v[i * sizeof(T) / 16].e[i % (16 / sizeof(T))];
+}
+
+}  // namespace ptoamd

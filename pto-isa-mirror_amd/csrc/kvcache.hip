@@ -1,6 +1,7 @@
 // The append to a cache of keys and values held in 8 bits: new tokens are quantised into their pages, one scale a page and head.
 #include "common_host.hpp"
 #include "kv8.hpp"
+#include "kv8_codes.hpp"
 #include "kv8_places.hpp"
 #include "lds_dma.hpp"
 
@@ -46,50 +47,12 @@ int kv8_from(const char* what, const ptoamd_kv8_cache* c, int tokens, const int3
     return PTOAMD_OK;
 }
 
-// Eight values in units of their scale -> eight codes.  int8: nearest, ties to even, clamped.  E4M3: the hardware's conversion, which
-// rounds every value inside +-448 to the nearest code, ties to even; values are clamped to that first.
-template <int CODE>
-__device__ __forceinline__ uint2 kv8_codes(const float* x)
-{
-    uint32_t w[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        if (CODE == PTOAMD_I8) {
-            w[h] = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                w[h] |= ((uint32_t)(int)__builtin_amdgcn_fmed3f(rintf(x[4 * h + i]), -127.0f, 127.0f) & 0xFFu) << (8 * i);
-        } else {
-            float c[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                c[i] = __builtin_amdgcn_fmed3f(x[4 * h + i], -448.0f, 448.0f);
-            int pk = __builtin_amdgcn_cvt_pk_fp8_f32(c[0], c[1], 0, false);
-            w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c[2], c[3], pk, true);
-        }
-    }
-    return make_uint2(w[0], w[1]);
-}
-
 struct AppendArgs {
     Kv8 cache;
     const uint8_t* src[2];           // k, v
     int64_t token[2], head[2];       // strides in bytes
     int blocks;                      // most pages that a sequence's new tokens touch
 };
-
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load8(const T* p, float* x)
-{
-    struct alignas(WIDE ? 16 : sizeof(T)) V { T e[16 / sizeof(T)]; };
-    V v[8 * sizeof(T) / 16];
-#pragma unroll
-    for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
-        v[i] = reinterpret_cast<const V*>(p)[i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = (float)v[i * sizeof(T) / 16].e[i % (16 / sizeof(T))];
-}
 
 // One workgroup a page of a sequence, head, and side (keys or values).  The new tokens' largest magnitude gives the page's scale, which
 // only grows; where it grows, the older tokens' codes are rounded again to the new one.  A thread has 8 elements of a row at a time.

@@ -2,10 +2,15 @@
 
     x -> gemm (queries, keys and values in one product) -> rope (queries and keys in one call) -> kvcache_append -> attention_kv8 -> gemm
 
-    python examples/attention_layer.py        # on an MI355X: two prompts, then a captured decode step; against the same layer in f32
+and several tokens at a time, drafted as a tree of which one path turns out to be right:
+
+    parents -> draft_tree;  x -> gemm -> kvcache_append_rope -> attention_kv8_tree -> gemm;  the path -> kvcache_keep
+
+    python examples/attention_layer.py        # on an MI355X: two prompts, then a captured decode step, or trees; against the same layer in f32
 """
 import math
 import os
+import random
 import sys
 
 import torch
@@ -44,6 +49,21 @@ class AttentionLayer:
         pa.kvcache_append(k, v, *cache, cu_tokens=cu_tokens, max_tokens=max_tokens)
         o = pa.attention_kv8(q, *cache, cu_tokens=cu_tokens, max_tokens=max_tokens, max_length=max_length)
         return pa.gemm(o.view(tokens, -1), self.w_out, pa.BF16, pa.BF16)
+
+    def drafted(self, x, tree, lengths, cu_tokens=None, max_tokens=None, max_length=0):
+        """x [tokens, width]: drafted tokens, sequence by sequence; tree: their rows of draft_tree(); lengths [sequences] int32, with them."""
+        pa, tokens = self.pa, x.shape[0]
+        qkv = pa.gemm(x, self.w_qkv, pa.BF16, pa.BF16).view(tokens, -1, self.head_dim)
+        q, k, v = qkv[:, :self.heads], qkv[:, self.heads:self.heads + self.kv_heads], qkv[:, self.heads + self.kv_heads:]
+        cache = (self.k, self.v, self.k_scale, self.v_scale, self.table, lengths, self.code_type)
+        pa.kvcache_append_rope(q, k, v, *cache, self.turns, tree=tree, cu_tokens=cu_tokens, max_tokens=max_tokens, out=q)
+        o = pa.attention_kv8_tree(q, *cache, tree, cu_tokens=cu_tokens, max_tokens=max_tokens, max_length=max_length)
+        return pa.gemm(o.view(tokens, -1), self.w_out, pa.BF16, pa.BF16)
+
+    def keep(self, kept, lengths, max_tokens, cu_tokens=None):
+        """The lengths with the path `kept` [sequences, most] of the drafted tokens alone, which the cache then holds behind what is older."""
+        return self.pa.kvcache_keep(kept, self.k, self.v, self.k_scale, self.v_scale, self.table, lengths, self.code_type, cu_tokens=cu_tokens,
+                                    max_tokens=max_tokens)
 
     def plain(self, x):
         """One sequence's x [tokens, width] from its first token on, in f32, without a cache."""
@@ -93,6 +113,42 @@ def serve(layer, prompts, chunk, steps):
     return [torch.cat(o) for o in outs]
 
 
+def serve_drafted(layer, prompts, known, chunk, drafted, seed=0):
+    """The first `known` tokens of each prompt in chunks, then trees of `drafted` tokens each, one path of which holds the sequence's next tokens: what a
+    server's drafter gives, and its model then finds right.  Returns each sequence's outputs of the tokens that were kept."""
+    rng = random.Random(seed)
+    outs = serve(layer, [p[:known] for p in prompts], chunk, 0)
+    done, pa = [known] * len(prompts), layer.pa
+    lengths = torch.tensor(done, dtype=torch.int32, device="cuda")
+    while any(d < p.shape[0] for d, p in zip(done, prompts)):
+        new = [drafted if d < p.shape[0] else 0 for d, p in zip(done, prompts)]
+        starts = torch.tensor([0] + new, dtype=torch.int32).cumsum(0, dtype=torch.int32)
+        parents, paths, x = [], [], []
+        for s, p in enumerate(prompts):
+            mine = [rng.randrange(-1, i) for i in range(new[s])]
+            path, at = [], rng.randrange(new[s]) if mine else -1
+            while at >= 0:
+                path.insert(0, at)
+                at = mine[at]
+            path = path[:p.shape[0] - done[s]]
+            wrong = torch.randn((new[s], p.shape[1]), generator=torch.Generator().manual_seed(rng.randrange(1 << 30))).to(p)
+            wrong[path] = p[done[s]:done[s] + len(path)]
+            parents += mine
+            paths.append(path)
+            x.append(wrong)
+        cu = starts.cuda()
+        tree = pa.draft_tree(torch.tensor(parents, dtype=torch.int32, device="cuda"), len(prompts), cu_tokens=cu, max_tokens=drafted)
+        lengths += cu[1:] - cu[:-1]
+        y = layer.drafted(torch.cat(x), tree, lengths, cu, drafted, max(done) + drafted)
+        most = max(len(path) for path in paths)
+        kept = torch.tensor([path + [-1] * (most - len(path)) for path in paths], dtype=torch.int32, device="cuda").view(len(prompts), most)
+        lengths = layer.keep(kept, lengths, drafted, cu)
+        for s, path in enumerate(paths):
+            outs[s] = torch.cat([outs[s], y[int(starts[s]):int(starts[s + 1])][path]])
+            done[s] += len(path)
+    return outs
+
+
 def relative_error(layer, prompts, outs):
     """The largest over sequences of |out - plain| / |plain|, both over all tokens."""
     return max(float((o.float() - layer.plain(p)).norm() / layer.plain(p).norm()) for o, p in zip(outs, prompts))
@@ -107,6 +163,8 @@ def main():
         prompts = [torch.randn((n, 1024), generator=g, device="cuda").bfloat16() for n in (700, 333)]
         outs = serve(layer, prompts, chunk=256, steps=8)
         print(f"{name} cache: relative error {relative_error(layer, prompts, outs):.4f} over {sum(p.shape[0] for p in prompts)} tokens")
+        outs = serve_drafted(layer, prompts, known=300, chunk=256, drafted=24)
+        print(f"{name} cache, drafted trees: relative error {relative_error(layer, prompts, outs):.4f}")
 
 
 if __name__ == "__main__":

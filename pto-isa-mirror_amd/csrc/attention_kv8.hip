@@ -196,6 +196,10 @@ int prepare_attention_kernels()
                     int rc = launch_attention_few(a, code, f16, 1, nullptr);
                     if (rc == PTOAMD_OK)
                         rc = launch_attention_many(a, code, f16, 1, nullptr);
+                    if (rc == PTOAMD_OK)
+                        rc = launch_attention_tree_few(a, code, f16, 1, nullptr);
+                    if (rc == PTOAMD_OK)
+                        rc = launch_attention_tree_many(a, code, f16, 1, nullptr);
                     if (rc != PTOAMD_OK)
                         return rc;
                 }
@@ -257,7 +261,7 @@ static int attention(const char* what, void* out, float* lse, const ptoamd_kv8_c
     const bool addressable = cache->k_page_stride >= 0 && cache->k_page_stride < 1LL << 34 && cache->v_page_stride >= 0 && cache->v_page_stride < 1LL << 34 &&
                              cache->k_token_stride >= 0 && cache->k_token_stride < 1 << 22 && cache->v_token_stride >= 0 && cache->v_token_stride < 1 << 22 &&
                              (long)cache->pages * cache->kv_heads < 1L << 30;
-    if (plan.kernel != AttentionPlan::GENERIC && cache_bits % 16 == 0 && addressable && !options().force_generic && tree == nullptr) {
+    if (plan.kernel != AttentionPlan::GENERIC && cache_bits % 16 == 0 && addressable && !options().force_generic) {
         a.wide = ((uint64_t)(uintptr_t)q | (uint64_t)(uintptr_t)out | (uint64_t)a.q_token | (uint64_t)a.q_head | (uint64_t)a.out_token | (uint64_t)a.out_head) % 16 == 0;
         a.splits = workspace != nullptr ? plan.splits : 1;
         a.chunk = plan.chunk;
@@ -267,7 +271,8 @@ static int attention(const char* what, void* out, float* lse, const ptoamd_kv8_c
         a.part_out = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (a.cuts != nullptr ? Cuts::BYTES : 0));
         a.part_sum = reinterpret_cast<float2*>(a.part_out + (size_t)plan.splits * tokens * heads * built_head(cache->head_dim));
         const bool few = plan.kernel == AttentionPlan::FEW;
-        const int rc = few ? launch_attention_few(a, cache->code_type, f16, cache->sequences, s) : launch_attention_many(a, cache->code_type, f16, cache->sequences, s);
+        const auto launch = tree != nullptr ? (few ? launch_attention_tree_few : launch_attention_tree_many) : (few ? launch_attention_few : launch_attention_many);
+        const int rc = launch(a, cache->code_type, f16, cache->sequences, s);
         if (rc != PTOAMD_OK)
             return rc;
         set_last_kernel(few ? (a.splits > 1 ? "attention_kv8_few_split" : "attention_kv8_few") : (a.splits > 1 ? "attention_kv8_many_split" : "attention_kv8_many"));

@@ -51,6 +51,9 @@ constexpr int MANY_KEYS = 64, MANY_START = 448 / MANY_KEYS;
 constexpr int few_waves(int head_dim, int row_tiles) { return head_dim <= 128 && row_tiles == 1 ? 8 : 4; }
 int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_many(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
+// (of drafted tokens)
+int launch_attention_tree_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
+int launch_attention_tree_many(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_join(const AttentionArgs& a, bool f16, int sequences, hipStream_t stream);
 int prepare_attention_kernels();  // the launch attributes of all of them, for the current device
 
@@ -108,6 +111,44 @@ __device__ __forceinline__ bool several_parts(const AttentionArgs& a, const Span
 __device__ __forceinline__ int2 visible_keys(const AttentionArgs& a, int place, int length)
 {
     return keys_of(place, length, a.causal, a.window);
+}
+
+// The keys that any of a sequence's new tokens first .. last sees: [x, y).  TREE: a token stands behind those that it sees, none to all that are drafted.
+template <bool TREE>
+__device__ __forceinline__ int2 keys_of_any(const AttentionArgs& a, const Span& s, int first, int last)
+{
+    const int place0 = s.length - s.count;
+    if (TREE)
+        return make_int2(first_key(place0, a.window), s.length);
+    return make_int2(visible_keys(a, place0 + first, s.length).x, visible_keys(a, place0 + last, s.length).y);
+}
+// Those that every one of them sees.
+template <bool TREE>
+__device__ __forceinline__ int2 keys_of_every(const AttentionArgs& a, const Span& s, int first, int last)
+{
+    const int place0 = s.length - s.count;
+    if (TREE)
+        return make_int2(first_key(s.length - 1, a.window), place0);
+    return make_int2(visible_keys(a, place0 + last, s.length).x, visible_keys(a, place0 + first, s.length).y);
+}
+// Words of a drafted token's row, its bits behind the sequence's last token cleared.
+__device__ __forceinline__ uint32_t drafted_word(const AttentionArgs& a, const Span& s, int token, int word)
+{
+    return word < a.tree_words ? a.tree[(int64_t)(s.first + token) * a.tree_words + word] & bits_below(s.count - 32 * word) : 0u;
+}
+// The first of the older keys that a token sees, whose `words` words lie in LDS.  (No row: none of them.)
+template <int WORDS>
+__device__ __forceinline__ int first_of_drafted(const AttentionArgs& a, const Span& s, const uint32_t* row, bool valid, int token)
+{
+    if (!valid)
+        return 0x7FFFFFFF;
+    return a.window > 0 ? first_key(s.length - s.count + others_seen(row, WORDS, s.count, token), a.window) : 0;
+}
+// Which of the keys key .. key + 31 a token sees (seen_keys: `key` is the same for all lanes, and words behind the last token are 0).
+template <int WORDS>
+__device__ __forceinline__ uint32_t drafted_keys(const uint32_t* row, int key, int first, int old)
+{
+    return (bits_below(old - key) & ~bits_below(first - key)) | row_bits(row, WORDS, key - old);
 }
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

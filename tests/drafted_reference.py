@@ -37,8 +37,19 @@ def flat(parents):
 
 def attention(q, cache, ways, window=0, scale=None):
     """As kv8_reference.attention, of drafted tokens: (out, lse, magnitude, spread) in 64 bits."""
+    return attention_and_least(q, cache, ways, window, scale)[0]
+
+
+def attention_and_least(q, cache, ways, window=0, scale=None):
+    """That, and what results may be off by beside it where elements of the keys of large weights are small.
+    A weight (p times its page's value scale s) is f16 on a scale on which the largest p s of the row is 2^11 or more; steps of f16 end at 2^-24, so a
+    rounding is off by 2^-25 at most where it is not relative: 2^-36 of the largest p s, times the code of each key.
+    An int8 code c is multiplied as c + 128, and 128 times the weights taken off in the same tile: sums on the way are up to 255 times the weights', whatever
+    the codes, and each instruction rounds them to f32 up to eight times (its 32 products are added four at a time): 16 * 255 * 2^-24 < 2^-12 of the sum of
+    p s."""
     tokens, heads, dim = q.shape
     scale = dim ** -0.5 if scale is None else scale
+    least = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     out, mag = torch.zeros(q.shape, dtype=torch.float64, device="cuda"), torch.zeros(q.shape, dtype=torch.float64, device="cuda")
     lse = torch.full((tokens, heads), -math.inf, dtype=torch.float64, device="cuda")
     spread = torch.zeros((tokens, heads), dtype=torch.float64, device="cuda")
@@ -63,7 +74,13 @@ def attention(q, cache, ways, window=0, scale=None):
             p = torch.nan_to_num(torch.exp(score - norm[:, :, None]), nan=0.0)
             out[at:at + n], mag[at:at + n] = (p @ v).transpose(0, 1), (p @ v.abs()).transpose(0, 1)
             lse[at:at + n] = norm.t()
+            unit = cache.v_scale[cache.table[s].long().clamp(min=0)].double().repeat_interleave(cache.page, 0)[:length].t().repeat_interleave(group, 0)  # [heads, length]
+            codes = torch.where(unit[:, :, None] > 0, v.abs() / unit[:, :, None], 0.0)
+            most = (p * unit[:, None]).amax(dim=2)
+            least[at:at + n] = (2.0 ** -36 * most[:, :, None] * (seen.double() @ codes)).transpose(0, 1)
+            if cache.code == "i8":
+                least[at:at + n] += 2.0 ** -12 * (p * unit[:, None]).sum(dim=2).t()[:, :, None]
             size = (qs.norm(dim=2)[:, :, None] * k.norm(dim=2)[:, None]).masked_fill(~seen, 0.0)
             spread[at:at + n] = scale * size.amax(dim=2).t()
         at += n
-    return out, lse, mag, spread
+    return (out, lse, mag, spread), least

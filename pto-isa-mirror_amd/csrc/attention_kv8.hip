@@ -105,6 +105,10 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 //          48 38 / 63, 64 46 / 65, 80 65 / 69; 32 of 8000 128 rows 353 / 278; one of 2000 48 rows 13 / 23, 96 15 / 25.  Of 256, 2 key heads, 32 of
 //          8000: 48 130 / 114, 64 168 / 115; 8 of 6000: 40 45 / 42, 64 59 / 45; one of 60000 40 57 / 52.
 //   many : more rows, 256 of them a workgroup (128 for heads of 256 elements)
+// Of drafted tokens, 128 rows a workgroup (HALVES) where there are no more: us, 256 rows a workgroup / 128, 16 sequences of 8192 keys, 64 / 8 heads of 128
+// E4M3, 16 tokens 147 / 105, one of 131072 150 / 110; of 64, 119 / 77; and 32 tokens, 256 rows, 179 / 180, 48 271 / 281, 64 291 / 334.  That kernel
+// and the few-rows one: heads of 128, 80 rows, 16 x 8192 163 / 100, 8 x 2000 and 1 x 16000 44 / 39 and 42 / 34, so from half as many keys on as above; 64 rows
+// 89 / 96, 33 / 37, 31 / 33; 96 rows over 2000 keys 15 / 25; of 64, 80 rows 92 / 87 of 16 x 8192, 27 / 32 of 8 x 2000.
 // Few rows are 16, 32, or, where the keys are that many, up to 48 a workgroup and 64 of heads of 128: codes are converted once for all of them.
 // 32 sequences of 8000 keys, 8 key heads of 128, us, 32 / 48 / 64 rows a workgroup: 32 rows 128 / 153 / 181, 48 226 / 156 / 183, 64 229 / 277 / 188;
 // of 64: 48 rows 114 / 85 / 135, 64 105 / 131 / 125; one sequence of 2000 keys, 48 rows 13.4 / 15.7 / 17.7.
@@ -124,11 +128,11 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 constexpr long PART_ROOM = 256L << 20;  // bytes
 struct AttentionPlan {
     enum { GENERIC, FEW, MANY } kernel;
-    int splits, chunk, row_tiles;
+    int splits, chunk, row_tiles, tile_rows;
 };
-static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int tokens, int max_tokens, int max_length, int window)
+static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int tokens, int max_tokens, int max_length, int window, bool tree)
 {
-    AttentionPlan p{AttentionPlan::GENERIC, 1, 0, 0};
+    AttentionPlan p{AttentionPlan::GENERIC, 1, 0, 0, 0};
     const int dim = built_head(c->head_dim);
     if (dim == 0)
         return p;
@@ -144,7 +148,8 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     const long items = (long)c->sequences * c->kv_heads;
     const long room = PART_ROOM / ((long)tokens * heads * (dim * 4 + 8));  // parts
     const bool busy = items * keys * dim > 65536 * cus;
-    p.kernel = rows <= (!busy ? 96 : dim == 256 ? 32 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
+    const bool fewer = busy || (tree && dim == 128 && items * keys * dim > 32768 * cus);
+    p.kernel = rows <= (!fewer ? 96 : dim == 256 ? 32 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
     if (p.kernel == AttentionPlan::FEW) {
         p.row_tiles = rows <= 16 || dim == 256 ? 1 : rows <= 32 || !busy ? 2 : rows <= 48 ? 3 : dim == 128 ? 4 : 2;
         const long step = 32 * few_waves(dim, p.row_tiles);  // the keys that a workgroup's waves have at a time
@@ -163,7 +168,10 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
         }
         return p;
     }
-    p.row_tiles = (int)((rows + many_rows(dim) - 1) / many_rows(dim));
+    p.tile_rows = many_rows(dim);
+    if (tree && rows <= 128)
+        p.tile_rows = 128;
+    p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
     const long tiles = p.row_tiles * items;  // of rows, a workgroup's each if no keys are cut
     const bool countable = (long)p.row_tiles * c->sequences <= Cuts::MOST && (double)tiles * c->max_pages * c->page_size < 1e9;
     const double full = (double)tiles / cus / (c->sequences > 1 ? 2 : 1);
@@ -193,6 +201,7 @@ int prepare_attention_kernels()
                     AttentionArgs a{};  // (of no heads: nothing is launched)
                     a.cache.head_dim = dim;
                     a.row_tiles = tiles;
+                    a.tile_rows = tiles == 1 ? 128 : 256;  // (of drafted tokens: both)
                     int rc = launch_attention_few(a, code, f16, 1, nullptr);
                     if (rc == PTOAMD_OK)
                         rc = launch_attention_many(a, code, f16, 1, nullptr);
@@ -204,6 +213,14 @@ int prepare_attention_kernels()
                         return rc;
                 }
     return PTOAMD_OK;
+}
+
+static size_t workspace_bytes_of(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window, bool tree)
+{
+    if (cache == nullptr || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads != 0 || tokens <= 0 || max_tokens <= 0 || cache->sequences <= 0 ||
+        cache->max_pages <= 0 || cache->page_size <= 0)
+        return 0;
+    return part_bytes(plan_attention(cache, heads, tokens, max_tokens, max_length, window, tree), heads, tokens, built_head(cache->head_dim));
 }
 
 // The call of both entry points: `causal`, or `tree` with rows of tree_words 64-bit words.
@@ -251,7 +268,7 @@ static int attention(const char* what, void* out, float* lse, const ptoamd_kv8_c
     a.tree_words = 2 * tree_words;
     hipStream_t s = as_stream(stream);
     const bool i8 = cache->code_type == PTOAMD_I8, f16 = type == PTOAMD_F16;
-    const AttentionPlan plan = plan_attention(cache, heads, tokens, max_tokens, max_length, window);
+    const AttentionPlan plan = plan_attention(cache, heads, tokens, max_tokens, max_length, window, tree != nullptr);
     const size_t need = part_bytes(plan, heads, tokens, built_head(cache->head_dim));
     PTOAMD_REQUIRE(workspace == nullptr || workspace_bytes >= need, PTOAMD_E_INVALID, "%s: a workspace of %zu bytes is needed (%zu)", what, need, workspace_bytes);
     PTOAMD_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, PTOAMD_E_ALIGNMENT, "%s: the workspace must be 16-byte aligned", what);
@@ -266,6 +283,7 @@ static int attention(const char* what, void* out, float* lse, const ptoamd_kv8_c
         a.splits = workspace != nullptr ? plan.splits : 1;
         a.chunk = plan.chunk;
         a.row_tiles = plan.row_tiles;
+        a.tile_rows = plan.tile_rows;
         a.sequences = cache->sequences;
         a.cuts = plan.kernel == AttentionPlan::MANY && a.splits > 1 ? static_cast<int*>(workspace) : nullptr;
         a.part_out = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (a.cuts != nullptr ? Cuts::BYTES : 0));
@@ -291,10 +309,7 @@ extern "C" {
 
 size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window)
 {
-    if (cache == nullptr || cache->kv_heads <= 0 || heads <= 0 || heads % cache->kv_heads != 0 || tokens <= 0 || max_tokens <= 0 || cache->sequences <= 0 ||
-        cache->max_pages <= 0 || cache->page_size <= 0)
-        return 0;
-    return part_bytes(plan_attention(cache, heads, tokens, max_tokens, max_length, window), heads, tokens, built_head(cache->head_dim));
+    return workspace_bytes_of(cache, heads, tokens, max_tokens, max_length, window, false);
 }
 
 int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, const void* q, int type, int heads, int tokens,
@@ -308,7 +323,7 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
 
 size_t ptoamd_attention_kv8_tree_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window)
 {
-    return ptoamd_attention_kv8_workspace_bytes(cache, heads, tokens, max_tokens, max_length, window);
+    return workspace_bytes_of(cache, heads, tokens, max_tokens, max_length, window, true);
 }
 
 int ptoamd_attention_kv8_tree(void* out, float* lse, const ptoamd_kv8_cache* cache, const uint64_t* tree, int tree_words, const void* q, int type,

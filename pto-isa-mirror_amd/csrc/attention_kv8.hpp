@@ -22,8 +22,9 @@ struct AttentionArgs {
     int wide;  // rows of q and out allow 16-byte accesses
     // The keys of a row in parts, where splits > 1 (at most so many): every part leaves its sums of a row (unscaled) and the row's reference and
     // sum, [split][token][head]; a second kernel joins them in the order of the parts.
-    // Few rows, row_tiles of 16 a workgroup: parts of `chunk` tokens, each a workgroup's.  Many: `cuts`, of the rows in row_tiles tiles a sequence (Cuts).
-    int splits, chunk, row_tiles, sequences;
+    // Few rows, row_tiles of 16 a workgroup: parts of `chunk` tokens, each a workgroup's.  Many: `cuts`, of the rows in row_tiles tiles of tile_rows a
+    // sequence (Cuts).
+    int splits, chunk, row_tiles, tile_rows, sequences;
     int* cuts;
     float* part_out;
     float2* part_sum;
@@ -45,7 +46,9 @@ struct Cuts {
 // which the queries' zeros there take out of the scores, and whose results are not stored.  0: only the generic kernel.
 constexpr int built_head(int head_dim) { return head_dim % 16 != 0 || head_dim > 256 ? 0 : head_dim <= 64 ? 64 : head_dim <= 128 ? 128 : 256; }
 constexpr int many_rows(int head_dim) { return head_dim == 256 ? 128 : 256; }  // a tile's
-constexpr int MANY_KEYS = 64, MANY_START = 448 / MANY_KEYS;
+constexpr int MANY_KEYS = 64;
+// What a tile of rows' start and end cost, in tiles of keys: those of half as many rows take half the time.
+constexpr int many_start(int head_dim, int tile_rows) { return 448 / MANY_KEYS * (many_rows(head_dim) / tile_rows); }
 
 // The waves of a few-rows workgroup of so many tiles of 16 rows: eight where two fit a SIMD's registers (heads up to 128 elements, one tile), else four.
 constexpr int few_waves(int head_dim, int row_tiles) { return head_dim <= 128 && row_tiles == 1 ? 8 : 4; }

@@ -29,8 +29,8 @@ __global__ void __launch_bounds__(256) attention_kv8_join_kernel(AttentionArgs a
     const int64_t at = (int64_t)(span.first + nth) * a.heads + head, stride = (int64_t)a.cache.tokens * a.heads;
     int from = 0, to;
     if (a.cuts != nullptr) {  // (rows of one part are written already)
-        const int kv_head = head / a.group, tile = seq * a.row_tiles + (nth * a.group + head - kv_head * a.group) / many_rows(D);
-        const int stretch = a.cuts[Cuts::STRETCH], first = kv_head * a.cuts[Cuts::HEAD] + a.cuts[Cuts::FIRST + tile] + MANY_START;
+        const int kv_head = head / a.group, tile = seq * a.row_tiles + (nth * a.group + head - kv_head * a.group) / a.tile_rows;
+        const int stretch = a.cuts[Cuts::STRETCH], first = kv_head * a.cuts[Cuts::HEAD] + a.cuts[Cuts::FIRST + tile] + many_start(D, a.tile_rows);
         const int last = kv_head * a.cuts[Cuts::HEAD] + a.cuts[Cuts::FIRST + tile + 1] - 1;
         to = last / stretch - first / stretch + 1;
         if (to == 1)

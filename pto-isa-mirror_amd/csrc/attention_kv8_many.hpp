@@ -36,22 +36,22 @@ struct ManyTile {
 
 // The tiles of keys that there are and a workgroup's stretch of them: long enough that a tile of rows has at most splits parts, and 256 keys at
 // least (with 1024, three sequences of 8642 keys with one key head took 52 us instead of 39).
-template <int D, int WAVES, bool TREE>
+template <int D, int WAVES, int ROWS, bool TREE>
 __device__ __forceinline__ void count_tiles(const AttentionArgs& a, int tiles, int* cuts)
 {
-    constexpr int KEYS = MANY_KEYS, LEAST = 256 / KEYS;
+    constexpr int KEYS = MANY_KEYS, LEAST = 256 / KEYS, START = many_start(D, ROWS);
     static_assert(64 * WAVES >= Cuts::MOST, "a thread counts a tile of rows");
     __shared__ int wave_sum[WAVES], wave_most[WAVES];
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     int own = 0;
     if (tid < tiles) {
-        const int seq = tid / a.row_tiles, row0 = (tid - seq * a.row_tiles) * many_rows(D);
+        const int seq = tid / a.row_tiles, row0 = (tid - seq * a.row_tiles) * ROWS;
         const Span span = span_of(a, seq);
         const int rows = span.count * a.group;
         if (row0 < rows) {  // (rows that see no key have a tile too: zeros are written there)
-            const int2 any = keys_of_any<TREE>(a, span, row0 / a.group, (min(row0 + many_rows(D), rows) - 1) / a.group);
+            const int2 any = keys_of_any<TREE>(a, span, row0 / a.group, (min(row0 + ROWS, rows) - 1) / a.group);
             const int from = any.x & ~31, to = any.y;
-            own = max((to - from + KEYS - 1) / KEYS, 1) + MANY_START;
+            own = max((to - from + KEYS - 1) / KEYS, 1) + START;
         }
     }
     int sum = own, most = own;
@@ -99,23 +99,27 @@ __device__ __forceinline__ float scaled_accumulator(float x, float by)
 }
 
 // TREE: of drafted tokens, whose rows of bits lie in LDS for the tiles of the step's own keys.
+// HALVES: half as many rows a workgroup, 128, and two tiles of keys at a time: the waves of a SIMD have the same rows, one those of every second tile, and
+// add up at the end.  So rows up to 128 leave no wave without work; each half stages its tiles alone, twice a wave's share.
 constexpr int MANY_TREE_WORDS = PTOAMD_MOST_DRAFTED / 32;
-template <typename T, int CODE, int D, int WAVES, bool TREE>
+template <typename T, int CODE, int D, int WAVES, bool TREE, bool HALVES>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) attention_kv8_many_kernel(AttentionArgs args)
 {
     typedef ManyTile<D> Tile;
-    constexpr int THREADS = 64 * WAVES, KEYS = Tile::KEYS, STEPS = D / 16, DT = D / 32;
+    constexpr int ROWS = 32 * WAVES / (HALVES ? 2 : 1), START = many_start(D, ROWS);
+    constexpr int GROUP = HALVES ? WAVES / 2 : WAVES;  // the waves that share a tile of keys
+    constexpr int THREADS = 64 * GROUP, KEYS = Tile::KEYS, STRIDE = HALVES ? 2 * KEYS : KEYS, STEPS = D / 16, DT = D / 32;
     constexpr int SIDE_UNITS = KEYS * D / 16, UNITS = 2 * SIDE_UNITS / THREADS;  // 16 codes each; a thread's
-    extern __shared__ __attribute__((aligned(16))) uint8_t tiles[];                   // two of keys, two of values
-    __shared__ float4 scales[2][KEYS / 16];                                                   // of 16 keys: key scale, value scale's log2 and inverse
+    extern __shared__ __attribute__((aligned(16))) uint8_t all_tiles[];               // two of keys, two of values (HALVES: of each)
+    __shared__ float4 all_scales[HALVES ? 2 : 1][2][KEYS / 16];                                                 // of 16 keys: key scale, value scale's log2 and inverse
     __shared__ int cuts[Cuts::SIZE];
-    __shared__ uint32_t drafted[TREE ? 32 * WAVES : 1][MANY_TREE_WORDS + 1];  // (rows a bank apart)
+    __shared__ uint32_t drafted[TREE ? ROWS : 1][MANY_TREE_WORDS + 1];  // (rows a bank apart)
     // A workgroup has one tile of rows and all their keys, or a stretch of what there is (Cuts): the end of a tile's keys, whole ones, the start of
     // another's.  Stretches go to the XCDs in eighths, so that neighbours, which share keys, share an L2.
     const int turn = gridDim.x % 8 == 0 ? (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8) : (int)blockIdx.x;
     int unit = 0, unit_end = 0;
     if (args.splits > 1) {
-        count_tiles<D, WAVES, TREE>(args, args.row_tiles * args.sequences, cuts);
+        count_tiles<D, WAVES, ROWS, TREE>(args, args.row_tiles * args.sequences, cuts);
         unit = turn * cuts[Cuts::STRETCH];
         unit_end = min(unit + cuts[Cuts::STRETCH], cuts[Cuts::HEAD] * args.cache.kv_heads);
         unit = __builtin_amdgcn_readfirstlane(unit), unit_end = __builtin_amdgcn_readfirstlane(unit_end);
@@ -126,7 +130,12 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         const ArgumentsAgain again;  // (for each tile of rows anew: what only its start needs is not kept through the loop)
         int tid = threadIdx.x;
         asm("" : "+v"(tid));
-        const int lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 32, hf = lane / 32;
+        const int half = HALVES ? __builtin_amdgcn_readfirstlane(tid / THREADS) : 0;
+        if constexpr (HALVES)
+            tid %= THREADS;
+        const int lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64), col = lane % 32, hf = lane / 32;  // (HALVES: among its half's)
+        uint8_t* tiles = all_tiles + half * 4 * Tile::BYTES;
+        auto& scales = all_scales[half];
         const AttentionArgs& a = *again.all();
         const Kv8& c = a.cache;
         int kv_head, row_tile, seq, skip = 0, part = -1, most = 1 << 30;
@@ -141,14 +150,14 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             const int first = __builtin_amdgcn_readfirstlane(cuts[Cuts::FIRST + tile]), next = __builtin_amdgcn_readfirstlane(cuts[Cuts::FIRST + tile + 1]);
             seq = tile / a.row_tiles;
             row_tile = tile - seq * a.row_tiles;
-            const int until = min(next - rest, unit_end - unit) + rest - first - MANY_START;
-            skip = max(rest - first - MANY_START, 0);
+            const int until = min(next - rest, unit_end - unit) + rest - first - START;
+            skip = max(rest - first - START, 0);
             most = until - skip;
             unit += next - rest;
             if (until <= 0)
                 continue;  // (the stretch ends before the first of its keys)
-            if (most < next - first - MANY_START)
-                part = turn - (kv_head * head_tiles + first + MANY_START) / stretch;
+            if (most < next - first - START)
+                part = turn - (kv_head * head_tiles + first + START) / stretch;
         } else {
             const int row_tiles = gridDim.x / c.kv_heads;
             kv_head = blockIdx.x % c.kv_heads;
@@ -156,12 +165,12 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             seq = blockIdx.y;
         }
         const Span span = span_of(a, seq);
-        const int rows = span.count * a.group, row0 = row_tile * 32 * WAVES;
+        const int rows = span.count * a.group, row0 = row_tile * ROWS;
         if (row0 >= rows)
             return;
         // the keys that any row of the workgroup sees, and of the part
         const int place0 = span.length - span.count;
-        const int2 any = keys_of_any<TREE>(a, span, row0 / a.group, (min(row0 + 32 * WAVES, rows) - 1) / a.group);
+        const int2 any = keys_of_any<TREE>(a, span, row0 / a.group, (min(row0 + ROWS, rows) - 1) / a.group);
         const int from = any.x, to = any.y;
         const int begin = (from & ~31) + skip * KEYS, end = most < (to - begin + KEYS - 1) / KEYS ? begin + most * KEYS : to;
 
@@ -191,7 +200,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             cq = r.up * (a.scale * 1.44269504088896341f) * KV8_UNIT<CODE>;
             scale_to_f16<T, STEPS>(q, r.down);
         }
-        // where a row's scores start: without the 128 that the keys' int8 codes carry
+        // where a row's scores start: without the 128 that the keys' int8 codes carry.  (TREE: taken off where scores are scaled, in one register for 16)
         f32x16 start = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         if (CODE == PTOAMD_I8) {
             const uint4 unbias = make_uint4(UNBIAS, UNBIAS, UNBIAS, UNBIAS);
@@ -199,6 +208,9 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             for (int st = 0; st < STEPS; ++st)
                 start = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, unbias), __builtin_bit_cast(f16x8, q[st]), start, 0, 0, 0);
         }
+        const float bias = start[0];  // (all keys')
+        if constexpr (TREE)
+            start = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
         // the keys that every row of the wave sees
         const int wave_row = row0 + 32 * wave;
         const int2 every = keys_of_every<TREE>(a, span, min(wave_row, rows - 1) / a.group, (min(wave_row + 32, rows) - 1) / a.group);
@@ -207,6 +219,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         // What a thread stages: units of 16 codes; a unit's side, key and 16 elements are the same for every tile.  A wave's units of a kind are keys of
         // one group of 16, so of one page: its id, scale and address are the scalar unit's work.  Values go one tile behind the keys, as they are used:
         // stage i is the keys of tile i and the values of tile i - 1.
+        const int own_begin = begin + half * KEYS;  // (tile i of its own starts at own_begin + i STRIDE)
         const int last_key = max(span.length - 1, 0), slot_mask = (1 << c.page_shift) - 1;
         const int32_t* table = c.table + (int64_t)seq * c.max_pages;
         int ids[UNITS], scale_id = 0;
@@ -217,9 +230,9 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         uint32_t source[UNITS], target[UNITS][2], none = 0;
         asm("" : "+v"(none));  // (a vector register's zero: a scale that is not read through the scalar cache, for which a barrier would wait)
         static_assert(SIDE_UNITS % THREADS == 0 || THREADS == 2 * SIDE_UNITS, "a unit is keys or values for all waves, or for half of them");
-        auto is_value = [&](int u) { return SIDE_UNITS < THREADS ? wave >= WAVES / 2 : u * THREADS >= SIDE_UNITS; };
-        const int wave_key = wave % (SIDE_UNITS < THREADS ? WAVES / 2 : WAVES) * (1024 / D);
-        auto unit_key = [&](int u, int stage) { return begin + (stage - (is_value(u) ? 1 : 0)) * KEYS + u * THREADS % SIDE_UNITS / (D / 16) + wave_key; };
+        auto is_value = [&](int u) { return SIDE_UNITS < THREADS ? wave >= GROUP / 2 : u * THREADS >= SIDE_UNITS; };
+        const int wave_key = wave % (SIDE_UNITS < THREADS ? GROUP / 2 : GROUP) * (1024 / D);
+        auto unit_key = [&](int u, int stage) { return own_begin + (stage - (is_value(u) ? 1 : 0)) * STRIDE + u * THREADS % SIDE_UNITS / (D / 16) + wave_key; };
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
             const int k = (tid + u * THREADS) % SIDE_UNITS / (D / 16), chunk = lane % (D / 16) * 2;
@@ -278,7 +291,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
                 const bool known = (unsigned)scale_id < (unsigned)c.pages;
                 const uint32_t at = (known ? scale_id : 0) * (uint32_t)c.kv_heads + kv_head;
                 raw_scale = make_float2(known ? c.k.scales[at] : NAN, known ? c.v.scales[at] : NAN);
-                scale_id = table[min(begin + (stage + 2) * KEYS + 16 * tid, last_key) >> c.page_shift];
+                scale_id = table[min(own_begin + (stage + 2) * STRIDE + 16 * tid, last_key) >> c.page_shift];
             }
         };
 
@@ -298,7 +311,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         // The matrix part of turn `tile`: the sums of the tile before, the scores of this one.  A SIMD has 32 clocks for a product that a wave issues in
         // four: in between go the reads of the fragment AHEAD products on, and a piece of the staging.  (The order is fixed by barriers for the
         // compiler, which would by itself read each fragment right before it is used.)
-        constexpr int PV = KEYS / 16 * DT, QK = KEYS / 32 * STEPS, AHEAD = 4;
+        constexpr int PV = KEYS / 16 * DT, QK = KEYS / 32 * STEPS, AHEAD = HALVES ? 2 : 4;
         static_assert(D != 256 || QK >= 8, "score products between the sums' products and scaled_accumulator");
         auto multiply = [&](int tile) __attribute__((always_inline)) {
             const uint8_t* values = tiles + (2 + ((tile - 1) & 1)) * Tile::BYTES;
@@ -338,7 +351,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         };
         // the vector part: scores to weights
         auto weigh = [&](int tile) __attribute__((always_inline)) {
-            const int key = begin + tile * KEYS, buffer = tile & 1;
+            const int key = own_begin + tile * STRIDE, buffer = tile & 1;
             const bool whole = key >= every_from && key + KEYS <= every_to;
             float4 sc[KEYS / 16];  // of 16 keys, 8 of them this lane's
             float scale[KEYS / 16], high = -INFINITY;
@@ -355,6 +368,8 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             for (int x = 0; x < KEYS / 16; ++x) {
                 sc[x] = scales[buffer][x];
                 scale[x] = cq * sc[x].x;
+                if (TREE && CODE == PTOAMD_I8)
+                    sc[x].y = fmaf(bias, scale[x], sc[x].y);
             }
             find(tile + 3);
             stage_scales(tile + 1);
@@ -422,15 +437,16 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         // Where there are two waves a SIMD, the second four go one segment behind the first: one wave of a SIMD multiplies while the other weighs.  Keys
         // and values have two buffers each; what multiply(j) writes, stage j + 1, was last read in multiply(j - 1), the segment before at the latest,
         // and is next read in multiply(j + 1), the segment after at the earliest.
-        const int count = begin < end ? (end - begin + KEYS - 1) / KEYS : 0;
-        const bool behind = WAVES == 8 && wave >= 4;
+        const int count = begin < end ? (end - begin + STRIDE - 1) / STRIDE : 0;
+        const int own_count = HALVES ? (max(end - own_begin, 0) + STRIDE - 1) / STRIDE : count;  // (the second half may have one less)
+        const bool behind = HALVES ? half != 0 : WAVES == 8 && wave >= 4;
         if (count > 0) {
             find(0);
 #pragma unroll
             for (int u = 0; u < UNITS; ++u)
                 fetch(u, 0);
             if (tid < KEYS / 16)
-                scale_id = table[min(begin + 16 * tid, last_key) >> c.page_shift];
+                scale_id = table[min(own_begin + 16 * tid, last_key) >> c.page_shift];
             find(1);
             static_for<UNITS * PIECES>([&](auto n_) __attribute__((always_inline)) {
                 constexpr int n = decltype(n_)::value;
@@ -445,12 +461,13 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             for (int tile = 0; tile <= count; ++tile) {
                 if (WAVES == 8)
                     __builtin_amdgcn_s_setprio(1);  // (ahead of the SIMD's other wave, whatever its age)
-                multiply(tile);
+                if (!HALVES || tile <= own_count)
+                    multiply(tile);
                 if (WAVES == 8) {
                     __builtin_amdgcn_s_setprio(0);
                     __syncthreads();
                 }
-                if (tile < count)
+                if (tile < own_count)
                     weigh(tile);
                 __syncthreads();
             }
@@ -459,6 +476,38 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         }
 
         sum += __shfl_xor(sum, 32);
+        if constexpr (HALVES) {
+            // the second half's sums to the first, on the reference of both, where the tiles were: 16 elements of a lane at a time, lane beside lane
+            float* other = reinterpret_cast<float*>(all_tiles) + wave * (DT * 16 + 2) * 64 + lane;
+            static_assert(GROUP * (DT * 16 + 2) * 64 * 4 <= 8 * Tile::BYTES, "the second half's sums lie in the tiles' room");
+            if (half != 0) {
+#pragma unroll
+                for (int m = 0; m < DT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        other[(m * 16 + i) * 64] = o[m][i];
+                other[DT * 16 * 64] = top;
+                other[(DT * 16 + 1) * 64] = sum;
+            }
+            __syncthreads();
+            if (half == 0) {
+                const float its_top = other[DT * 16 * 64], its_sum = other[(DT * 16 + 1) * 64], to_top = fmaxf(top, its_top);
+                const float mine = __builtin_amdgcn_exp2f(top - to_top), its = __builtin_amdgcn_exp2f(its_top - to_top);
+                top = to_top;
+                sum = sum * mine + its_sum * its;
+#pragma unroll
+                for (int m = 0; m < DT; ++m)
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        o[m][i] = o[m][i] * mine + other[(m * 16 + i) * 64] * its;
+            }
+            __syncthreads();  // (rows leave through the same room)
+            if (half != 0) {
+                if (unit < unit_end)
+                    __syncthreads();  // (the first half's, behind its rows)
+                continue;
+            }
+        }
         const ArgumentsAgain e;
         const int64_t part_row = (int64_t)max(part, 0) * c.tokens * a.heads;
         if (valid && hf == 0) {
@@ -473,7 +522,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         // nobody reads those), so that two lanes have a row's and store 16 each.
         const float inverse = part >= 0 ? 1.0f : sum == 0.0f ? 0.0f : 1.0f / sum;
         uint8_t* mine = tiles + wave * 4096;
-        static_assert(WAVES * 4096 <= 4 * Tile::BYTES, "a wave's rows of 32 f32 lie in the tiles' room");
+        static_assert(GROUP * 4096 <= 4 * Tile::BYTES, "a wave's rows of 32 f32 lie in the tiles' room");
         const int own = lane / 2, own_row = row0 + 32 * wave + own, own_token = own_row / a.group, own_head = kv_head * a.group + own_row - own_token * a.group;
         float* part_out = e.global<float>(offsetof(AttentionArgs, part_out)) + (part_row + (int64_t)(span.first + own_token) * a.heads + own_head) * D + 16 * (lane % 2);
         uint8_t* out = e.global<uint8_t>(offsetof(AttentionArgs, out)) + (int64_t)(span.first + own_token) * ARGUMENT(e, out_token) + (int64_t)own_head * ARGUMENT(e, out_head) + 32 * (lane % 2);
@@ -506,16 +555,15 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
     } while (unit < unit_end);
 }
 
-template <typename T, int CODE, int D, int WAVES, bool TREE>
+template <typename T, int CODE, int D, int WAVES, bool TREE, bool HALVES>
 static int launch_many(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
-    constexpr int bytes = 4 * ManyTile<D>::BYTES;
-    PTOAMD_HIP_CHECK((ensure_dynamic_lds<&attention_kv8_many_kernel<T, CODE, D, WAVES, TREE>>(bytes)));
+    constexpr int bytes = (HALVES ? 8 : 4) * ManyTile<D>::BYTES;
+    PTOAMD_HIP_CHECK((ensure_dynamic_lds<&attention_kv8_many_kernel<T, CODE, D, WAVES, TREE, HALVES>>(bytes)));
     if (a.heads == 0)  // (prepare_attention_kernels)
         return PTOAMD_OK;
-    static_assert(32 * WAVES == many_rows(D), "the tiles of rows that the cuts count");
-    const dim3 grid = a.splits > 1 ? dim3(device_compute_units()) : dim3((unsigned)(a.row_tiles * a.cache.kv_heads), (unsigned)sequences);
-    hipLaunchKernelGGL((attention_kv8_many_kernel<T, CODE, D, WAVES, TREE>), grid, dim3(64 * WAVES), bytes, stream, a);
+    const dim3 grid = a.splits > 1 ? dim3((unsigned)device_compute_units()) : dim3((unsigned)(a.row_tiles * a.cache.kv_heads), (unsigned)sequences);
+    hipLaunchKernelGGL((attention_kv8_many_kernel<T, CODE, D, WAVES, TREE, HALVES>), grid, dim3(64 * WAVES), bytes, stream, a);
     PTOAMD_HIP_CHECK(hipGetLastError());
     return PTOAMD_OK;
 }
@@ -523,9 +571,15 @@ template <typename T, int CODE, bool TREE>
 static int choose_size(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
     switch (built_head(a.cache.head_dim)) {
-        case 64: return launch_many<T, CODE, 64, 8, TREE>(a, sequences, stream);
-        case 128: return launch_many<T, CODE, 128, 8, TREE>(a, sequences, stream);
-        default: return launch_many<T, CODE, 256, 4, TREE>(a, sequences, stream);
+        case 64:
+            if (TREE && a.tile_rows == 128)
+                return launch_many<T, CODE, 64, 8, TREE, TREE>(a, sequences, stream);
+            return launch_many<T, CODE, 64, 8, TREE, false>(a, sequences, stream);
+        case 128:
+            if (TREE && a.tile_rows == 128)
+                return launch_many<T, CODE, 128, 8, TREE, TREE>(a, sequences, stream);
+            return launch_many<T, CODE, 128, 8, TREE, false>(a, sequences, stream);
+        default: return launch_many<T, CODE, 256, 4, TREE, false>(a, sequences, stream);
     }
 }
 

@@ -32,17 +32,4 @@ __device__ __forceinline__ uint2 kv8_codes(const float* x)
 template <int CODE>
 constexpr float KV8_PER_LARGEST = CODE == PTOAMD_I8 ? 1.0f / 127.0f : 1.0f / 448.0f;  // a page's scale over its largest magnitude
 
-template <typename T, bool WIDE>
-__device__ __forceinline__ void load8(const T* p, float* x)
-{
-    struct alignas(WIDE ? 16 : sizeof(T)) V { T e[16 / sizeof(T)]; };
-    V v[8 * sizeof(T) / 16];
-#pragma unroll
-    for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
-        v[i] = reinterpret_cast<const V*>(p)[i];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = (float)v[i * sizeof(T) / 16].e[i % (16 / sizeof(T))];
-}
-
 }  // namespace ptoamd

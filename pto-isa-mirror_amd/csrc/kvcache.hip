@@ -54,6 +54,19 @@ struct AppendArgs {
     int blocks;                      // most pages that a sequence's new tokens touch
 };
 
+template <typename T, bool WIDE>
+__device__ __forceinline__ void load8(const T* p, float* x)
+{
+    struct alignas(WIDE ? 16 : sizeof(T)) V { T e[16 / sizeof(T)]; };
+    V v[8 * sizeof(T) / 16];
+#pragma unroll
+    for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
+        v[i] = reinterpret_cast<const V*>(p)[i];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = (float)v[i * sizeof(T) / 16].e[i % (16 / sizeof(T))];
+}
+
 // One workgroup a page of a sequence, head, and side (keys or values).  The new tokens' largest magnitude gives the page's scale, which
 // only grows; where it grows, the older tokens' codes are rounded again to the new one.  A thread has 8 elements of a row at a time.
 // Magnitudes are compared as integers, so that an infinity or a NaN among them is the largest, whatever the order.

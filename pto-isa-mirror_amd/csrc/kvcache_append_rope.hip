@@ -20,7 +20,8 @@ struct AppendRopeArgs {
     int tree_words;                                // of 32 bits
     int table_rows, half, heads, interleaved;
     int blocks;                                    // most pages that a sequence's new tokens touch
-    unsigned append_groups, wide;                  // workgroups of the append; those that a token's queries take
+    unsigned wide, pairs;                          // workgroups that the queries of two tokens take; such pairs of a sequence
+    uint64_t share;                                // of the workgroups that append, in 2^-32
 
     // the position that the nth new token of a sequence, row `row` of the operands, is turned by; `start` is its first new token's place
     __device__ __forceinline__ int position(int row, int nth, int count, int start) const
@@ -31,118 +32,132 @@ struct AppendRopeArgs {
     }
 };
 
-// The order of a head's elements in 16s, a thread's unit: 8 elements and the 8 that they are paired with, so that a pair is one thread's.  HALVES: i and
-// i + half; NEIGHBOURS: 2 i and 2 i + 1.  ANY is for rotations that are not made of 16s, and for operands off 16 bytes: elements one by one.
-enum RopeOrder { HALVES, NEIGHBOURS, ANY };
-struct Chunks {
-    int lo, hi;  // the unit's two runs of 8 elements; the same one twice where only 8 are left
+// A thread's unit of a head: VEC pairs, so that a pair is one thread's, as two runs of VEC elements: half a rotation apart or, INTERLEAVED, next to each other;
+// of the elements behind the rotation two runs next to each other.  (Where VEC elements are left there, the same run twice.)
+struct Runs {
+    int lo, hi;
 };
-template <RopeOrder ORDER>
-__device__ __forceinline__ Chunks chunks_of(int u, int half, int dim)
+template <int VEC, bool INTERLEAVED>
+__device__ __forceinline__ Runs runs_of(int u, int half, int dim)
 {
-    const int lo = ORDER == HALVES && 8 * u < half ? 8 * u : 16 * u, hi = ORDER == HALVES && 8 * u < half ? 8 * u + half : 16 * u + 8;
-    return Chunks{lo, hi < dim ? hi : lo};
+    const bool apart = !INTERLEAVED && VEC * u < half;
+    const int lo = apart ? VEC * u : 2 * VEC * u, hi = apart ? lo + half : lo + VEC;
+    return Runs{lo, hi < dim ? hi : lo};
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void load_run(const T* p, float* x)
+{
+    constexpr int EACH = VEC * sizeof(T) > 16 ? 16 / sizeof(T) : VEC;
+    struct alignas(EACH * sizeof(T)) V { T e[EACH]; };
+    V v[VEC / EACH];
+#pragma unroll
+    for (int i = 0; i < VEC / EACH; ++i)
+        v[i] = reinterpret_cast<const V*>(p)[i];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+        x[i] = (float)v[i / EACH].e[i % EACH];
+}
+template <typename T, int VEC>
+__device__ __forceinline__ void store_run(T* p, const float* x)
+{
+    constexpr int EACH = VEC * sizeof(T) > 16 ? 16 / sizeof(T) : VEC;
+    struct alignas(EACH * sizeof(T)) V { T e[EACH]; };
+    V v[VEC / EACH];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+        v[i / EACH].e[i % EACH] = (T)x[i];
+#pragma unroll
+    for (int i = 0; i < VEC / EACH; ++i)
+        reinterpret_cast<V*>(p)[i] = v[i];
+}
+template <int CODE, int VEC>
+__device__ __forceinline__ void store_codes(uint8_t* p, const float* x)
+{
+    float eight[8] = {};
+#pragma unroll
+    for (int i = 0; i < VEC; ++i)
+        eight[i] = x[i];
+    const uint2 w = kv8_codes<CODE>(eight);
+    if constexpr (VEC == 8)
+        *reinterpret_cast<uint2*>(p) = w;
+    else if constexpr (VEC == 4)
+        *reinterpret_cast<uint32_t*>(p) = w.x;
+    else
+        *p = (uint8_t)w.x;
 }
 
 // A unit of a row, turned.  (A position that the table does not have: NaN.)
-template <typename T, RopeOrder ORDER>
+template <typename T, int VEC, bool INTERLEAVED>
 __device__ __forceinline__ void load_turned(const AppendRopeArgs& a, const T* row, int position, int u, int dim, float* x)
 {
-    const bool known = (unsigned)position < (unsigned)a.table_rows;
-    const float* turn = a.table + (int64_t)(known ? position : 0) * 2 * a.half;
-    const float unknown = known ? 0.0f : NAN;
-    if constexpr (ORDER == ANY) {
+    const Runs at = runs_of<VEC, INTERLEAVED>(u, a.half, dim);
+    load_run<T, VEC>(row + at.lo, x);
+    load_run<T, VEC>(row + at.hi, x + VEC);
+    if (VEC * u < a.half) {
+        const bool known = (unsigned)position < (unsigned)a.table_rows;
+        const float* turn = a.table + (int64_t)(known ? position : 0) * 2 * a.half + VEC * u;
+        const float unknown = known ? 0.0f : NAN;
+        float c[VEC], s[VEC];
+        load_run<float, VEC>(turn, c);
+        load_run<float, VEC>(turn + a.half, s);
 #pragma unroll
-        for (int j = 0; j < 16; ++j) {
-            const int e = min(16 * u + j, dim - 1);
-            x[j] = (float)row[e];
-            if (e < 2 * a.half) {
-                const int pair = a.interleaved ? e / 2 : e < a.half ? e : e - a.half;
-                const bool second = a.interleaved ? e % 2 != 0 : e >= a.half;
-                const int other = a.interleaved ? e ^ 1 : second ? e - a.half : e + a.half;
-                const float c = turn[pair] + unknown, s = turn[a.half + pair] + unknown, y = (float)row[other];
-                x[j] = second ? y * s + x[j] * c : x[j] * c - y * s;
-            }
-        }
-    } else {
-        const Chunks at = chunks_of<ORDER>(u, a.half, dim);
-        load8<T, true>(row + at.lo, x);
-        load8<T, true>(row + at.hi, x + 8);
-        if (8 * u < a.half) {
-            float c[8], s[8];
-            load8<float, true>(turn + 8 * u, c);
-            load8<float, true>(turn + a.half + 8 * u, s);
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const int p = ORDER == HALVES ? j : 2 * j, q = ORDER == HALVES ? j + 8 : 2 * j + 1;
-                const float first = x[p], second = x[q], cosine = c[j] + unknown, sine = s[j] + unknown;
-                x[p] = first * cosine - second * sine;
-                x[q] = first * sine + second * cosine;
-            }
+        for (int j = 0; j < VEC; ++j) {
+            const int p = INTERLEAVED ? 2 * j : j, q = INTERLEAVED ? 2 * j + 1 : j + VEC;
+            const float first = x[p], second = x[q], cosine = c[j] + unknown, sine = s[j] + unknown;
+            x[p] = first * cosine - second * sine;
+            x[q] = first * sine + second * cosine;
         }
     }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* p, const float* x)
-{
-    struct alignas(16) V { T e[16 / sizeof(T)]; };
-    V v[8 * sizeof(T) / 16];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        v[i * sizeof(T) / 16].e[i % (16 / sizeof(T))] = (T)x[i];
-#pragma unroll
-    for (int i = 0; i < (int)(8 * sizeof(T) / 16); ++i)
-        reinterpret_cast<V*>(p)[i] = v[i];
-}
 
-// Queries: a thread has a unit of one token's head.  (ANY: a pair, or one element behind the pairs, so that the result may lie where the operand does.)
-template <typename T, RopeOrder ORDER, int THREADS>
+constexpr int ROPE_TOKENS = 2;
+
+// Queries: a thread has a unit of a head of two consecutive tokens, all loads of both in flight before the first is used, as in rope.hip.
+template <typename T, int VEC, bool INTERLEAVED, int THREADS>
 __device__ __forceinline__ void turn_queries(const AppendRopeArgs& a, unsigned group)
 {
     const Kv8& c = a.cache;
     const unsigned row_group = group / a.wide;
-    const int seq = row_group / (unsigned)c.max_tokens, nth = row_group - (unsigned)seq * c.max_tokens;
+    const int seq = row_group / a.pairs, nth = (row_group - (unsigned)seq * a.pairs) * ROPE_TOKENS;
     const int first = c.first_token(seq), count = c.token_count(seq, first);
-    const int units = ORDER == ANY ? c.head_dim - a.half : (c.head_dim + 15) / 16;
+    const int units = (c.head_dim + 2 * VEC - 1) / (2 * VEC);
     const int unit = (group - row_group * a.wide) * THREADS + threadIdx.x, head = unit / units, u = unit - head * units;
     if (nth >= count || head >= a.heads)
         return;
-    const int position = a.position(first + nth, nth, count, max(c.lengths[seq], 0) - count);
-    const T* x = reinterpret_cast<const T*>(a.q + (int64_t)(first + nth) * a.q_token + (int64_t)head * a.q_head);
-    T* out = reinterpret_cast<T*>(a.q_out + (int64_t)(first + nth) * a.out_token + (int64_t)head * a.out_head);
-    if constexpr (ORDER == ANY) {
-        if (u >= a.half) {
-            out[u + a.half] = x[u + a.half];
-            return;
-        }
-        const bool known = (unsigned)position < (unsigned)a.table_rows;
-        const float* turn = a.table + (int64_t)(known ? position : 0) * 2 * a.half;
-        const float cosine = known ? turn[u] : NAN, sine = known ? turn[a.half + u] : NAN;
-        const int i = a.interleaved ? 2 * u : u, j = a.interleaved ? 2 * u + 1 : u + a.half;
-        const float p = (float)x[i], q = (float)x[j];
-        out[i] = (T)(p * cosine - q * sine);
-        out[j] = (T)(p * sine + q * cosine);
-    } else {
-        float y[16];
-        load_turned<T, ORDER>(a, x, position, u, c.head_dim, y);
-        const Chunks at = chunks_of<ORDER>(u, a.half, c.head_dim);
-        store8(out + at.lo, y);
-        store8(out + at.hi, y + 8);
+    const int start = max(c.lengths[seq], 0) - count;
+    const uint8_t* x = a.q + (int64_t)head * a.q_head;
+    uint8_t* out = a.q_out + (int64_t)head * a.out_head;
+    const Runs at = runs_of<VEC, INTERLEAVED>(u, a.half, c.head_dim);
+    float y[ROPE_TOKENS][2 * VEC];
+#pragma unroll
+    for (int k = 0; k < ROPE_TOKENS; ++k) {
+        const int token = min(nth + k, count - 1), row = first + token;
+        load_turned<T, VEC, INTERLEAVED>(a, reinterpret_cast<const T*>(x + (int64_t)row * a.q_token), a.position(row, token, count, start), u, c.head_dim, y[k]);
+    }
+#pragma unroll
+    for (int k = 0; k < ROPE_TOKENS; ++k) {
+        if (nth + k >= count)
+            break;
+        T* to = reinterpret_cast<T*>(out + (int64_t)(first + nth + k) * a.out_token);
+        store_run<T, VEC>(to + at.lo, y[k]);
+        store_run<T, VEC>(to + at.hi, y[k] + VEC);
     }
 }
 
-// The first workgroups append, one a page of a sequence, head and side (keys or values): the append of kvcache.hip, with keys turned as they are read.  The
-// others turn queries.  Products and sums in f32; a key is rounded once, to its code.
-template <typename T, int CODE, RopeOrder ORDER, int THREADS>
+// Some workgroups append, one a page of a sequence, head and side (keys or values): the append of kvcache.hip, with keys turned as they are read.  The
+// others turn queries; the two kinds stand among each other in the grid, since a page's chain of loads leaves the memory to the queries.
+// Products and sums in f32; a key is rounded once, to its code.
+template <typename T, int CODE, int VEC, bool INTERLEAVED, int THREADS>
 __global__ void __launch_bounds__(THREADS) kvcache_append_rope_kernel(AppendRopeArgs a)
 {
     const Kv8& c = a.cache;
-    if (blockIdx.x >= a.append_groups) {
-        turn_queries<T, ORDER, THREADS>(a, blockIdx.x - a.append_groups);
+    const unsigned before_it = (unsigned)((blockIdx.x * a.share) >> 32);
+    if ((unsigned)(((blockIdx.x + 1) * a.share) >> 32) == before_it) {
+        turn_queries<T, VEC, INTERLEAVED, THREADS>(a, blockIdx.x - before_it);
         return;
     }
-    const bool values = blockIdx.x % 2 != 0;
-    const unsigned page_head = blockIdx.x / 2, nth_page = page_head / (unsigned)c.kv_heads;
+    const bool values = before_it % 2 != 0;
+    const unsigned page_head = before_it / 2, nth_page = page_head / (unsigned)c.kv_heads;
     const int head = page_head - nth_page * c.kv_heads, seq = nth_page / (unsigned)a.blocks, nth = nth_page - seq * (unsigned)a.blocks;
     const Kv8Side side = values ? c.v : c.k;
     const int first = c.first_token(seq), count = c.token_count(seq, first), length = c.length(seq);
@@ -157,25 +172,37 @@ __global__ void __launch_bounds__(THREADS) kvcache_append_rope_kernel(AppendRope
     if (page < 0)
         return;
     const int older = lo - (block << c.page_shift), fresh = hi - lo;
-    const int per_token = (c.head_dim + 15) / 16, units = fresh * per_token;
+    const int per_token = (c.head_dim + 2 * VEC - 1) / (2 * VEC), units = fresh * per_token;
     const uint8_t* src = a.src[values] + (int64_t)head * a.head[values];
     auto load = [&](int token, int u, float* x) __attribute__((always_inline)) {  // of the page's new tokens
         const int row_at = first + lo - start + token;
         const T* row = reinterpret_cast<const T*>(src + (int64_t)row_at * a.token[values]);
         if (values) {
-            const Chunks at = chunks_of<ANY>(u, 0, c.head_dim);
-            load8<T, ORDER != ANY>(row + at.lo, x);
-            load8<T, ORDER != ANY>(row + at.hi, x + 8);
+            const Runs at = runs_of<VEC, true>(u, 0, c.head_dim);
+            load_run<T, VEC>(row + at.lo, x);
+            load_run<T, VEC>(row + at.hi, x + VEC);
         } else {
-            load_turned<T, ORDER>(a, row, a.position(row_at, lo - start + token, count, start), u, c.head_dim, x);
+            load_turned<T, VEC, INTERLEAVED>(a, row, a.position(row_at, lo - start + token, count, start), u, c.head_dim, x);
         }
     };
     uint32_t largest = 0;
-    for (int u = threadIdx.x; u < units; u += THREADS) {
-        float x[16];
+    constexpr int HELD = 16 / VEC;  // units of a thread that stay in registers, 32 values; others, of pages of more than 32 KB a head, are read again
+    float held[HELD][2 * VEC];
+#pragma unroll
+    for (int h = 0; h < HELD; ++h) {
+        const int u = min((int)threadIdx.x + h * THREADS, units - 1);
+        load(u / per_token, u % per_token, held[h]);
+    }
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+#pragma unroll
+        for (int i = 0; i < 2 * VEC; ++i)
+            largest = max(largest, f2u(held[h][i]) & 0x7FFFFFFFu);
+    for (int u = threadIdx.x + HELD * THREADS; u < units; u += THREADS) {
+        float x[2 * VEC];
         load(u / per_token, u % per_token, x);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 2 * VEC; ++i)
             largest = max(largest, f2u(x[i]) & 0x7FFFFFFFu);
     }
     __shared__ uint32_t wave_largest[THREADS / 64];
@@ -212,56 +239,74 @@ __global__ void __launch_bounds__(THREADS) kvcache_append_rope_kernel(AppendRope
         }
     }
     const float inverse = after > 0.0f ? 1.0f / after : 0.0f;
-    for (int u = threadIdx.x; u < units; u += THREADS) {
+    auto write = [&](int u, float* x) __attribute__((always_inline)) {
         const int token = u / per_token;
-        float x[16];
-        load(token, u % per_token, x);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
+        for (int i = 0; i < 2 * VEC; ++i)
             x[i] = inverse > 0.0f ? x[i] * inverse : 0.0f;  // (a NaN scale: codes of zero)
-        const Chunks at = values ? chunks_of<ANY>(u % per_token, 0, c.head_dim) : chunks_of<ORDER>(u % per_token, a.half, c.head_dim);
+        const Runs at = values ? runs_of<VEC, true>(u % per_token, 0, c.head_dim) : runs_of<VEC, INTERLEAVED>(u % per_token, a.half, c.head_dim);
         uint8_t* to = dst + (int64_t)(older + token) * side.token;
-        *reinterpret_cast<uint2*>(to + at.lo) = kv8_codes<CODE>(x);
-        if (at.hi != at.lo)
-            *reinterpret_cast<uint2*>(to + at.hi) = kv8_codes<CODE>(x + 8);
+        store_codes<CODE, VEC>(to + at.lo, x);
+        store_codes<CODE, VEC>(to + at.hi, x + VEC);
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+        if (threadIdx.x + h * THREADS < (unsigned)units)
+            write(threadIdx.x + h * THREADS, held[h]);
+    for (int u = threadIdx.x + HELD * THREADS; u < units; u += THREADS) {
+        float x[2 * VEC];
+        load(u / per_token, u % per_token, x);
+        write(u, x);
     }
 }
 
-template <typename T, int CODE, RopeOrder ORDER, int THREADS>
+template <typename T, int CODE, int VEC, bool INTERLEAVED, int THREADS>
 static int launch_append_rope(AppendRopeArgs a, int sequences, hipStream_t stream)
 {
-    const long units = (long)a.heads * (ORDER == ANY ? a.cache.head_dim - a.half : (a.cache.head_dim + 15) / 16);
+    const long units = (long)a.heads * ((a.cache.head_dim + 2 * VEC - 1) / (2 * VEC));
     const long wide = (units + THREADS - 1) / THREADS, append = 2L * sequences * a.blocks * a.cache.kv_heads;
-    const long groups = append + (long)sequences * a.cache.max_tokens * wide;
+    const long pairs = (a.cache.max_tokens + ROPE_TOKENS - 1) / ROPE_TOKENS, groups = append + sequences * pairs * wide;
     PTOAMD_REQUIRE(groups <= 0x7FFFFFFF, PTOAMD_E_UNSUPPORTED, "ptoamd_kvcache_append_rope: %d sequences of %d tokens are too many for one launch", sequences,
                    a.cache.max_tokens);
-    a.append_groups = (unsigned)append;
     a.wide = (unsigned)(wide > 0 ? wide : 1);
-    hipLaunchKernelGGL((kvcache_append_rope_kernel<T, CODE, ORDER, THREADS>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a);
+    a.pairs = (unsigned)pairs;
+    a.share = (((uint64_t)append << 32) + groups - 1) / groups;  // (rounded up: after all workgroups, all of the append have been)
+    hipLaunchKernelGGL((kvcache_append_rope_kernel<T, CODE, VEC, INTERLEAVED, THREADS>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a);
     PTOAMD_HIP_CHECK(hipGetLastError());
     set_last_kernel("kvcache_append_rope");
     return PTOAMD_OK;
 }
 // Threads by the bytes that a page's new tokens have of a head, as in kvcache.hip.
-template <typename T, int CODE, RopeOrder ORDER>
+template <typename T, int CODE, int VEC, bool INTERLEAVED>
 static int choose_threads(const AppendRopeArgs& a, int sequences, hipStream_t stream)
 {
     const int page = 1 << a.cache.page_shift;
     const long bytes = (long)(a.cache.max_tokens < page ? a.cache.max_tokens : page) * a.cache.head_dim * sizeof(T);
     if (bytes <= 8192)
-        return launch_append_rope<T, CODE, ORDER, 128>(a, sequences, stream);
-    return bytes <= 16384 ? launch_append_rope<T, CODE, ORDER, 256>(a, sequences, stream) : launch_append_rope<T, CODE, ORDER, 512>(a, sequences, stream);
+        return launch_append_rope<T, CODE, VEC, INTERLEAVED, 128>(a, sequences, stream);
+    if (bytes <= 16384)
+        return launch_append_rope<T, CODE, VEC, INTERLEAVED, 256>(a, sequences, stream);
+    return launch_append_rope<T, CODE, VEC, INTERLEAVED, 512>(a, sequences, stream);
+}
+// Runs of eight elements where the rotation is made of them and operands start on theirs (16 bytes), else of four, else single elements.
+template <typename T, int CODE, bool INTERLEAVED>
+static int choose_run(const AppendRopeArgs& a, int sequences, hipStream_t stream)
+{
+    uint64_t bits = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.q_out | (uint64_t)a.q_token | (uint64_t)a.q_head | (uint64_t)a.out_token |
+                    (uint64_t)a.out_head;
+    for (int i = 0; i < 2; ++i)
+        bits |= (uint64_t)(uintptr_t)a.src[i] | (uint64_t)a.token[i] | (uint64_t)a.head[i];
+    const uint64_t table = (uint64_t)(uintptr_t)a.table;
+    if (a.half % 8 == 0 && bits % 16 == 0 && table % 16 == 0)
+        return choose_threads<T, CODE, 8, INTERLEAVED>(a, sequences, stream);
+    if (a.half % 4 == 0 && bits % (4 * sizeof(T)) == 0 && table % 16 == 0)
+        return choose_threads<T, CODE, 4, INTERLEAVED>(a, sequences, stream);
+    return launch_append_rope<T, CODE, 1, INTERLEAVED, 256>(a, sequences, stream);
 }
 template <typename T, int CODE>
 static int choose_order(const AppendRopeArgs& a, int sequences, hipStream_t stream)
 {
-    uint64_t bits = (uint64_t)(uintptr_t)a.q | (uint64_t)(uintptr_t)a.q_out | (uint64_t)(uintptr_t)a.table | (uint64_t)a.q_token | (uint64_t)a.q_head |
-                    (uint64_t)a.out_token | (uint64_t)a.out_head;
-    for (int i = 0; i < 2; ++i)
-        bits |= (uint64_t)(uintptr_t)a.src[i] | (uint64_t)a.token[i] | (uint64_t)a.head[i];
-    if (a.half % 8 != 0 || bits % 16 != 0)
-        return choose_threads<T, CODE, ANY>(a, sequences, stream);
-    return a.interleaved ? choose_threads<T, CODE, NEIGHBOURS>(a, sequences, stream) : choose_threads<T, CODE, HALVES>(a, sequences, stream);
+    return a.interleaved ? choose_run<T, CODE, true>(a, sequences, stream) : choose_run<T, CODE, false>(a, sequences, stream);
 }
 template <typename T>
 static int choose_code(const AppendRopeArgs& a, int code, int sequences, hipStream_t stream)

@@ -115,6 +115,10 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 // Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
 // (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
 // heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.
+// Of drafted tokens parts are down to one turn of eight waves, as many as one workgroup a CU leaves; whole up to 1024 keys of heads of 64, 768 of 128, 512 of 256.
+// us, whole / parts of 256, 512 keys, 64 / 8 heads of 128: 1 token over 600, 1000, 2000 keys 9.6 / 10.5, 12.2 / 10.7, 17.6 / 10.7; 4 x 6 tokens over 1000, 2000
+// 15.8 / 16.3, 21.4 / 26.8 / 17.9 (two groups of rows: 512 workgroups); 6 over 5000 39 / 25.4 / 16.8; of 64, 4 x 6 over 1000 10.9 / 13.1; 16 / 2 of 256, 2 over 600
+// 14.8 / 14.3.
 // Many rows: in equal stretches (Cuts) where that is less than a tile of rows' keys by more than the second start and the join cost (800 keys of
 // heads of 128, 1600 of 64, 400 of 256); several sequences, whose lengths the host does not know, count as half of the longest.  us, whole / cut, 32 / 8 heads of 128:
 //   128 tokens over 700, 1024, 1500 keys 30 / 35, 38 / 37, 52 / 39; 512 over 700, 1024, 1500, 2500, 16384 30 / 38, 38 / 42, 52 / 47, 78 / 55, 441 / 174;
@@ -152,12 +156,19 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     p.kernel = rows <= (!fewer ? 96 : dim == 256 ? 32 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
     if (p.kernel == AttentionPlan::FEW) {
         p.row_tiles = rows <= 16 || dim == 256 ? 1 : rows <= 32 || !busy ? 2 : rows <= 48 ? 3 : dim == 128 ? 4 : 2;
-        const long step = 32 * few_waves(dim, p.row_tiles);  // the keys that a workgroup's waves have at a time
+        const long step = 32 * few_waves(dim, p.row_tiles, tree);  // the keys that a workgroup's waves have at a time
         const long turns = (keys + step - 1) / step;
         long splits = (cus + items - 1) / items;
         splits = splits < turns / 2 ? splits : turns / 2;
         if (turns <= (dim == 256 ? 4 : 6))
             splits = 1;
+        if (tree) {
+            const long groups = items * ((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
+            splits = groups < cus ? cus / groups : 1;
+            splits = splits < turns ? splits : turns;
+            if (turns <= (dim == 64 ? 4 : dim == 128 ? 3 : 2))
+                splits = 1;
+        }
         const long even = (keys + 4095) / 4096;
         splits = splits > even ? splits : even;
         const long most = room < 65535 ? room : 65535;  // (parts are a grid's slowest index)

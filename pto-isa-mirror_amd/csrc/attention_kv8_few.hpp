@@ -35,9 +35,11 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
     constexpr int STEPS = D / 32, VW = D / 64, MT = D / 16, PITCH = D + 4;
     constexpr int RING = 2;  // tiles of a wave in registers
     constexpr int STRIDE = 32 * WAVES;
+    constexpr bool Q_IN_LDS = few_queries_in_lds(D, NT, TREE);
     extern __shared__ __attribute__((aligned(16))) float shared[];  // [WAVES / 2][16 NT][PITCH]
     __shared__ float wave_top[WAVES][16 * NT], wave_sum[WAVES][16 * NT];
-    __shared__ uint32_t drafted[TREE ? WAVES : 1][TREE ? 16 * NT : 1][FEW_TREE_WORDS];
+    __shared__ uint4 queries[Q_IN_LDS ? NT * STEPS : 1][Q_IN_LDS ? 64 : 1];
+    __shared__ uint32_t drafted[TREE ? WAVES : 1][TREE ? 16 * NT : 1][FEW_TREE_WORDS + 1];  // (last: the first of the older keys that the row sees)
     const Kv8& c = a.cache;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 16, g = lane / 16;
     // (workgroups go to the XCDs in turn: parts, of which short sequences leave most empty, are the slowest index)
@@ -108,13 +110,13 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
 
     // the queries, as fragments: step st = 2 cc + e of a lane is elements 64 cc + 16 g + 8 e ..
     uint4 q[NT][STEPS];
-    int2 seen[NT];  // (TREE: x, the first of the older keys)
+    int2 seen[NT];
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         const int row = row0 + 16 * t + col, token = row / a.group;
         const bool valid = row < rows;
         if constexpr (TREE)
-            seen[t].x = first_of_drafted<FEW_TREE_WORDS>(a, span, drafted[wave][16 * t + col], valid, token);
+            drafted[wave][16 * t + col][FEW_TREE_WORDS] = first_of_drafted<FEW_TREE_WORDS>(a, span, drafted[wave][16 * t + col], valid, token);
         else
             seen[t] = valid ? visible_keys(a, span.length - span.count + token, span.length) : make_int2(0, 0);
         const uint8_t* p = a.q + (int64_t)(span.first + (valid ? token : 0)) * a.q_token + (int64_t)(kv_head * a.group + (valid ? row - token * a.group : 0)) * a.q_head;
@@ -130,6 +132,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
     }
     float cq[NT];  // what a product of codes is multiplied with beside the key scale, in units of log2
     f32x4 start[NT];
+    float bias[NT];  // (TREE: what `start` is, for all keys, taken off where scores are scaled: one register for four)
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
         uint32_t largest = largest_of<STEPS>(q[t]);
@@ -146,6 +149,13 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
             for (int st = 0; st < STEPS; ++st)
                 start[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, unbias), __builtin_bit_cast(f16x8, q[t][st]), start[t], 0, 0, 0);
         }
+        bias[t] = start[t][0];
+        if (TREE)
+            start[t] = f32x4{0, 0, 0, 0};
+        if constexpr (Q_IN_LDS)  // (every wave the same, and each reads behind its own)
+#pragma unroll
+            for (int st = 0; st < STEPS; ++st)
+                queries[t * STEPS + st][lane] = q[t][st];
     }
     // tiles of keys that every row sees need no mask; keys that none sees have their codes cleared
     const int every_from = first_key(span.length - 1, a.window);
@@ -164,6 +174,8 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
     }
 
     auto compute = [&](FewTile<D>& tile, int key) __attribute__((always_inline)) {
+        if constexpr (Q_IN_LDS)
+            asm volatile("" ::: "memory");  // (or the queries are read once, into registers)
         const int scale = (int)f2u(tile.scale + tile.unknown);
         const float ks[2] = {u2f(__builtin_amdgcn_readlane(scale, 0)), u2f(__builtin_amdgcn_readlane(scale, 1))};
         const float vs[2] = {u2f(__builtin_amdgcn_readlane(scale, 2)), u2f(__builtin_amdgcn_readlane(scale, 3))};
@@ -187,8 +199,10 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
                         f = make_uint4(kv8_pair_to_f16<CODE, false>(w[2 * e]), kv8_pair_to_f16<CODE, true>(w[2 * e]),
                                        kv8_pair_to_f16<CODE, false>(w[2 * e + 1]), kv8_pair_to_f16<CODE, true>(w[2 * e + 1]));
 #pragma unroll
-                    for (int t = 0; t < NT; ++t)
-                        s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, f), __builtin_bit_cast(f16x8, q[t][2 * cc + e]), s[t][h], 0, 0, 0);
+                    for (int t = 0; t < NT; ++t) {
+                        const uint4 its = Q_IN_LDS ? queries[t * STEPS + 2 * cc + e][lane] : q[t][2 * cc + e];
+                        s[t][h] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, f), __builtin_bit_cast(f16x8, its), s[t][h], 0, 0, 0);
+                    }
                 }
             });
         }
@@ -200,13 +214,14 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
             float w[2][4], high = -INFINITY;
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float scale = cq[t] * ks[h];
+                const float scale = cq[t] * ks[h], add = TREE && CODE == PTOAMD_I8 ? fmaf(bias[t], scale, value[h].log2) : value[h].log2;
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-                    w[h][i] = fmaf(s[t][h][i], scale, value[h].log2);
+                    w[h][i] = fmaf(s[t][h][i], scale, add);
             }
             if (TREE && !whole) {
-                const uint32_t mine = drafted_keys<FEW_TREE_WORDS>(drafted[wave][16 * t + col], key, seen[t].x, every_to) >> (4 * g);
+                const uint32_t* row = drafted[wave][16 * t + col];
+                const uint32_t mine = drafted_keys<FEW_TREE_WORDS>(row, key, (int)row[FEW_TREE_WORDS], every_to) >> (4 * g);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     w[j / 4][j % 4] = (mine & 1u << (16 * (j / 4) + j % 4)) != 0 ? w[j / 4][j % 4] : -INFINITY;
@@ -400,10 +415,10 @@ static int choose_tiles(const AttentionArgs& a, int sequences, hipStream_t strea
 {
     // (two tiles of 256 columns' sums and fragments do not fit the registers, nor four of 128 columns more than one wave a SIMD)
     switch (a.row_tiles) {
-        case 1: return launch_few<T, CODE, D, 1, few_waves(D, 1), TREE>(a, sequences, stream);
-        case 2: if constexpr (D < 256) return launch_few<T, CODE, D, 2, few_waves(D, 2), TREE>(a, sequences, stream); break;
-        case 3: if constexpr (D < 256) return launch_few<T, CODE, D, 3, few_waves(D, 3), TREE>(a, sequences, stream); break;
-        case 4: if constexpr (D == 128) return launch_few<T, CODE, D, 4, few_waves(D, 4), TREE>(a, sequences, stream); break;
+        case 1: return launch_few<T, CODE, D, 1, few_waves(D, 1, TREE), TREE>(a, sequences, stream);
+        case 2: if constexpr (D < 256) return launch_few<T, CODE, D, 2, few_waves(D, 2, TREE), TREE>(a, sequences, stream); break;
+        case 3: if constexpr (D < 256) return launch_few<T, CODE, D, 3, few_waves(D, 3, TREE), TREE>(a, sequences, stream); break;
+        case 4: if constexpr (D == 128) return launch_few<T, CODE, D, 4, few_waves(D, 4, TREE), TREE>(a, sequences, stream); break;
     }
     return PTOAMD_E_INVALID;  // (no plan has it)
 }

@@ -115,7 +115,10 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 // Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
 // (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
 // heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.
-// Of drafted tokens parts are down to one turn of eight waves, as many as one workgroup a CU leaves; whole up to 1024 keys of heads of 64, 768 of 128, 512 of 256.
+// Of drafted tokens 16 rows a workgroup where every such tile has a CU and they have no more than four turns each: us, two tiles a workgroup / one, 64 / 8 heads of
+// 128: 6 tokens over 300 keys 10.8 / 8.4, 1000 14.2 / 11.6, 4000 16.1 / 13.6, 16000 21.6 / 22.2; 4 x 8 over 1000 17.5 / 15.7, over 4000 22.8 / 24.0; 16 x 3 over
+// 1000 20.1 / 13.9; 16 x 6 over 300, 384 tiles, 11.2 / 15.0; of 64, 6 over 300 7.5 / 5.9.  And parts are down to one turn
+// of eight waves, as many as one workgroup a CU leaves; whole up to 1024 keys of heads of 64, 768 of 128, 512 of 256.
 // us, whole / parts of 256, 512 keys, 64 / 8 heads of 128: 1 token over 600, 1000, 2000 keys 9.6 / 10.5, 12.2 / 10.7, 17.6 / 10.7; 4 x 6 tokens over 1000, 2000
 // 15.8 / 16.3, 21.4 / 26.8 / 17.9 (two groups of rows: 512 workgroups); 6 over 5000 39 / 25.4 / 16.8; of 64, 4 x 6 over 1000 10.9 / 13.1; 16 / 2 of 256, 2 over 600
 // 14.8 / 14.3.
@@ -156,6 +159,11 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     p.kernel = rows <= (!fewer ? 96 : dim == 256 ? 32 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
     if (p.kernel == AttentionPlan::FEW) {
         p.row_tiles = rows <= 16 || dim == 256 ? 1 : rows <= 32 || !busy ? 2 : rows <= 48 ? 3 : dim == 128 ? 4 : 2;
+        if (tree) {
+            const long alone = items * ((rows + 15) / 16);
+            if (alone <= cus && alone * ((keys + 255) / 256) <= 4 * cus)
+                p.row_tiles = 1;
+        }
         const long step = 32 * few_waves(dim, p.row_tiles, tree);  // the keys that a workgroup's waves have at a time
         const long turns = (keys + step - 1) / step;
         long splits = (cus + items - 1) / items;

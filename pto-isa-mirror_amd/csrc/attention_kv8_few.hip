@@ -102,8 +102,9 @@ static void launch_join(const AttentionArgs& a, int sequences, hipStream_t strea
 {
     const long rows = (long)a.cache.max_tokens * a.heads;
     constexpr int ROWS = 1024 / D;
-    // (rows for four workgroups a compute unit, of a group of lanes each: before that a row's parts are what keeps the card busy)
-    if (rows * sequences >= 4L * ROWS * device_compute_units())
+    // (rows for four workgroups a compute unit, of a group of lanes each: before that a row's parts are what keeps the card busy.  Of drafted tokens, also where
+    // the parts are few: 16 x 6 tokens over 4000 keys in two, 64 / 8 heads of 128, 47.8 us with a row a workgroup, 43.0; one over 1000 in four 10.7 and 11.1)
+    if (rows * sequences >= 4L * ROWS * device_compute_units() || (a.tree != nullptr && a.splits <= 4))
         hipLaunchKernelGGL((attention_kv8_join_kernel<T, D, ROWS>), dim3((unsigned)((rows + ROWS - 1) / ROWS), 1, (unsigned)sequences), dim3(256), 0, stream, a);
     else
         hipLaunchKernelGGL((attention_kv8_join_kernel<T, D, 1>), dim3((unsigned)rows, 1, (unsigned)sequences), dim3(256), 0, stream, a);

@@ -177,40 +177,52 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         const int row = row0 + 32 * wave + col, token = row / a.group;
         const bool valid = row < rows;
         const int head = kv_head * a.group + (valid ? row - token * a.group : 0);
-        int2 seen;  // (TREE: x, the first of the older keys)
-        if constexpr (TREE) {
-            for (int i = lane; i < 32 * MANY_TREE_WORDS; i += 64) {  // (a wave's own rows)
-                const int its = 32 * wave + i / MANY_TREE_WORDS, word = i % MANY_TREE_WORDS;
-                drafted[its][word] = row0 + its < rows ? drafted_word(a, span, (row0 + its) / a.group, word) : 0u;
+        // The queries, the TREE's rows of bits and, behind them, the first tile's codes are asked for before any of them is waited for.
+        constexpr int ROW_WORDS = 32 * MANY_TREE_WORDS / 64;
+        uint32_t words[ROW_WORDS];  // (of a wave's own rows)
+        if constexpr (TREE)
+#pragma unroll
+            for (int i = 0; i < ROW_WORDS; ++i) {
+                const int its = row0 + 32 * wave + (lane + 64 * i) / MANY_TREE_WORDS, word = lane % MANY_TREE_WORDS;
+                words[i] = a.tree[(int64_t)(span.first + (its < rows ? its / a.group : 0)) * a.tree_words + (word < a.tree_words ? word : 0)];
             }
-            seen.x = first_of_drafted<MANY_TREE_WORDS>(a, span, drafted[32 * wave + col], valid, token);
-        } else {
-            seen = valid ? visible_keys(a, place0 + token, span.length) : make_int2(0, 0);
-        }
         uint4 q[STEPS];
-        float cq;
         {
             const uint8_t* p = a.q + (int64_t)(span.first + (valid ? token : 0)) * a.q_token + (int64_t)head * a.q_head;
 #pragma unroll
             for (int st = 0; st < STEPS; ++st)
                 q[st] = valid && 16 * st < c.head_dim ? load_row8(p + 2 * (16 * st + 8 * hf), a.wide) : make_uint4(0, 0, 0, 0);
+        }
+        int2 seen = make_int2(0, 0);  // (TREE: x, the first of the older keys)
+        float cq = 0.0f, bias = 0.0f;
+        // where a row's scores start: without the 128 that the keys' int8 codes carry.  (TREE: taken off where scores are scaled, in one register for 16)
+        f32x16 start = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        auto take_queries = [&]() __attribute__((always_inline)) {
+            if constexpr (TREE) {
+#pragma unroll
+                for (int i = 0; i < ROW_WORDS; ++i) {
+                    const int its = 32 * wave + (lane + 64 * i) / MANY_TREE_WORDS, word = lane % MANY_TREE_WORDS;
+                    drafted[its][word] = row0 + its < rows && word < a.tree_words ? words[i] & bits_below(span.count - 32 * word) : 0u;
+                }
+                seen.x = first_of_drafted<MANY_TREE_WORDS>(a, span, drafted[32 * wave + col], valid, token);
+            } else {
+                seen = valid ? visible_keys(a, place0 + token, span.length) : make_int2(0, 0);
+            }
             uint32_t largest = largest_of<STEPS>(q);
             largest = max(largest, (uint32_t)__shfl_xor((int)largest, 32));
             const RowScale r = row_scale<T>(largest);
             cq = r.up * (a.scale * 1.44269504088896341f) * KV8_UNIT<CODE>;
             scale_to_f16<T, STEPS>(q, r.down);
-        }
-        // where a row's scores start: without the 128 that the keys' int8 codes carry.  (TREE: taken off where scores are scaled, in one register for 16)
-        f32x16 start = {0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-        if (CODE == PTOAMD_I8) {
-            const uint4 unbias = make_uint4(UNBIAS, UNBIAS, UNBIAS, UNBIAS);
+            if (CODE == PTOAMD_I8) {
+                const uint4 unbias = make_uint4(UNBIAS, UNBIAS, UNBIAS, UNBIAS);
 #pragma unroll
-            for (int st = 0; st < STEPS; ++st)
-                start = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, unbias), __builtin_bit_cast(f16x8, q[st]), start, 0, 0, 0);
-        }
-        const float bias = start[0];  // (all keys')
-        if constexpr (TREE)
-            start = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                for (int st = 0; st < STEPS; ++st)
+                    start = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, unbias), __builtin_bit_cast(f16x8, q[st]), start, 0, 0, 0);
+            }
+            bias = start[0];  // (all keys')
+            if constexpr (TREE)
+                start = f32x16{0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+        };
         // the keys that every row of the wave sees
         const int wave_row = row0 + 32 * wave;
         const int2 every = keys_of_every<TREE>(a, span, min(wave_row, rows - 1) / a.group, (min(wave_row + 32, rows) - 1) / a.group);
@@ -445,6 +457,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
             for (int u = 0; u < UNITS; ++u)
                 fetch(u, 0);
+            take_queries();
             if (tid < KEYS / 16)
                 scale_id = table[min(own_begin + 16 * tid, last_key) >> c.page_shift];
             find(1);

@@ -106,18 +106,24 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 //          8000: 48 130 / 114, 64 168 / 115; 8 of 6000: 40 45 / 42, 64 59 / 45; one of 60000 40 57 / 52.
 //   many : more rows, 256 of them a workgroup (128 for heads of 256 elements)
 // Of drafted tokens, 128 rows a workgroup (HALVES) where there are no more: us, 256 rows a workgroup / 128, 16 sequences of 8192 keys, 64 / 8 heads of 128
-// E4M3, 16 tokens 147 / 105, one of 131072 150 / 110; of 64, 119 / 77; and 32 tokens, 256 rows, 179 / 180, 48 271 / 281, 64 291 / 334.  That kernel
-// and the few-rows one: heads of 128, 80 rows, 16 x 8192 163 / 100, 8 x 2000 and 1 x 16000 44 / 39 and 42 / 34, so from half as many keys on as above; 64 rows
-// 89 / 96, 33 / 37, 31 / 33; 96 rows over 2000 keys 15 / 25; of 64, 80 rows 92 / 87 of 16 x 8192, 27 / 32 of 8 x 2000.
+// E4M3, 16 tokens 147 / 105, one of 131072 150 / 110; of 64, 119 / 77; and 32 tokens, 256 rows, 179 / 180, 48 271 / 281, 64 291 / 334.  The
+// few-rows kernel takes up to 64 rows (32 of heads of 256), and more where its workgroups of 32 rows (16) fit the card at once, two to a CU but of
+// heads of 128, and have 16 turns of 256 keys a CU or fewer, 32 of heads of 64.  us, few / many, E4M3, rows a key head x sequences x keys, 64 / 8 heads of
+// 128: 512 x 1 x 300, 1000, 3000, 6000, 16000 9 / 21, 14 / 37, 24 / 42, 32 / 45, 72 / 65; 1024 x 1 x 3000 30 / 45; 256 x 1 x 16000 41 / 49, 60000
+// 137 / 90; 96 x 16 x 300 21 / 18, 128 x 16 x 1000 33 / 30, 512 x 4 x 1000 32 / 42, 3000 57 / 59; 256 x 4 x 3000 30 / 45; 128 x 8 x 2000, 4000 24 / 37,
+// 36 / 47; 80 x 16 x 8192 163 / 100; of 64: 512 x 4 x 1000, 3000 18 / 34, 31 / 46; 256 x 16 x 300 20 / 17; 768 x 2 x 8000 58 / 73; 128 x 16 x 4000
+// 39 / 49; 512 x 1 x 60000 133 / 115; 16 / 2 of 256: 512 x 4 x 1000 21 / 44; 1024 x 4 x 1000, 3000 38 / 52, 75 / 75; 512 x 16 x 1000 73 / 67;
+// 512 x 1 x 16000 53 / 61, 768 95 / 72; 128 x 16 x 4000 49 / 62, 256 91 / 86.
 // Few rows are 16, 32, or, where the keys are that many, up to 48 a workgroup and 64 of heads of 128: codes are converted once for all of them.
 // 32 sequences of 8000 keys, 8 key heads of 128, us, 32 / 48 / 64 rows a workgroup: 32 rows 128 / 153 / 181, 48 226 / 156 / 183, 64 229 / 277 / 188;
 // of 64: 48 rows 114 / 85 / 135, 64 105 / 131 / 125; one sequence of 2000 keys, 48 rows 13.4 / 15.7 / 17.7.
 // Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
 // (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
 // heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.
-// Of drafted tokens 16 rows a workgroup where every such tile has a CU and they have no more than four turns each: us, two tiles a workgroup / one, 64 / 8 heads of
-// 128: 6 tokens over 300 keys 10.8 / 8.4, 1000 14.2 / 11.6, 4000 16.1 / 13.6, 16000 21.6 / 22.2; 4 x 8 over 1000 17.5 / 15.7, over 4000 22.8 / 24.0; 16 x 3 over
-// 1000 20.1 / 13.9; 16 x 6 over 300, 384 tiles, 11.2 / 15.0; of 64, 6 over 300 7.5 / 5.9.  And parts are down to one turn
+// Of drafted tokens 16 rows a workgroup where every such tile has a CU and they have no more than four turns of 256 keys a CU (eight of heads of 64):
+// us, two tiles a workgroup / one, 64 / 8 heads of 128: 6 tokens over 300 keys 10.8 / 8.4, 1000 14.2 / 11.6, 4000 16.1 / 13.6, 16000 21.6 / 22.2; 4 x 8
+// over 1000 17.5 / 15.7, over 4000 22.8 / 24.0; 16 x 3 over 1000 20.1 / 13.9; 16 x 6 over 300, 384 tiles, 11.2 / 15.0; of 64, 6 over 300 7.5 / 5.9,
+// 8 x 8 over 2000 15.5 / 12.2, 4000 21.7 / 20.7, 32 over 6000 17.9 / 19.9.  And parts are down to one turn
 // of eight waves, as many as one workgroup a CU leaves; whole up to 1024 keys of heads of 64, 768 of 128, 512 of 256.
 // us, whole / parts of 256, 512 keys, 64 / 8 heads of 128: 1 token over 600, 1000, 2000 keys 9.6 / 10.5, 12.2 / 10.7, 17.6 / 10.7; 4 x 6 tokens over 1000, 2000
 // 15.8 / 16.3, 21.4 / 26.8 / 17.9 (two groups of rows: 512 workgroups); 6 over 5000 39 / 25.4 / 16.8; of 64, 4 x 6 over 1000 10.9 / 13.1; 16 / 2 of 256, 2 over 600
@@ -155,13 +161,17 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     const long items = (long)c->sequences * c->kv_heads;
     const long room = PART_ROOM / ((long)tokens * heads * (dim * 4 + 8));  // parts
     const bool busy = items * keys * dim > 65536 * cus;
-    const bool fewer = busy || (tree && dim == 128 && items * keys * dim > 32768 * cus);
-    p.kernel = rows <= (!fewer ? 96 : dim == 256 ? 32 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
+    p.kernel = rows <= (!busy ? 96 : dim == 256 ? 32 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
+    if (tree) {
+        const long groups = items * (dim == 256 ? (rows + 15) / 16 : (rows + 31) / 32);
+        const bool fits = groups <= (dim == 128 ? 1 : 2) * cus && groups * ((keys + 255) / 256) <= (dim == 64 ? 32 : 16) * cus;
+        p.kernel = rows <= (dim == 256 ? 32 : 64) || (fits && max_tokens <= 32 * FEW_TREE_WORDS) ? AttentionPlan::FEW : AttentionPlan::MANY;
+    }
     if (p.kernel == AttentionPlan::FEW) {
         p.row_tiles = rows <= 16 || dim == 256 ? 1 : rows <= 32 || !busy ? 2 : rows <= 48 ? 3 : dim == 128 ? 4 : 2;
         if (tree) {
             const long alone = items * ((rows + 15) / 16);
-            if (alone <= cus && alone * ((keys + 255) / 256) <= 4 * cus)
+            if (alone <= cus && alone * ((keys + 255) / 256) <= (dim == 64 ? 8 : 4) * cus)
                 p.row_tiles = 1;
         }
         const long step = 32 * few_waves(dim, p.row_tiles, tree);  // the keys that a workgroup's waves have at a time

@@ -57,6 +57,8 @@ constexpr int few_waves(int head_dim, int row_tiles, bool tree = false)
 {
     return (head_dim <= 128 && row_tiles == 1) || (tree && (row_tiles == 2 || head_dim != 128)) ? 8 : 4;
 }
+// Few rows hold the bits of 96 drafted tokens a sequence at most: with eight words the kernels of heads of 256 do not fit the registers.
+constexpr int FEW_TREE_WORDS = 3;
 constexpr bool few_queries_in_lds(int head_dim, int row_tiles, bool tree) { return tree && ((head_dim == 64 && row_tiles == 2) || head_dim == 256); }
 int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_many(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);

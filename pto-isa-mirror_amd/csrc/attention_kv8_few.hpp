@@ -28,7 +28,6 @@ struct FewTile {
 };
 
 // TREE: of drafted tokens.  Keys of the step itself are few: their tiles alone look at a row's bits, which every wave has in LDS for itself.
-constexpr int FEW_TREE_WORDS = 3;  // 96 rows' tokens
 template <typename T, int CODE, int D, int NT, int WAVES, bool TREE>
 __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(AttentionArgs a)
 {

@@ -56,6 +56,15 @@ def test_rows_of_every_count(pa, code, tokens, group):  # noqa: F811
 
 
 @pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("tokens", [63, 95, 96, 97, 129])
+@pytest.mark.parametrize("group", [1, 3, 8])
+def test_many_rows_over_short_caches(pa, code, dim, tokens, group):  # noqa: F811
+    run(pa, code, [1300], [tokens], 2 * group, 2, dim, 64, strided=True)
+    run(pa, code, [300, 0, 33], [tokens, tokens // 3, 1], 2 * group, 2, dim, 16, dtype=torch.float16, width=3)
+
+
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
 @pytest.mark.parametrize("dim", [16, 48, 96, 112, 192, 240])
 def test_heads_of_other_sizes(pa, code, dim):  # noqa: F811
     run(pa, code, [1, 300, 0, 2077], [5, 1, 9, 12], 8, 2, dim, 16, token_major=True)

@@ -458,7 +458,7 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
  * ptoamd_draft_tree makes the rows from parents: a token sees itself and its ancestors.
  *   parents : [tokens] int32, the place of a token's parent among its sequence's drafted ones, or -1: the last token that is older.  A parent that
  *             is neither -1 nor before the token leaves the token's row empty (and its descendants see nothing beyond the token).
- *   tree    : [tokens][tree_words].  Rows that no sequence has are not written.
+ *   tree    : [tokens][tree_words], apart from parents and cu_tokens.  Rows that no sequence has are not written.
  *   cu_tokens, max_tokens : as for the append below; NULL: tokens = sequences * max_tokens
  */
 #define PTOAMD_MOST_DRAFTED 256
@@ -500,7 +500,7 @@ int ptoamd_attention_kv8_tree(void* out, float* lse, const ptoamd_kv8_cache* cac
  * Keeps a path of the drafted tokens: they move together behind the older ones, in the codes that they have.
  *   kept        : [sequences][max_kept] int32: drafted tokens in ascending order.  A list ends at the first entry that is not above the one before, or
  *                 is none of 0 .. n - 1 (so -1 fills it up); r entries are kept
- *   new_lengths : [sequences] int32, gets lengths[s] - n + r.  Must not be lengths.
+ *   new_lengths : [sequences] int32, gets lengths[s] - n + r.  Apart from lengths, kept and cu_tokens.
  *   cu_tokens   : as for the append: n = cu_tokens[s + 1] - cu_tokens[s], at most max_tokens.  NULL: n = max_tokens
  * Token kept[i] moves from place lengths[s] - n + kept[i] to lengths[s] - n + i.  Within a page its codes are copied.  Where tokens come into a page
  * from others, a = max |code| * (scale of their page) of those, the page's scale becomes s1 = max(s0, a * (1 / Q)) as in an append; what was there and

@@ -261,9 +261,11 @@ int ptoamd_kvcache_keep(const ptoamd_kv8_cache* cache, int32_t* new_lengths, con
     PTOAMD_REQUIRE(new_lengths && (kept || max_kept == 0), PTOAMD_E_INVALID, "%s: null operand", what);
     PTOAMD_REQUIRE((reinterpret_cast<uintptr_t>(new_lengths) | reinterpret_cast<uintptr_t>(kept)) % 4 == 0, PTOAMD_E_ALIGNMENT,
                    "%s: kept and new_lengths must be aligned to their elements", what);
-    // (all of a sequence's workgroups read its length)
-    PTOAMD_REQUIRE(new_lengths + cache->sequences <= cache->lengths || cache->lengths + cache->sequences <= new_lengths, PTOAMD_E_INVALID,
-                   "%s: new_lengths must not be lengths", what);
+    // (all of a sequence's workgroups read its length, its list and its place in the batch)
+    auto apart = [&](const int32_t* p, long n) { return p == nullptr || new_lengths + cache->sequences <= p || p + n <= new_lengths; };
+    PTOAMD_REQUIRE(apart(cache->lengths, cache->sequences), PTOAMD_E_INVALID, "%s: new_lengths must not be lengths", what);
+    PTOAMD_REQUIRE(apart(kept, (long)cache->sequences * max_kept) && apart(cu_tokens, cache->sequences + 1L), PTOAMD_E_INVALID,
+                   "%s: new_lengths must not overlap kept or cu_tokens", what);
     a.kept = kept;
     a.new_lengths = new_lengths;
     a.max_kept = max_kept;

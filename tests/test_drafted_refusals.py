@@ -42,7 +42,8 @@ TREE = [(dict(words=0), -1, "words"), (dict(words=5), -1, "words"), (dict(cu=AT,
 
 @pytest.mark.parametrize("change,code,text", TREE + [
     (dict(tree=None), -1, "null"), (dict(parents=None), -1, "null"), (dict(parents=AT + 2), -3, "aligned"), (dict(tokens=-1), -1, "negative"),
-    (dict(sequences=0), -1, "positive"), (dict(most=-1), -1, "negative"), (dict(tokens=3), -1, "sequences * max_tokens")])
+    (dict(sequences=0), -1, "positive"), (dict(most=-1), -1, "negative"), (dict(tokens=3), -1, "sequences * max_tokens"),
+    (dict(parents=AT + 8), -1, "overlap"), (dict(parents=AT - 4), -1, "overlap"), (dict(parents=AT + 64, cu=AT - 8), -1, "overlap")])
 def test_draft_tree(change, code, text):
     rc, error = call("ptoamd_draft_tree", **change)
     assert rc == code and text in error, error
@@ -75,7 +76,8 @@ def test_attention(change, code, text):
 @pytest.mark.parametrize("change,code,text", [c for c in KV8 if not {"tokens", "most"} & set(c[0])] + [
     (dict(new=None), -1, "null"), (dict(kept=None), -1, "null"), (dict(kept=AT + 2), -3, "aligned"), (dict(new=AT + 1026), -3, "aligned"), (dict(most=0), -1, "positive"),
     (dict(max_kept=-1), -1, "negative"), (dict(most=257), -2, "at most 256"), (dict(new=AT), -1, "must not be lengths"), (dict(new=AT + 4), -1, "must not be lengths"),
-    (dict(new=AT - 4), -1, "must not be lengths")])
+    (dict(new=AT - 4), -1, "must not be lengths"), (dict(new=AT + 28, cache_lengths=AT + 1024), -1, "overlap kept"), (dict(kept=AT + 1020), -1, "overlap kept"),
+    (dict(cu=AT + 1016), -1, "overlap kept or cu_tokens")])
 def test_keep(change, code, text):
     rc, error = call("ptoamd_kvcache_keep", **change)
     assert rc == code and text in error, error

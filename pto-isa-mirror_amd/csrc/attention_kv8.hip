@@ -128,6 +128,11 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 // us, whole / parts of 256, 512 keys, 64 / 8 heads of 128: 1 token over 600, 1000, 2000 keys 9.6 / 10.5, 12.2 / 10.7, 17.6 / 10.7; 4 x 6 tokens over 1000, 2000
 // 15.8 / 16.3, 21.4 / 26.8 / 17.9 (two groups of rows: 512 workgroups); 6 over 5000 39 / 25.4 / 16.8; of 64, 4 x 6 over 1000 10.9 / 13.1; 16 / 2 of 256, 2 over 600
 // 14.8 / 14.3.
+// Of drafted tokens, where workgroups are more than CUs they are of the longer sequences first, so that the last to start are short ones; each finds its
+// sequence with the loads that it makes anyway.  us, as sequences come / longer first, E4M3, of any length up to the longest (of which most are short): 40 of
+// 4001 keys and 63 tokens, 16 / 16 heads of 64, 68 / 57 (50 / 38); 64 of 3000 and 8, 32 / 8 of 128, 53 / 44 (42 / 31); 48 of 2000 and 16, 16 / 16, 49 / 45
+// (35 / 32); 200 of 3000 and 4, 32 / 4, 86 / 82 (57 / 46); all of the longest length 42 to 153, the same.  (In parts of 1024 keys and joined, so that the
+// longest is several workgroups': 92, 71, 59 and 124; empty workgroups and the join take more than it gives.)
 // Many rows: in equal stretches (Cuts) where that is less than a tile of rows' keys by more than the second start and the join cost (800 keys of
 // heads of 128, 1600 of 64, 400 of 256); several sequences, whose lengths the host does not know, count as half of the longest.  us, whole / cut, 32 / 8 heads of 128:
 //   128 tokens over 700, 1024, 1500 keys 30 / 35, 38 / 37, 52 / 39; 512 over 700, 1024, 1500, 2500, 16384 30 / 38, 38 / 42, 52 / 47, 78 / 55, 441 / 174;
@@ -142,10 +147,11 @@ constexpr long PART_ROOM = 256L << 20;  // bytes
 struct AttentionPlan {
     enum { GENERIC, FEW, MANY } kernel;
     int splits, chunk, row_tiles, tile_rows;
+    int longest;
 };
 static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int tokens, int max_tokens, int max_length, int window, bool tree)
 {
-    AttentionPlan p{AttentionPlan::GENERIC, 1, 0, 0, 0};
+    AttentionPlan p{AttentionPlan::GENERIC, 1, 0, 0, 0, false};
     const int dim = built_head(c->head_dim);
     if (dim == 0)
         return p;
@@ -183,6 +189,7 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
         if (tree) {
             const long groups = items * ((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
             splits = groups < cus ? cus / groups : 1;
+            p.longest = c->sequences > 1 && groups > cus ? (int)keys : 0;
             splits = splits < turns ? splits : turns;
             if (turns <= (dim == 64 ? 4 : dim == 128 ? 3 : 2))
                 splits = 1;
@@ -314,6 +321,7 @@ static int attention(const char* what, void* out, float* lse, const ptoamd_kv8_c
         a.row_tiles = plan.row_tiles;
         a.tile_rows = plan.tile_rows;
         a.sequences = cache->sequences;
+        a.longest = plan.longest;
         a.cuts = plan.kernel == AttentionPlan::MANY && a.splits > 1 ? static_cast<int*>(workspace) : nullptr;
         a.part_out = reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + (a.cuts != nullptr ? Cuts::BYTES : 0));
         a.part_sum = reinterpret_cast<float2*>(a.part_out + (size_t)plan.splits * tokens * heads * built_head(cache->head_dim));

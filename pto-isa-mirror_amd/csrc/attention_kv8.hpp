@@ -31,6 +31,7 @@ struct AttentionArgs {
     // of drafted tokens, in place of `causal`: rows of tree_words 32-bit words (seen_keys)
     const uint32_t* tree;
     int tree_words;
+    int longest;  // few rows: 0, or sequences are taken in the order of span_in_turn
 };
 
 // Many rows, keys in parts: all (key head, tile of rows, tile of keys) that there are, in this order, in equal stretches, one for a workgroup a CU.
@@ -114,6 +115,41 @@ __device__ __forceinline__ Span span_of(const AttentionArgs& a, int seq)
     }
     s.length = min(max(load_uniform(c.lengths + seq), 0), c.max_pages << c.page_shift);
     s.begin = first_key(s.length - s.count, a.window) & ~31;
+    return s;
+}
+// That of the nth sequence in the order of their lengths, the longer first: by steps of half an octave below `longest`, those of a step in their order, the
+// shortest last.  A wave looks at up to 64 sequences, a lane at one; of more every second, third, ... is in one order, and the orders take turns.
+__device__ __forceinline__ Span span_in_turn(const AttentionArgs& a, int nth, int* nth_seq)
+{
+    const Kv8& c = a.cache;
+    const int orders = (a.sequences + 63) / 64, order = nth % orders, lane = threadIdx.x % 64, seq = order + lane * orders;
+    const bool there = seq < a.sequences;
+    const int at = there ? seq : 0, length = min(max(c.lengths[at], 0), c.max_pages << c.page_shift);
+    int first = at * c.max_tokens, count = c.max_tokens;
+    if (c.cu_tokens != nullptr) {
+        const int from = c.cu_tokens[at], to = c.cu_tokens[at + 1];
+        first = min(max(from, 0), c.tokens);
+        count = min(max(to, first) - first, min(c.max_tokens, c.tokens - first));
+    }
+    const int step = max((int)(f2u((float)a.longest) - f2u((float)max(length, 1))) >> 22, 0);
+    constexpr int STEPS = 8;  // (the last has all that are shorter)
+    nth /= orders;
+    uint64_t its = 0;
+    for (int i = 0; i <= STEPS; ++i) {
+        its = __ballot(there && (i < STEPS ? step == i : step >= STEPS));
+        const int n = __popcll(its);
+        if (nth < n)
+            break;
+        nth -= n;
+    }
+    const int before = __builtin_amdgcn_mbcnt_hi((uint32_t)(its >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)its, 0));
+    const int found = __builtin_ctzll(__ballot((its >> lane & 1) != 0 && before == nth));
+    Span s;
+    s.first = __builtin_amdgcn_readlane(first, found);
+    s.count = __builtin_amdgcn_readlane(count, found);
+    s.length = __builtin_amdgcn_readlane(length, found);
+    s.begin = first_key(s.length - s.count, a.window) & ~31;
+    *nth_seq = order + found * orders;
     return s;
 }
 // Whether a sequence's keys are in several parts, which are joined; else its workgroups write what the call returns.

@@ -42,8 +42,9 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
     const Kv8& c = a.cache;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 16, g = lane / 16;
     // (workgroups go to the XCDs in turn: parts, of which short sequences leave most empty, are the slowest index)
-    const int kv_head = blockIdx.x % c.kv_heads, row0 = blockIdx.x / c.kv_heads * 16 * NT, seq = blockIdx.y, part = blockIdx.z;
-    const Span span = span_of(a, seq);
+    const int kv_head = blockIdx.x % c.kv_heads, row0 = blockIdx.x / c.kv_heads * 16 * NT, part = blockIdx.z;
+    int seq = blockIdx.y;
+    const Span span = TREE && a.longest > 0 ? span_in_turn(a, blockIdx.y, &seq) : span_of(a, blockIdx.y);
     const int rows = span.count * a.group;
     const int begin = a.splits > 1 ? span.begin + part * a.chunk : span.begin;
     const int end = part + 1 < a.splits ? min(span.length, begin + a.chunk) : span.length;  // (the last takes what a wrong max_length left out)

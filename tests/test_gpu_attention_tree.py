@@ -113,6 +113,23 @@ def test_sequences_of_very_different_lengths(pa, code, dim, kw):  # noqa: F811
     run(pa, code, [20, 12011], [20, 70], 8, 2, dim, 16, dtype=torch.float16, **kw)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("sequences", [33, 64, 65, 130, 200])
+def test_batches_of_more_workgroups_than_compute_units(pa, dim, sequences):  # noqa: F811
+    rng = random.Random(sequences + dim)
+    counts = [rng.choice([0, 1, 2, 4, 4]) for _ in range(sequences)]
+    olds = [rng.choice([0, 0, 1, 17, 33, 90, 255, 256, 400, 700, 1040]) for _ in counts]
+    counts[sequences // 2], olds[0], counts[0] = 4, 0, 0  # (and a sequence of no tokens at all)
+    run(pa, "e4m3", olds, counts, 16, 8, dim, 16)
+    assert pa.last_kernel() == "attention_kv8_few"
+    # as many tokens each, without cu_tokens
+    cache = ref.Cache("i8", [3 + o // 4 for o in olds], 8, dim, 16, 3)
+    ways = dr.ways_of(dr.parents_of([3] * sequences, 4))
+    q = queries(3 * sequences, 16, dim, torch.bfloat16, 5, False)
+    out, lse = pa.attention_kv8_tree(q, *cache.operands(pa), dr.rows_of(ways, 1), want_lse=True)
+    ref.check_attention(out, dr.attention(q, cache, ways), lse)
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256, 72])
 @pytest.mark.parametrize("counts", [[3, 1, 4], [40, 5, 64], [200, 3, 70], [256, 100, 1]])
 def test_any_bits(pa, dim, counts):  # noqa: F811

@@ -58,8 +58,6 @@ constexpr int few_waves(int head_dim, int row_tiles, bool tree = false)
 {
     return (head_dim <= 128 && row_tiles == 1) || (tree && (row_tiles == 2 || head_dim != 128)) ? 8 : 4;
 }
-// Few rows hold the bits of 96 drafted tokens a sequence at most: with eight words the kernels of heads of 256 do not fit the registers.
-constexpr int FEW_TREE_WORDS = 3;
 constexpr bool few_queries_in_lds(int head_dim, int row_tiles, bool tree) { return tree && ((head_dim == 64 && row_tiles == 2) || head_dim == 256); }
 int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
 int launch_attention_many(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);
@@ -184,18 +182,16 @@ __device__ __forceinline__ uint32_t drafted_word(const AttentionArgs& a, const S
     return word < a.tree_words ? a.tree[(int64_t)(s.first + token) * a.tree_words + word] & bits_below(s.count - 32 * word) : 0u;
 }
 // The first of the older keys that a token sees, whose `words` words lie in LDS.  (No row: none of them.)
-template <int WORDS>
-__device__ __forceinline__ int first_of_drafted(const AttentionArgs& a, const Span& s, const uint32_t* row, bool valid, int token)
+__device__ __forceinline__ int first_of_drafted(const AttentionArgs& a, const Span& s, const uint32_t* row, int words, bool valid, int token)
 {
     if (!valid)
         return 0x7FFFFFFF;
-    return a.window > 0 ? first_key(s.length - s.count + others_seen(row, WORDS, s.count, token), a.window) : 0;
+    return a.window > 0 ? first_key(s.length - s.count + others_seen(row, words, s.count, token), a.window) : 0;
 }
 // Which of the keys key .. key + 31 a token sees (seen_keys: `key` is the same for all lanes, and words behind the last token are 0).
-template <int WORDS>
-__device__ __forceinline__ uint32_t drafted_keys(const uint32_t* row, int key, int first, int old)
+__device__ __forceinline__ uint32_t drafted_keys(const uint32_t* row, int words, int key, int first, int old)
 {
-    return (bits_below(old - key) & ~bits_below(first - key)) | row_bits(row, WORDS, key - old);
+    return (bits_below(old - key) & ~bits_below(first - key)) | row_bits(row, words, key - old);
 }
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

@@ -29,16 +29,17 @@ struct FewTile {
 
 // TREE: of drafted tokens.  Keys of the step itself are few: their tiles alone look at a row's bits, which every wave has in LDS for itself.
 template <typename T, int CODE, int D, int NT, int WAVES, bool TREE>
-__global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(AttentionArgs a)
+__global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(TREE && D == 64 && NT <= 2 ? 4 : WAVES / 4))) attention_kv8_few_kernel(AttentionArgs a)
 {
     constexpr int STEPS = D / 32, VW = D / 64, MT = D / 16, PITCH = D + 4;
     constexpr int RING = 2;  // tiles of a wave in registers
     constexpr int STRIDE = 32 * WAVES;
+    constexpr int TREE_WORDS = PTOAMD_MOST_DRAFTED / 32;
     constexpr bool Q_IN_LDS = few_queries_in_lds(D, NT, TREE);
     extern __shared__ __attribute__((aligned(16))) float shared[];  // [WAVES / 2][16 NT][PITCH]
     __shared__ float wave_top[WAVES][16 * NT], wave_sum[WAVES][16 * NT];
     __shared__ uint4 queries[Q_IN_LDS ? NT * STEPS : 1][Q_IN_LDS ? 64 : 1];
-    __shared__ uint32_t drafted[TREE ? WAVES : 1][TREE ? 16 * NT : 1][FEW_TREE_WORDS + 1];  // (last: the first of the older keys that the row sees)
+    __shared__ uint32_t drafted[TREE ? WAVES : 1][TREE ? 16 * NT : 1][TREE_WORDS + 1];  // (last: the first of the older keys that the row sees)
     const Kv8& c = a.cache;
     const int lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64), col = lane % 16, g = lane / 16;
     // (workgroups go to the XCDs in turn: parts, of which short sequences leave most empty, are the slowest index)
@@ -75,7 +76,10 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
             const __amdgpu_buffer_rsrc_t vr = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(v_head + ((uint64_t)page * v_page * 8 + slot * (uint32_t)c.v.token)), 0, bytes, 0x20000);
 #pragma unroll
             for (int cc = 0; cc < D / 64; ++cc)
-                tile.k[h][cc] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane[cc], 0, 0));
+                if (TREE && D == 256 && cc == 1)  // (a register less: such heads have more than 128 elements)
+                    tile.k[h][cc] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane[0], 64, 0));
+                else
+                    tile.k[h][cc] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(kr, k_lane[cc], 0, 0));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = i * (int)c.v.token;
@@ -90,7 +94,13 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
                 }
             }
         }
-        tile.scale = scales[(uint32_t)(page_lane * c.kv_heads + kv_head)];
+        if constexpr (TREE && D == 256) {
+            int again = lane;
+            asm("" : "+v"(again));  // (or the address is kept in two registers)
+            tile.scale = (again & 2 ? c.v.scales : c.k.scales)[(uint32_t)(page_lane * c.kv_heads + kv_head)];
+        } else {
+            tile.scale = scales[(uint32_t)(page_lane * c.kv_heads + kv_head)];
+        }
         tile.unknown = known ? 0.0f : NAN;  // (added where the scale is used: here it would be waited for)
         __builtin_amdgcn_sched_barrier(0);  // (the order of the loads is what the waits count on)
     };
@@ -100,11 +110,11 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
     for (int s = 0; s < RING; ++s)
         ids[s] = find(first + s * STRIDE);
 
+    const int tree_words = a.tree_words;  // (at most TREE_WORDS)
     if constexpr (TREE) {
-#pragma unroll
-        for (int i = lane; i < 16 * NT * FEW_TREE_WORDS; i += 64) {
-            const int row = row0 + i / FEW_TREE_WORDS;
-            drafted[wave][i / FEW_TREE_WORDS][i % FEW_TREE_WORDS] = row < rows ? drafted_word(a, span, row / a.group, i % FEW_TREE_WORDS) : 0u;
+        for (int i = lane; i < 16 * NT * tree_words; i += 64) {
+            const int row = row0 + i % (16 * NT), word = i / (16 * NT);
+            drafted[wave][i % (16 * NT)][word] = row < rows ? drafted_word(a, span, row / a.group, word) : 0u;
         }
     }
 
@@ -116,7 +126,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
         const int row = row0 + 16 * t + col, token = row / a.group;
         const bool valid = row < rows;
         if constexpr (TREE)
-            drafted[wave][16 * t + col][FEW_TREE_WORDS] = first_of_drafted<FEW_TREE_WORDS>(a, span, drafted[wave][16 * t + col], valid, token);
+            drafted[wave][16 * t + col][TREE_WORDS] = first_of_drafted(a, span, drafted[wave][16 * t + col], tree_words, valid, token);
         else
             seen[t] = valid ? visible_keys(a, span.length - span.count + token, span.length) : make_int2(0, 0);
         const uint8_t* p = a.q + (int64_t)(span.first + (valid ? token : 0)) * a.q_token + (int64_t)(kv_head * a.group + (valid ? row - token * a.group : 0)) * a.q_head;
@@ -221,7 +231,7 @@ __global__ void __launch_bounds__(64 * WAVES) attention_kv8_few_kernel(Attention
             }
             if (TREE && !whole) {
                 const uint32_t* row = drafted[wave][16 * t + col];
-                const uint32_t mine = drafted_keys<FEW_TREE_WORDS>(row, key, (int)row[FEW_TREE_WORDS], every_to) >> (4 * g);
+                const uint32_t mine = drafted_keys(row, tree_words, key, (int)row[TREE_WORDS], every_to) >> (4 * g);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     w[j / 4][j % 4] = (mine & 1u << (16 * (j / 4) + j % 4)) != 0 ? w[j / 4][j % 4] : -INFINITY;

@@ -57,7 +57,7 @@ def test_rows_of_every_count(pa, code, tokens, group):  # noqa: F811
 
 @pytest.mark.parametrize("code", ["i8", "e4m3"])
 @pytest.mark.parametrize("dim", [64, 128, 256])
-@pytest.mark.parametrize("tokens", [63, 95, 96, 97, 129])
+@pytest.mark.parametrize("tokens", [63, 95, 96, 97, 129, 256])
 @pytest.mark.parametrize("group", [1, 3, 8])
 def test_many_rows_over_short_caches(pa, code, dim, tokens, group):  # noqa: F811
     run(pa, code, [1300], [tokens], 2 * group, 2, dim, 64, strided=True)

@@ -110,8 +110,8 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
     constexpr int GROUP = HALVES ? WAVES / 2 : WAVES;  // the waves that share a tile of keys
     constexpr int THREADS = 64 * GROUP, KEYS = Tile::KEYS, STRIDE = HALVES ? 2 * KEYS : KEYS, STEPS = D / 16, DT = D / 32;
     constexpr int SIDE_UNITS = KEYS * D / 16, UNITS = 2 * SIDE_UNITS / THREADS;  // 16 codes each; a thread's
-    extern __shared__ __attribute__((aligned(16))) uint8_t all_tiles[];               // two of keys, two of values (HALVES: of each)
-    __shared__ float4 all_scales[HALVES ? 2 : 1][2][KEYS / 16];                                                 // of 16 keys: key scale, value scale's log2 and inverse
+    extern __shared__ __attribute__((aligned(16))) uint8_t all_tiles[];  // two of keys, two of values (HALVES: of each)
+    __shared__ float4 all_scales[HALVES ? 2 : 1][2][KEYS / 16];  // of 16 keys: key scale, value scale's log2 and inverse
     __shared__ int cuts[Cuts::SIZE];
     __shared__ uint32_t drafted[TREE ? ROWS : 1][MANY_TREE_WORDS + 1];  // (rows a bank apart)
     // A workgroup has one tile of rows and all their keys, or a stretch of what there is (Cuts): the end of a tile's keys, whole ones, the start of
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         float2 raw_scale = make_float2(0, 0);
         float unit_scale[UNITS];  // of values: the scale of their page
         uint32_t no_page = 0;     // bit u: the table names no page for unit u (asked of E4M3 codes, which may be NaN; no int8 code is)
-        uint32_t source[UNITS], target[UNITS][2], none = 0;
+        uint32_t source[UNITS], none = 0;
         asm("" : "+v"(none));  // (a vector register's zero: a scale that is not read through the scalar cache, for which a barrier would wait)
         static_assert(SIDE_UNITS % THREADS == 0 || THREADS == 2 * SIDE_UNITS, "a unit is keys or values for all waves, or for half of them");
         auto is_value = [&](int u) { return SIDE_UNITS < THREADS ? wave >= GROUP / 2 : u * THREADS >= SIDE_UNITS; };
@@ -247,11 +247,13 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         auto unit_key = [&](int u, int stage) { return own_begin + (stage - (is_value(u) ? 1 : 0)) * STRIDE + u * THREADS % SIDE_UNITS / (D / 16) + wave_key; };
 #pragma unroll
         for (int u = 0; u < UNITS; ++u) {
-            const int k = (tid + u * THREADS) % SIDE_UNITS / (D / 16), chunk = lane % (D / 16) * 2;
             source[u] = (uint32_t)(lane / (D / 16)) * (uint32_t)(is_value(u) ? c.v.token : c.k.token) + (lane % (D / 16) * 16 < c.head_dim ? lane % (D / 16) * 16 : 0);
-            target[u][0] = is_value(u) ? Tile::value_at(k, chunk / 2) : Tile::key_at(k, chunk);
-            target[u][1] = is_value(u) ? Tile::value_at(k, chunk / 2) + 16 : Tile::key_at(k, chunk + 1);
         }
+        // Where a unit's two halves go in a tile: of keys or values, its first unit's places (a side's units are multiples of 16 keys apart), the second half
+        // 16 bytes from the first in either direction.
+        static_assert(SIDE_UNITS <= THREADS || THREADS / (D / 16) % 16 == 0, "a unit's permutation is its side's");
+        const int own_key = tid % SIDE_UNITS / (D / 16), own_chunk = lane % (D / 16) * 2;
+        const int key_target = Tile::key_at(own_key, own_chunk), value_target = Tile::value_at(own_key, own_chunk / 2);
         auto find = [&](int stage) {
 #pragma unroll
             for (int u = 0; u < UNITS; ++u)
@@ -269,7 +271,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         };
         // the seven pieces of a unit's way from codes to LDS, and the eighth that reads the next one
         constexpr int PIECES = 8;
-        uint32_t staged[8];
+        uint32_t staged[4];
         auto piece = [&](auto u_, auto piece_, int stage) __attribute__((always_inline)) {
             constexpr int u = decltype(u_)::value, which = decltype(piece_)::value;
             if constexpr (which == 0) {
@@ -281,14 +283,14 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
                     raw[u].z = seen_by_some ? raw[u].z : 0u;
                     raw[u].w = seen_by_some ? raw[u].w : 0u;
                 }
-            } else if constexpr (which < 5) {
-                const uint32_t x = kv8_turn<CODE>(which == 1 ? raw[u].x : which == 2 ? raw[u].y : which == 3 ? raw[u].z : raw[u].w);
-                staged[2 * which - 2] = is_value(u) ? kv8_pair_to_f16<CODE, false>(x) : kv8_key_pair<CODE, false>(x);
-                staged[2 * which - 1] = is_value(u) ? kv8_pair_to_f16<CODE, true>(x) : kv8_key_pair<CODE, true>(x);
+            } else if constexpr (which < 7 && which % 3 != 0) {
+                const uint32_t x = kv8_turn<CODE>(which == 1 ? raw[u].x : which == 2 ? raw[u].y : which == 4 ? raw[u].z : raw[u].w);
+                staged[which % 3 * 2 - 2] = is_value(u) ? kv8_pair_to_f16<CODE, false>(x) : kv8_key_pair<CODE, false>(x);
+                staged[which % 3 * 2 - 1] = is_value(u) ? kv8_pair_to_f16<CODE, true>(x) : kv8_key_pair<CODE, true>(x);
             } else if constexpr (which < 7) {
                 uint8_t* to_tile = tiles + (is_value(u) ? 2 + ((stage - 1) & 1) : stage & 1) * Tile::BYTES;
-                *reinterpret_cast<uint4*>(to_tile + target[u][which - 5]) =
-                    make_uint4(staged[4 * (which - 5)], staged[4 * (which - 5) + 1], staged[4 * (which - 5) + 2], staged[4 * (which - 5) + 3]);
+                const int target = ((is_value(u) ? value_target : key_target) ^ (which == 3 ? 0 : 16)) + u * THREADS % SIDE_UNITS / (D / 16) * 2 * D;
+                *reinterpret_cast<uint4*>(to_tile + target) = make_uint4(staged[0], staged[1], staged[2], staged[3]);
             } else {
                 fetch(u, stage + 1);
             }
@@ -323,7 +325,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
         // The matrix part of turn `tile`: the sums of the tile before, the scores of this one.  A SIMD has 32 clocks for a product that a wave issues in
         // four: in between go the reads of the fragment AHEAD products on, and a piece of the staging.  (The order is fixed by barriers for the
         // compiler, which would by itself read each fragment right before it is used.)
-        constexpr int PV = KEYS / 16 * DT, QK = KEYS / 32 * STEPS, AHEAD = HALVES ? 2 : 4;
+        constexpr int PV = KEYS / 16 * DT, QK = KEYS / 32 * STEPS, AHEAD = 4;
         static_assert(D != 256 || QK >= 8, "score products between the sums' products and scaled_accumulator");
         auto multiply = [&](int tile) __attribute__((always_inline)) {
             const uint8_t* values = tiles + (2 + ((tile - 1) & 1)) * Tile::BYTES;

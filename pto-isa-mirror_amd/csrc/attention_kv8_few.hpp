@@ -27,7 +27,10 @@ struct FewTile {
     float unknown;  // NaN where the table names no page
 };
 
-// TREE: of drafted tokens.  Keys of the step itself are few: their tiles alone look at a row's bits, which every wave has in LDS for itself.
+// TREE: of drafted tokens.  Keys of the step itself are few: their tiles alone look at a row's bits, which every wave has in LDS for itself.  Eight waves a
+// workgroup but for three and four tiles of rows of heads of 128 (few_waves): rows are many more than in decode, and twice the waves halve the turns.
+// Bound: a wave's instructions and, of short sequences, the chain length -> page -> codes.  7 tokens over 300 keys, 32 / 8 heads of 128, int8, 8.4 us; 8 of 24 over 1000,
+// 64 / 8 heads, E4M3, 31; 40 of up to 63 over up to 3503 (665 on average), 16 / 16 of 64, 32: the longest sequence's 14 turns of two workgroups a CU.
 template <typename T, int CODE, int D, int NT, int WAVES, bool TREE>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(TREE && D == 64 && NT <= 2 ? 4 : WAVES / 4))) attention_kv8_few_kernel(AttentionArgs a)
 {

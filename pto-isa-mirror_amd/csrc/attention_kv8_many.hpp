@@ -101,6 +101,8 @@ __device__ __forceinline__ float scaled_accumulator(float x, float by)
 // TREE: of drafted tokens, whose rows of bits lie in LDS for the tiles of the step's own keys.
 // HALVES: half as many rows a workgroup, 128, and two tiles of keys at a time: the waves of a SIMD have the same rows, one those of every second tile, and
 // add up at the end.  So rows up to 128 leave no wave without work; each half stages its tiles alone, twice a wave's share.
+// Bound: as above, and the staging.  16 sequences of 16 tokens over 8192 keys, 64 / 8 heads of 128, E4M3, 104 us (112 where no cache holds them): the matrix unit is
+// busy for 28 % of the clocks, the vector unit for 38 %; with all pages in the L2 95.  Fragments read four products ahead instead of two changed nothing.
 constexpr int MANY_TREE_WORDS = PTOAMD_MOST_DRAFTED / 32;
 template <typename T, int CODE, int D, int WAVES, bool TREE, bool HALVES>
 __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu(WAVES / 4, WAVES / 4))) attention_kv8_many_kernel(AttentionArgs args)

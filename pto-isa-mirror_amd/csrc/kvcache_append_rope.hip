@@ -147,6 +147,9 @@ __device__ __forceinline__ void turn_queries(const AppendRopeArgs& a, unsigned g
 // Some workgroups append, one a page of a sequence, head and side (keys or values): the append of kvcache.hip, with keys turned as they are read.  The
 // others turn queries; the two kinds stand among each other in the grid, since a page's chain of loads leaves the memory to the queries.
 // Products and sums in f32; a key is rounded once, to its code.
+// Bound: HBM where there are many tokens (6 ragged prompts of up to 2048, 32 / 8 heads of 128, bf16 to E4M3: 235 MB in 48 us, 4.9 TB/s), else the chain
+// lengths -> values, page, table row -> largest -> codes: 16 tokens 5.9 us, 16 sequences of 24 with a tree 7.2.  The prompts again and again on the same tensors: 42 us,
+// as two calls 53; on the way there, a unit a thread and keys read twice, 59.
 template <typename T, int CODE, int VEC, bool INTERLEAVED, int THREADS>
 __global__ void __launch_bounds__(THREADS) kvcache_append_rope_kernel(AppendRopeArgs a)
 {

@@ -106,17 +106,19 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 //          8000: 48 130 / 114, 64 168 / 115; 8 of 6000: 40 45 / 42, 64 59 / 45; one of 60000 40 57 / 52.
 //   many : more rows, 256 of them a workgroup (128 for heads of 256 elements)
 // Of drafted tokens, 128 rows a workgroup (HALVES) where there are no more: us, 256 rows a workgroup / 128, 16 sequences of 8192 keys, 64 / 8 heads of 128
-// E4M3, 16 tokens 147 / 105, one of 131072 150 / 110; of 64, 119 / 77; and 32 tokens, 256 rows, 179 / 180, 48 271 / 281, 64 291 / 334.  The
-// few-rows kernel takes up to 64 rows (32 of heads of 256), and more where its workgroups of 32 rows (16) are few: 2 a CU of heads of 128, 3 of 64, 2.5 of
-// 256, or 1, 2, 2 of up to two turns of 256 keys; and have 16 turns a CU or fewer, 32, 18.  us, few / many, E4M3, rows a key head x sequences x keys, 64 / 8
-// heads of 128: 512 x 1 x 300, 1000, 3000, 6000, 16000 9 / 21, 14 / 37, 24 / 42, 32 / 45, 72 / 65; 1024 x 1 x 3000 30 / 45; 256 x 1 x 16000 41 / 49, 60000
-// 137 / 90; 128 x 16 x 300, 1000, 2000 22 / 18, 33 / 30, 45 / 49; 256 x 8 x 300, 1000, 2000 22 / 21, 32 / 42, 45 / 52; 384 x 8 47 / 41, 65 / 66 of 1000, 2000; 80 x
-// 16 x 8192 163 / 100; a quarter to all of 192 x 8 x up to 1000, 2000 21 / 28, 25 / 34; of 64: 512 x 4 x 300, 1000, 3000 12 / 17, 18 / 34, 31 / 46; 384 x 8 x 300,
-// 1000, 2000 16 / 18, 23 / 34, 33 / 58; 128 x 32 x 300, 1000 19 / 14, 31 / 24; 768 x 2 x 8000 58 / 73; 1464 x 7 x 528, 16 / 2 heads, 19 / 26; 512 x 1 x 60000 133 / 115; 16 / 2 of 256: 512 x 4 x 1000
-// 21 / 44; 512 x 8 x 300, 1000, 2000 25 / 30, 39 / 52, 58 / 64; 384 x 16 37 / 30, 57 / 59, 85 / 77; 512 x 1 x 16000 53 / 61, 768 95 / 72; 128 x 16 x 4000 49 / 62.
-// Few rows are 16, 32, or, where the keys are that many, up to 48 a workgroup and 64 of heads of 128: codes are converted once for all of them.
-// 32 sequences of 8000 keys, 8 key heads of 128, us, 32 / 48 / 64 rows a workgroup: 32 rows 128 / 153 / 181, 48 226 / 156 / 183, 64 229 / 277 / 188;
-// of 64: 48 rows 114 / 85 / 135, 64 105 / 131 / 125; one sequence of 2000 keys, 48 rows 13.4 / 15.7 / 17.7.  (More than 64: 6 sequences of 7301, 154 rows of drafted tokens, 8 / 4 heads of 128, 32 / 48 / 64 rows 39 / 62 / 57.)
+// E4M3, 16 tokens 147 / 105, one of 131072 150 / 110; of 64, 119 / 77; and 32 tokens, 256 rows, 179 / 180, 48 271 / 281, 64 291 / 334.  The few-rows
+// kernel takes up to 64 rows (32 of heads of 256), and more where its workgroups of 32 rows (16) are few: 2 a CU of heads of 128, 3 of 64, 2.5 of 256, or
+// 1, 2, 2 of up to two turns of 256 keys; and have 16 turns a CU or fewer, 32, 18.  us, few / many, E4M3, rows a key head x sequences x keys, 64 / 8 heads
+// of 128: 512 x 1 x 300, 1000, 3000, 6000, 16000 9 / 21, 14 / 37, 24 / 42, 32 / 45, 72 / 65; 1024 x 1 x 3000 30 / 45; 256 x 1 x 16000 41 / 49, 60000 137 /
+// 90; 128 x 16 x 300, 1000, 2000 22 / 18, 33 / 30, 45 / 49; 256 x 8 x 300, 1000, 2000 22 / 21, 32 / 42, 45 / 52; 384 x 8 47 / 41, 65 / 66 of 1000, 2000;
+// 80 x 16 x 8192 163 / 100; a quarter to all of 192 x 8 x up to 1000, 2000 21 / 28, 25 / 34; of 64: 512 x 4 x 300, 1000, 3000 12 / 17, 18 / 34, 31 / 46;
+// 384 x 8 x 300, 1000, 2000 16 / 18, 23 / 34, 33 / 58; 128 x 32 x 300, 1000 19 / 14, 31 / 24; 768 x 2 x 8000 58 / 73; 1464 x 7 x 528, 16 / 2 heads, 19 /
+// 26; 512 x 1 x 60000 133 / 115; 16 / 2 of 256: 512 x 4 x 1000 21 / 44; 512 x 8 x 300, 1000, 2000 25 / 30, 39 / 52, 58 / 64; 384 x 16 37 / 30, 57 / 59, 85
+// / 77; 512 x 1 x 16000 53 / 61, 768 95 / 72; 128 x 16 x 4000 49 / 62.
+// Few rows are 16, 32, or, where the keys are that many, up to 48 a workgroup and 64 of heads of 128: codes are converted once for all of them. 32
+// sequences of 8000 keys, 8 key heads of 128, us, 32 / 48 / 64 rows a workgroup: 32 rows 128 / 153 / 181, 48 226 / 156 / 183, 64 229 / 277 / 188; of 64:
+// 48 rows 114 / 85 / 135, 64 105 / 131 / 125; one sequence of 2000 keys, 48 rows 13.4 / 15.7 / 17.7.  (More than 64: 6 sequences of 7301, 154 rows of
+// drafted tokens, 8 / 4 heads of 128, 32 / 48 / 64 rows 39 / 62 / 57.)
 // Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
 // (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
 // heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.

@@ -20,7 +20,8 @@ struct AppendRopeArgs {
     int tree_words;                                // of 32 bits
     int table_rows, half, heads, interleaved;
     int blocks;                                    // most pages that a sequence's new tokens touch
-    unsigned wide, pairs;                          // workgroups that the queries of two tokens take; such pairs of a sequence
+    unsigned wide, pairs;                          // workgroups that the queries of two tokens take; such pairs of a sequence, or 0: pairs of the batch's rows
+    int sequences;
     uint64_t share;                                // of the workgroups that append, in 2^-32
 
     // the position that the nth new token of a sequence, row `row` of the operands, is turned by; `start` is its first new token's place
@@ -112,33 +113,79 @@ __device__ __forceinline__ void load_turned(const AppendRopeArgs& a, const T* ro
 
 constexpr int ROPE_TOKENS = 2;
 
-// Queries: a thread has a unit of a head of two consecutive tokens, all loads of both in flight before the first is used, as in rope.hip.
+// The last sequence that starts at a row or before it, or -1: 64 starts at a time.  (Whatever cu_tokens holds, a sequence that there is.)
+__device__ __forceinline__ int sequence_of(const AppendRopeArgs& a, int row)
+{
+    const int lane = threadIdx.x % 64;
+    int seq = 0;
+    for (int step = a.sequences > 4096 ? 4096 : a.sequences > 64 ? 64 : 1; step > 0; step /= 64) {
+        const int at = seq + lane * step, before = __popcll(__ballot(at < a.sequences && a.cache.cu_tokens[min(at, a.sequences)] <= row));
+        if (before == 0)
+            return -1;
+        seq += (before - 1) * step;
+    }
+    return seq;
+}
+
+// Queries: a thread has a unit of a head of two consecutive tokens, all loads of both in flight before the first is used, as in rope.hip.  The two are a sequence's
+// (pairs), or, with cu_tokens, two rows of the batch, whose sequences are looked for: max_tokens may be far above the tokens that there are.  us, pairs of max_tokens of every
+// sequence / of rows, 32 / 8 heads of 128: 64 sequences of 128 tokens, max_tokens 128 35.0 / 34.2, 512 38.9 / 34.5, 2048 79 / 47; 256 of 4, 4 13.1 / 13.2, 64 33 / 21; 64 of
+// 1, 1 5.6 / 5.5, 8 6.3 / 6.7, 64 11.6 / 8.3.
 template <typename T, int VEC, bool INTERLEAVED, int THREADS>
 __device__ __forceinline__ void turn_queries(const AppendRopeArgs& a, unsigned group)
 {
     const Kv8& c = a.cache;
     const unsigned row_group = group / a.wide;
-    const int seq = row_group / a.pairs, nth = (row_group - (unsigned)seq * a.pairs) * ROPE_TOKENS;
-    const int first = c.first_token(seq), count = c.token_count(seq, first);
+    int seq = -1, first = 0, count = 0, start = 0;
+    auto enter = [&](int its) {
+        seq = its;
+        first = c.first_token(seq), count = c.token_count(seq, first);
+        start = max(c.lengths[seq], 0) - count;
+    };
+    int row[ROPE_TOKENS], position[ROPE_TOKENS];  // (row -1: not a sequence's)
+    if (a.pairs > 0) {
+        enter(row_group / a.pairs);
+        const int nth = (row_group - (unsigned)seq * a.pairs) * ROPE_TOKENS;
+        if (nth >= count)
+            return;
+#pragma unroll
+        for (int k = 0; k < ROPE_TOKENS; ++k) {
+            const int token = min(nth + k, count - 1);
+            row[k] = nth + k < count ? first + token : -1;
+            position[k] = a.position(first + token, token, count, start);
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < ROPE_TOKENS; ++k) {
+            const int at = row_group * ROPE_TOKENS + k;
+            if (at < c.tokens && (seq < 0 || at >= first + count)) {
+                const int its = sequence_of(a, at);
+                if (its >= 0)
+                    enter(__builtin_amdgcn_readfirstlane(its));
+            }
+            const bool there = at < c.tokens && seq >= 0 && at >= first && at < first + count;
+            row[k] = there ? at : -1;
+            position[k] = there ? a.position(at, at - first, count, start) : 0;
+        }
+    }
     const int units = (c.head_dim + 2 * VEC - 1) / (2 * VEC);
     const int unit = (group - row_group * a.wide) * THREADS + threadIdx.x, head = unit / units, u = unit - head * units;
-    if (nth >= count || head >= a.heads)
+    static_assert(ROPE_TOKENS == 2, "one of two rows stands in for the other");
+    const int some = max(row[0], row[1]);
+    if (some < 0 || head >= a.heads)
         return;
-    const int start = max(c.lengths[seq], 0) - count;
     const uint8_t* x = a.q + (int64_t)head * a.q_head;
     uint8_t* out = a.q_out + (int64_t)head * a.out_head;
     const Runs at = runs_of<VEC, INTERLEAVED>(u, a.half, c.head_dim);
     float y[ROPE_TOKENS][2 * VEC];
 #pragma unroll
-    for (int k = 0; k < ROPE_TOKENS; ++k) {
-        const int token = min(nth + k, count - 1), row = first + token;
-        load_turned<T, VEC, INTERLEAVED>(a, reinterpret_cast<const T*>(x + (int64_t)row * a.q_token), a.position(row, token, count, start), u, c.head_dim, y[k]);
-    }
+    for (int k = 0; k < ROPE_TOKENS; ++k)
+        load_turned<T, VEC, INTERLEAVED>(a, reinterpret_cast<const T*>(x + (int64_t)(row[k] < 0 ? some : row[k]) * a.q_token), position[k], u, c.head_dim, y[k]);
 #pragma unroll
     for (int k = 0; k < ROPE_TOKENS; ++k) {
-        if (nth + k >= count)
-            break;
-        T* to = reinterpret_cast<T*>(out + (int64_t)(first + nth + k) * a.out_token);
+        if (row[k] < 0)
+            continue;
+        T* to = reinterpret_cast<T*>(out + (int64_t)row[k] * a.out_token);
         store_run<T, VEC>(to + at.lo, y[k]);
         store_run<T, VEC>(to + at.hi, y[k] + VEC);
     }
@@ -268,11 +315,14 @@ static int launch_append_rope(AppendRopeArgs a, int sequences, hipStream_t strea
 {
     const long units = (long)a.heads * ((a.cache.head_dim + 2 * VEC - 1) / (2 * VEC));
     const long wide = (units + THREADS - 1) / THREADS, append = 2L * sequences * a.blocks * a.cache.kv_heads;
-    const long pairs = (a.cache.max_tokens + ROPE_TOKENS - 1) / ROPE_TOKENS, groups = append + sequences * pairs * wide;
+    // (without cu_tokens a row's sequence is a division away and all have the same tokens)
+    const long pairs = a.cache.cu_tokens == nullptr ? (a.cache.max_tokens + ROPE_TOKENS - 1) / ROPE_TOKENS : 0;
+    const long groups = append + (pairs > 0 ? sequences * pairs : (a.cache.tokens + ROPE_TOKENS - 1) / ROPE_TOKENS) * wide;
     PTOAMD_REQUIRE(groups <= 0x7FFFFFFF, PTOAMD_E_UNSUPPORTED, "ptoamd_kvcache_append_rope: %d sequences of %d tokens are too many for one launch", sequences,
                    a.cache.max_tokens);
     a.wide = (unsigned)(wide > 0 ? wide : 1);
     a.pairs = (unsigned)pairs;
+    a.sequences = sequences;
     a.share = (((uint64_t)append << 32) + groups - 1) / groups;  // (rounded up: after all workgroups, all of the append have been)
     hipLaunchKernelGGL((kvcache_append_rope_kernel<T, CODE, VEC, INTERLEAVED, THREADS>), dim3((unsigned)groups), dim3(THREADS), 0, stream, a);
     PTOAMD_HIP_CHECK(hipGetLastError());

@@ -173,6 +173,36 @@ def test_tokens_without_a_place_and_pages_that_are_none(pa):  # noqa: F811
             assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) if a.is_floating_point() else torch.equal(a, b), (lengths, n)
 
 
+@pytest.mark.parametrize("sequences", [1, 2, 63, 64, 65, 130, 4096, 4097, 5000])
+def test_any_number_of_sequences_and_loose_bounds(pa, sequences):  # noqa: F811
+    """Ragged batches, sequences without tokens among them, behind the first rows and before the last of the batch, max_tokens up to all rows: queries as rope's at
+    each token's place, caches as with the bound that is the most."""
+    g = torch.Generator().manual_seed(sequences)
+    counts = torch.randint(0, 4, (sequences,), generator=g, dtype=torch.int32)
+    counts[torch.rand(sequences, generator=g) < 0.3] = 0
+    counts[sequences // 2] = 9
+    olds = torch.randint(0, 20, (sequences,), generator=g, dtype=torch.int32)
+    cu = torch.cat([torch.zeros(1, dtype=torch.int32), counts.cumsum(0, dtype=torch.int32)]) + 3
+    used, rows = int(counts.sum()), int(counts.sum()) + 8
+    owner = torch.repeat_interleave(torch.arange(sequences), counts.long())
+    positions = torch.zeros(rows, dtype=torch.int32)
+    positions[3:3 + used] = olds[owner] + torch.arange(used, dtype=torch.int32) - (cu[:-1] - 3)[owner]
+    q, k, v = fused(rows, 6, 2, 64, torch.bfloat16, 19)
+    table, lengths = pa.rope_table(64, 64), (olds + counts).cuda()
+    expected = pa.rope(q, table, positions.cuda())
+    results = []
+    for most in (9, 2 * used, rows + 1000):
+        cache = [torch.zeros((2 * sequences, 2, 16, 64), dtype=torch.uint8, device="cuda") for _ in range(2)] + [torch.zeros((2 * sequences, 2), device="cuda") for _ in range(2)]
+        blocks = torch.arange(2 * sequences, dtype=torch.int32, device="cuda").view(sequences, 2)
+        out = torch.full((rows, 6, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+        pa.kvcache_append_rope(q, k, v, *cache, blocks, lengths, pa.I8, table, cu_tokens=cu.cuda(), max_tokens=most, out=out)
+        assert torch.equal(out[3:3 + used], expected[3:3 + used]) and bool((out[:3] == 7.0).all()) and bool((out[3 + used:] == 7.0).all())
+        results.append(cache)
+    assert bool((results[0][2] > 0).any())
+    for cache in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(cache, results[0]))
+
+
 @pytest.mark.parametrize("tree", [False, True])
 def test_padded_batches(pa, tree):  # noqa: F811
     """Rows that no sequence has are neither read nor written."""

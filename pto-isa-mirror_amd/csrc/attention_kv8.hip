@@ -107,18 +107,21 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 //   many : more rows, 256 of them a workgroup (128 for heads of 256 elements)
 // Of drafted tokens, 128 rows a workgroup (HALVES) where there are no more: us, 256 rows a workgroup / 128, 16 sequences of 8192 keys, 64 / 8 heads of 128
 // E4M3, 16 tokens 147 / 105, one of 131072 150 / 110; of 64, 119 / 77; and 32 tokens, 256 rows, 179 / 180, 48 271 / 281, 64 291 / 334.  The few-rows
-// kernel takes up to 64 rows (32 of heads of 256), and more where its workgroups of 32 rows (16) are few: 2 a CU of heads of 128, 3 of 64, 2.5 of 256, or
+// kernel takes up to 64 rows (32 of heads of 256), and more where its workgroups of 32 rows (16) are few: 2 a CU of heads of 128, 3 of 64, 4 of 256, or
 // 1, 2, 2 of up to two turns of 256 keys; and have 16 turns a CU or fewer, 32, 18.  us, few / many, E4M3, rows a key head x sequences x keys, 64 / 8 heads
 // of 128: 512 x 1 x 300, 1000, 3000, 6000, 16000 9 / 21, 14 / 37, 24 / 42, 32 / 45, 72 / 65; 1024 x 1 x 3000 30 / 45; 256 x 1 x 16000 41 / 49, 60000 137 /
 // 90; 128 x 16 x 300, 1000, 2000 22 / 18, 33 / 30, 45 / 49; 256 x 8 x 300, 1000, 2000 22 / 21, 32 / 42, 45 / 52; 384 x 8 47 / 41, 65 / 66 of 1000, 2000;
 // 80 x 16 x 8192 163 / 100; a quarter to all of 192 x 8 x up to 1000, 2000 21 / 28, 25 / 34; of 64: 512 x 4 x 300, 1000, 3000 12 / 17, 18 / 34, 31 / 46;
 // 384 x 8 x 300, 1000, 2000 16 / 18, 23 / 34, 33 / 58; 128 x 32 x 300, 1000 19 / 14, 31 / 24; 768 x 2 x 8000 58 / 73; 1464 x 7 x 528, 16 / 2 heads, 19 /
-// 26; 512 x 1 x 60000 133 / 115; 16 / 2 of 256: 512 x 4 x 1000 21 / 44; 512 x 8 x 300, 1000, 2000 25 / 30, 39 / 52, 58 / 64; 384 x 16 37 / 30, 57 / 59, 85
-// / 77; 512 x 1 x 16000 53 / 61, 768 95 / 72; 128 x 16 x 4000 49 / 62.
+// 26; 512 x 1 x 60000 133 / 115; 16 / 2 of 256, int8: 512 x 4 x 1000 21 / 43; 512 x 8 x 300, 1000, 2000
+// 19 / 28, 31 / 50, 47 / 62; 800 x 8 36 / 29, 58 / 61, 88 / 80; 512 x 16 38 / 30, 59 / 65, 90 / 86; 512 x 1 x 16000 53 / 61, 768 95 / 72.
 // Few rows are 16, 32, or, where the keys are that many, up to 48 a workgroup and 64 of heads of 128: codes are converted once for all of them. 32
 // sequences of 8000 keys, 8 key heads of 128, us, 32 / 48 / 64 rows a workgroup: 32 rows 128 / 153 / 181, 48 226 / 156 / 183, 64 229 / 277 / 188; of 64:
 // 48 rows 114 / 85 / 135, 64 105 / 131 / 125; one sequence of 2000 keys, 48 rows 13.4 / 15.7 / 17.7.  (More than 64: 6 sequences of 7301, 154 rows of
 // drafted tokens, 8 / 4 heads of 128, 32 / 48 / 64 rows 39 / 62 / 57.)
+// Heads of 256 have 16, and of drafted tokens 32 with four waves, which have the registers of two, where workgroups of 16 are more than 5/4 of the CUs:
+// us, int8, 16 / 2 heads, 16 / 32 rows a workgroup: 8 sequences of 1000 keys, 256, 512, 800 rows 22 / 29, 40 / 31, 74 / 58; of 300 13 / 24, 25 / 19, 46 /
+// 36; 16 of 2000, 256 58 / 47, of up to 2000 41 / 46; 8 / 4 heads, 304 rows, four of up to 1412, 304 workgroups, 24 / 29.
 // Parts of the keys.  Few rows: as many as give every CU a workgroup, of two turns of its waves or more, and none where all keys are few turns
 // (a second launch and the join cost 4 to 5 us, a turn 0.7 (heads of 64) to 2 us (256): 300 keys 8.1 us whole, 11.9 in two parts; 1060 keys of
 // heads of 256 16 in five parts, 23 whole); and at most 4096 keys a part, so that a long sequence among short ones is not one workgroup's.
@@ -170,11 +173,13 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
     const long room = PART_ROOM / ((long)tokens * heads * (dim * 4 + 8));  // parts
     const bool busy = items * keys * dim > 65536 * cus;
     p.kernel = rows <= (!busy ? 96 : dim == 256 ? 32 : 64) ? AttentionPlan::FEW : AttentionPlan::MANY;
+    long groups = 0;
     if (tree) {
         // (sequences with fewer tokens than the most have fewer workgroups: those of all tokens, and half a one for what each sequence leaves in its last)
         const long each = dim == 256 ? 16 : 32, turns = (keys + 255) / 256, at_most = items * ((rows + each - 1) / each);
-        const long by_tokens = ((long)tokens * heads / each + items / 2), groups = by_tokens < at_most ? by_tokens : at_most;
-        const bool fits = 2 * groups <= (turns < 3 ? (dim == 128 ? 2 : 4) : dim == 64 ? 6 : dim == 128 ? 4 : 5) * cus && groups * turns <= (dim == 64 ? 32 : 18) * cus;
+        const long by_tokens = (long)tokens * heads / each + items / 2;
+        groups = by_tokens < at_most ? by_tokens : at_most;
+        const bool fits = groups <= (turns < 3 ? (dim == 128 ? 1 : 2) : dim == 64 ? 3 : dim == 128 ? 2 : 4) * cus && groups * turns <= (dim == 64 ? 32 : 18) * cus;
         p.kernel = rows <= (dim == 256 ? 32 : 64) || fits ? AttentionPlan::FEW : AttentionPlan::MANY;
     }
     if (p.kernel == AttentionPlan::FEW) {
@@ -183,6 +188,8 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
             const long alone = items * ((rows + 15) / 16);
             if (alone <= cus && alone * ((keys + 255) / 256) <= (dim == 64 ? 8 : 4) * cus)
                 p.row_tiles = 1;
+            if (dim == 256 && rows > 16 && 4 * groups > 5 * cus)
+                p.row_tiles = 2;
         }
         const long step = 32 * few_waves(dim, p.row_tiles, tree);  // the keys that a workgroup's waves have at a time
         const long turns = (keys + step - 1) / step;
@@ -191,9 +198,9 @@ static AttentionPlan plan_attention(const ptoamd_kv8_cache* c, int heads, int to
         if (turns <= (dim == 256 ? 4 : 6))
             splits = 1;
         if (tree) {
-            const long groups = items * ((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
-            splits = groups < cus ? cus / groups : 1;
-            p.longest = c->sequences > 1 && groups > cus ? (int)keys : 0;
+            const long all = items * ((rows + 16 * p.row_tiles - 1) / (16 * p.row_tiles));
+            splits = all < cus ? cus / all : 1;
+            p.longest = c->sequences > 1 && all > cus ? (int)keys : 0;
             splits = splits < turns ? splits : turns;
             if (turns <= (dim == 64 ? 4 : dim == 128 ? 3 : 2))
                 splits = 1;
@@ -236,13 +243,13 @@ int prepare_attention_kernels()
         for (bool f16 : {false, true})
             for (int dim : {64, 128, 256})
                 for (int tiles : {1, 2, 3, 4}) {
-                    if (tiles > (dim == 64 ? 3 : dim == 128 ? 4 : 1))
+                    if (tiles > (dim == 64 ? 3 : dim == 128 ? 4 : 2))
                         continue;
                     AttentionArgs a{};  // (of no heads: nothing is launched)
                     a.cache.head_dim = dim;
                     a.row_tiles = tiles;
                     a.tile_rows = tiles == 1 ? 128 : 256;  // (of drafted tokens: both)
-                    int rc = launch_attention_few(a, code, f16, 1, nullptr);
+                    int rc = dim == 256 && tiles > 1 ? PTOAMD_OK : launch_attention_few(a, code, f16, 1, nullptr);
                     if (rc == PTOAMD_OK)
                         rc = launch_attention_many(a, code, f16, 1, nullptr);
                     if (rc == PTOAMD_OK)

@@ -56,7 +56,7 @@ constexpr int many_start(int head_dim, int tile_rows) { return 448 / MANY_KEYS *
 // tokens over 8192 keys, 64 / 8 heads of 128, 134 / 119; of 64, 16 x 4 48 / 37, 16 x 6 59 / 45, 40 x 30 ragged up to 4001 35 / 24; of 256, 48 x 2 57 / 50.
 constexpr int few_waves(int head_dim, int row_tiles, bool tree = false)
 {
-    return (head_dim <= 128 && row_tiles == 1) || (tree && (row_tiles == 2 || head_dim != 128)) ? 8 : 4;
+    return (head_dim <= 128 && row_tiles == 1) || (tree && (head_dim == 256 ? row_tiles == 1 : row_tiles == 2 || head_dim == 64)) ? 8 : 4;
 }
 constexpr bool few_queries_in_lds(int head_dim, int row_tiles, bool tree) { return tree && ((head_dim == 64 && row_tiles == 2) || head_dim == 256); }
 int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequences, hipStream_t stream);

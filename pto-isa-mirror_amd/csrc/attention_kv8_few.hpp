@@ -28,7 +28,7 @@ struct FewTile {
 };
 
 // TREE: of drafted tokens.  Keys of the step itself are few: their tiles alone look at a row's bits, which every wave has in LDS for itself.  Eight waves a
-// workgroup but for three and four tiles of rows of heads of 128 (few_waves): rows are many more than in decode, and twice the waves halve the turns.
+// workgroup but for three and four tiles of rows of heads of 128 and two of 256 (few_waves): rows are many more than in decode, and twice the waves halve the turns.
 // Bound: a wave's instructions and, of short sequences, the chain length -> page -> codes.  7 tokens over 300 keys, 32 / 8 heads of 128, int8, 8.4 us; 8 of 24 over 1000,
 // 64 / 8 heads, E4M3, 31; 40 of up to 63 over up to 3503 (665 on average), 16 / 16 of 64, 32: the longest sequence's 14 turns of two workgroups a CU.
 template <typename T, int CODE, int D, int NT, int WAVES, bool TREE>
@@ -426,10 +426,10 @@ static int launch_few(const AttentionArgs& a, int sequences, hipStream_t stream)
 template <typename T, int CODE, int D, bool TREE>
 static int choose_tiles(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
-    // (two tiles of 256 columns' sums and fragments do not fit the registers, nor four of 128 columns more than one wave a SIMD)
+    // (two tiles of 256 columns' sums and fragments fit the registers of one wave a SIMD alone, as do four of 128 columns)
     switch (a.row_tiles) {
         case 1: return launch_few<T, CODE, D, 1, few_waves(D, 1, TREE), TREE>(a, sequences, stream);
-        case 2: if constexpr (D < 256) return launch_few<T, CODE, D, 2, few_waves(D, 2, TREE), TREE>(a, sequences, stream); break;
+        case 2: if constexpr (D < 256 || TREE) return launch_few<T, CODE, D, 2, few_waves(D, 2, TREE), TREE>(a, sequences, stream); break;
         case 3: if constexpr (D < 256) return launch_few<T, CODE, D, 3, few_waves(D, 3, TREE), TREE>(a, sequences, stream); break;
         case 4: if constexpr (D == 128) return launch_few<T, CODE, D, 4, few_waves(D, 4, TREE), TREE>(a, sequences, stream); break;
     }

@@ -13,14 +13,15 @@ from test_gpu_parity import pa  # noqa: F401
 pytestmark = pytest.mark.gpu
 
 
-def run(pa, code, olds, counts, heads, kv_heads, dim, page, dtype=torch.bfloat16, seed=1, token_major=False, strided=False, ways=None, width=0, **kw):
+def run(pa, code, olds, counts, heads, kv_heads, dim, page, dtype=torch.bfloat16, seed=1, token_major=False, strided=False, ways=None, width=0, small=False, **kw):
     cache = ref.Cache(code, [max(o + n, 0) for o, n in zip(olds, counts)], kv_heads, dim, page, seed, token_major)
     q = queries(sum(counts), heads, dim, dtype, seed + 1, strided)
     ways = dr.ways_of(dr.parents_of(counts, seed, width)) if ways is None else ways
     rows = dr.rows_of(ways, -(-max(counts) // 64))
     print("drafted", code, olds[:4], counts[:4], heads, kv_heads, dim, page, kw, flush=True)
     out, lse = pa.attention_kv8_tree(q, *cache.operands(pa), rows, cu_tokens=ref.starts(counts), max_tokens=max(counts), want_lse=True, **kw)
-    expected = dr.attention(q, cache, ways, **{k: v for k, v in kw.items() if k in ("window", "scale")})
+    (result, norm, magnitude, spread), least = dr.attention_and_least(q, cache, ways, **{k: v for k, v in kw.items() if k in ("window", "scale")})
+    expected = (result, norm, magnitude + 2.0 ** 11 * least if small else magnitude, spread)  # (2^-11 of a magnitude is what the check allows)
     ref.check_attention(out, expected, lse)
     return cache, q, rows, out, lse
 
@@ -128,6 +129,19 @@ def test_batches_of_more_workgroups_than_compute_units(pa, dim, sequences):  # n
     q = queries(3 * sequences, 16, dim, torch.bfloat16, 5, False)
     out, lse = pa.attention_kv8_tree(q, *cache.operands(pa), dr.rows_of(ways, 1), want_lse=True)
     ref.check_attention(out, dr.attention(q, cache, ways), lse)
+
+
+@pytest.mark.parametrize("code", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim,kw", [(256, {}), (256, {"window": 300}), (176, {})])
+def test_large_heads_of_many_rows(pa, code, dtype, dim, kw):  # noqa: F811
+    """Sequences of a few keys among them: of 60 x 16 x 256 sums some are of codes that are all small, where the 128 that int8 codes are multiplied with shows.  (By
+    attention_and_least, 2^-12 of the sum of p s: f16, int8, an element was off by 3.8e-7, of which 5e-8 were beyond the check's 2^-11 of sum p s |code|; s here is
+    some 0.9 / 127, so that bound allows 1.7e-6 more.)"""
+    rng = random.Random(dim + len(kw))
+    counts = [rng.randint(0, 9) for _ in range(60)]
+    run(pa, code, [rng.choice([0, 5, 31, 250, 600]) for _ in counts], counts, 16, 2, dim, 16, dtype, strided=True, small=True, **kw)
+    run(pa, code, [5000, 300, 4500, 0, 77], [70, 65, 55, 3, 60], 24, 3, dim, 64, dtype, **kw)
 
 
 @pytest.mark.parametrize("dim", [64, 128, 256, 72])

@@ -14,7 +14,7 @@ int launch_attention_few(const AttentionArgs& a, int code, bool f16, int sequenc
 // elements each.  ROWS = 1: few rows of many parts, one a workgroup, whose 1024 / D groups of lanes take every (1024 / D)-th part and are added in
 // order.  Else ROWS = 1024 / D rows a workgroup, a group of lanes each: no group waits for another.
 // (1309 rows of tokens, 32 heads of 128, two parts: 42.3 us with ROWS = 1, some 14 with 8.)
-template <typename T, int D, int ROWS>
+template <typename T, int D, int ROWS, bool TREE>
 __global__ void __launch_bounds__(256) attention_kv8_join_kernel(AttentionArgs a)
 {
     constexpr int LANES = D / 4, GROUPS = 256 / LANES, STEP = ROWS == 1 ? GROUPS : 1;
@@ -38,7 +38,7 @@ __global__ void __launch_bounds__(256) attention_kv8_join_kernel(AttentionArgs a
     } else {
         if (!several_parts(a, span))
             return;
-        const int2 keys = a.tree != nullptr ? keys_of_any<true>(a, span, nth, nth) : visible_keys(a, span.length - span.count + nth, span.length);
+        const int2 keys = TREE ? keys_of_any<true>(a, span, nth, nth) : visible_keys(a, span.length - span.count + nth, span.length);
         from = min((keys.x - span.begin) / a.chunk, a.splits - 1);
         to = keys.y > keys.x ? min((keys.y - 1 - span.begin) / a.chunk, a.splits - 1) + 1 : from;
     }
@@ -97,33 +97,34 @@ __global__ void __launch_bounds__(256) attention_kv8_join_kernel(AttentionArgs a
         a.lse[at] = sum == 0.0f ? -INFINITY : (top + __builtin_amdgcn_logf(sum)) * 0.69314718055994531f;
 }
 
-template <typename T, int D>
+template <typename T, int D, bool TREE>
 static void launch_join(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
     const long rows = (long)a.cache.max_tokens * a.heads;
     constexpr int ROWS = 1024 / D;
     // (rows for four workgroups a compute unit, of a group of lanes each: before that a row's parts are what keeps the card busy.  Of drafted tokens, also where
     // the parts are few: 16 x 6 tokens over 4000 keys in two, 64 / 8 heads of 128, 47.8 us with a row a workgroup, 43.0; one over 1000 in four 10.7 and 11.1)
-    if (rows * sequences >= 4L * ROWS * device_compute_units() || (a.tree != nullptr && a.splits <= 4))
-        hipLaunchKernelGGL((attention_kv8_join_kernel<T, D, ROWS>), dim3((unsigned)((rows + ROWS - 1) / ROWS), 1, (unsigned)sequences), dim3(256), 0, stream, a);
+    if (rows * sequences >= 4L * ROWS * device_compute_units() || (TREE && a.splits <= 4))
+        hipLaunchKernelGGL((attention_kv8_join_kernel<T, D, ROWS, TREE>), dim3((unsigned)((rows + ROWS - 1) / ROWS), 1, (unsigned)sequences), dim3(256), 0, stream, a);
     else
-        hipLaunchKernelGGL((attention_kv8_join_kernel<T, D, 1>), dim3((unsigned)rows, 1, (unsigned)sequences), dim3(256), 0, stream, a);
+        hipLaunchKernelGGL((attention_kv8_join_kernel<T, D, 1, TREE>), dim3((unsigned)rows, 1, (unsigned)sequences), dim3(256), 0, stream, a);
 }
-template <typename T>
+template <typename T, bool TREE>
 static void choose_join(const AttentionArgs& a, int sequences, hipStream_t stream)
 {
     switch (built_head(a.cache.head_dim)) {
-        case 64: launch_join<T, 64>(a, sequences, stream); break;
-        case 128: launch_join<T, 128>(a, sequences, stream); break;
-        default: launch_join<T, 256>(a, sequences, stream); break;
+        case 64: launch_join<T, 64, TREE>(a, sequences, stream); break;
+        case 128: launch_join<T, 128, TREE>(a, sequences, stream); break;
+        default: launch_join<T, 256, TREE>(a, sequences, stream); break;
     }
 }
 int launch_attention_join(const AttentionArgs& a, bool f16, int sequences, hipStream_t stream)
 {
+    const bool tree = a.tree != nullptr;
     if (f16)
-        choose_join<_Float16>(a, sequences, stream);
+        tree ? choose_join<_Float16, true>(a, sequences, stream) : choose_join<_Float16, false>(a, sequences, stream);
     else
-        choose_join<__bf16>(a, sequences, stream);
+        tree ? choose_join<__bf16, true>(a, sequences, stream) : choose_join<__bf16, false>(a, sequences, stream);
     PTOAMD_HIP_CHECK(hipGetLastError());
     return PTOAMD_OK;
 }

@@ -17,7 +17,7 @@ __global__ void __launch_bounds__(64) attention_kv8_generic_kernel(AttentionArgs
     const int length = c.length(seq), dim = c.head_dim;
     const int old = length - count;
     const uint32_t* bits = TREE ? a.tree + (int64_t)(first + nth) * a.tree_words : nullptr;
-    const int2 keys = TREE ? make_int2(first_key(old + others_seen(bits, a.tree_words, count, nth), a.window), length) : visible_keys(a, old + nth, length);
+    const int2 keys = TREE ? make_int2(first_of_older(bits, a.tree_words, count, nth, old, a.window), length) : visible_keys(a, old + nth, length);
     __shared__ float q[512], weight[64];  // (weights below 0: of keys that are not seen)
     const T* row = reinterpret_cast<const T*>(a.q + (int64_t)(first + nth) * a.q_token + (int64_t)head * a.q_head);
     for (int i = lane; i < dim; i += 64)
@@ -30,9 +30,7 @@ __global__ void __launch_bounds__(64) attention_kv8_generic_kernel(AttentionArgs
         __syncthreads();  // q; the weights of the tile before have been read
         const int key = base + lane;
         float s = -INFINITY;
-        bool seen = key < keys.y;
-        if (TREE && seen && key >= old)
-            seen = (row_bits(bits, a.tree_words, key - old) & 1u) != 0;
+        const bool seen = TREE ? (seen_keys(bits, a.tree_words, base + (lane & 32), keys.x, old, length) >> (lane & 31) & 1u) != 0 : key < keys.y;
         if (seen) {
             const int page = c.page_of(seq, key >> c.page_shift), slot = key & ((1 << c.page_shift) - 1);
             const uint8_t* k = c.k.codes + (int64_t)max(page, 0) * c.k.page + (int64_t)kv_head * c.k.head + (int64_t)slot * c.k.token;

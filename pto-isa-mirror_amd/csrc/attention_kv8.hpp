@@ -179,19 +179,14 @@ __device__ __forceinline__ int2 keys_of_every(const AttentionArgs& a, const Span
 // Words of a drafted token's row, its bits behind the sequence's last token cleared.
 __device__ __forceinline__ uint32_t drafted_word(const AttentionArgs& a, const Span& s, int token, int word)
 {
-    return word < a.tree_words ? a.tree[(int64_t)(s.first + token) * a.tree_words + word] & bits_below(s.count - 32 * word) : 0u;
+    return own_word(a.tree + (int64_t)(s.first + token) * a.tree_words, a.tree_words, word, s.count);
 }
 // The first of the older keys that a token sees, whose `words` words lie in LDS.  (No row: none of them.)
 __device__ __forceinline__ int first_of_drafted(const AttentionArgs& a, const Span& s, const uint32_t* row, int words, bool valid, int token)
 {
     if (!valid)
         return 0x7FFFFFFF;
-    return a.window > 0 ? first_key(s.length - s.count + others_seen(row, words, s.count, token), a.window) : 0;
-}
-// Which of the keys key .. key + 31 a token sees (seen_keys: `key` is the same for all lanes, and words behind the last token are 0).
-__device__ __forceinline__ uint32_t drafted_keys(const uint32_t* row, int words, int key, int first, int old)
-{
-    return (bits_below(old - key) & ~bits_below(first - key)) | row_bits(row, words, key - old);
+    return first_of_older(row, words, s.count, token, s.length - s.count, a.window);
 }
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));

@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
             }
             if (TREE && !whole) {
                 const uint32_t* row = drafted[wave][16 * t + col];
-                const uint32_t mine = drafted_keys(row, tree_words, key, (int)row[TREE_WORDS], every_to) >> (4 * g);
+                const uint32_t mine = seen_by_own(row, tree_words, key, (int)row[TREE_WORDS], every_to) >> (4 * g);
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
                     w[j / 4][j % 4] = (mine & 1u << (16 * (j / 4) + j % 4)) != 0 ? w[j / 4][j % 4] : -INFINITY;

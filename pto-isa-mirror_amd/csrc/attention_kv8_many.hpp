@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
 #pragma unroll
                 for (int i = 0; i < ROW_WORDS; ++i) {
                     const int its = 32 * wave + (lane + 64 * i) / MANY_TREE_WORDS, word = lane % MANY_TREE_WORDS;
-                    drafted[its][word] = row0 + its < rows && word < a.tree_words ? words[i] & bits_below(span.count - 32 * word) : 0u;
+                    drafted[its][word] = row0 + its < rows && word < a.tree_words ? own_bits(words[i], word, span.count) : 0u;
                 }
                 seen.x = first_of_drafted(a, span, drafted[32 * wave + col], MANY_TREE_WORDS, valid, token);
             } else {
@@ -402,7 +402,7 @@ __global__ void __launch_bounds__(64 * WAVES) __attribute__((amdgpu_waves_per_eu
                 if constexpr (TREE)
 #pragma unroll
                     for (int h = 0; h < 2; ++h)
-                        mine[h] = drafted_keys(drafted[32 * wave + col], MANY_TREE_WORDS, key + 32 * h, seen.x, place0) >> (4 * hf);
+                        mine[h] = seen_by_own(drafted[32 * wave + col], MANY_TREE_WORDS, key + 32 * h, seen.x, place0) >> (4 * hf);
 #pragma unroll
                 for (int x = 0; x < KEYS / 16; ++x)
 #pragma unroll

@@ -4,6 +4,7 @@
 #include <stdint.h>
 
 #include "../../include/ptoamd.h"
+#include "kv8_places.hpp"
 
 namespace ptoamd {
 
@@ -32,6 +33,22 @@ __host__ __device__ __forceinline__ int others_seen(const uint32_t* row, int wor
 __host__ __device__ __forceinline__ uint32_t seen_keys(const uint32_t* row, int words, int key, int first, int old, int length)
 {
     return (bits_below(old - key) & ~bits_below(first - key)) | (row_bits(row, words, key - old) & bits_below(length - key));
+}
+// The same of a row whose bits of tokens that the sequence does not have are 0 already (own_word): no key behind the last has one.
+__host__ __device__ __forceinline__ uint32_t seen_by_own(const uint32_t* row, int words, int key, int first, int old)
+{
+    return (bits_below(old - key) & ~bits_below(first - key)) | row_bits(row, words, key - old);
+}
+// A row's word without the bits of tokens that a sequence of `count` drafted ones does not have; of a row of `words` words, 0 behind them.
+__host__ __device__ __forceinline__ uint32_t own_bits(uint32_t x, int word, int count) { return x & bits_below(count - 32 * word); }
+__host__ __device__ __forceinline__ uint32_t own_word(const uint32_t* row, int words, int word, int count)
+{
+    return word < words ? own_bits(row[word], word, count) : 0u;
+}
+// The first of the `old` older keys that a window leaves to the token numbered `self`, which stands behind the others that it sees.  (0: no window.)
+__host__ __device__ __forceinline__ int first_of_older(const uint32_t* row, int words, int count, int self, int old, int window)
+{
+    return window > 0 ? first_key(old + others_seen(row, words, count, self), window) : 0;
 }
 
 }  // namespace ptoamd

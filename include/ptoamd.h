@@ -458,12 +458,15 @@ int ptoamd_attention_kv8(void* out, float* lse, const ptoamd_kv8_cache* cache, c
  * ptoamd_draft_tree makes the rows from parents: a token sees itself and its ancestors.
  *   parents : [tokens] int32, the place of a token's parent among its sequence's drafted ones, or -1: the last token that is older.  A parent that
  *             is neither -1 nor before the token leaves the token's row empty (and its descendants see nothing beyond the token).
- *   tree    : [tokens][tree_words], apart from parents and cu_tokens.  Rows that no sequence has are not written.
+ *   tree    : [tokens][tree_words], apart from parents and cu_tokens.  Rows that no sequence has are not written; by ptoamd_draft_tree_all they become
+ *             empty ones.
  *   cu_tokens, max_tokens : as for the append below; NULL: tokens = sequences * max_tokens
  */
 #define PTOAMD_MOST_DRAFTED 256
 int ptoamd_draft_tree(uint64_t* tree, int tree_words, const int32_t* parents, int tokens, int sequences, const int32_t* cu_tokens, int max_tokens,
                       void* stream);
+int ptoamd_draft_tree_all(uint64_t* tree, int tree_words, const int32_t* parents, int tokens, int sequences, const int32_t* cu_tokens, int max_tokens,
+                          void* stream);
 
 /*
  * ptoamd_rope of q and k and ptoamd_kvcache_append of k and v in one launch: queries [tokens][heads][head_dim] are turned into q_out, keys on their way

@@ -53,7 +53,7 @@ EXPORTS = [
     "ptoamd_tquant_int8_para", "ptoamd_tquant_mx", "ptoamd_tdequant", "ptoamd_tdequant_para", "ptoamd_mx_scale_relayout",
     "ptoamd_last_kernel", "ptoamd_reload_options",
     "ptoamd_rope_table", "ptoamd_rope", "ptoamd_kvcache_append", "ptoamd_attention_kv8_workspace_bytes", "ptoamd_attention_kv8",
-    "ptoamd_draft_tree", "ptoamd_kvcache_append_rope", "ptoamd_attention_kv8_tree_workspace_bytes", "ptoamd_attention_kv8_tree", "ptoamd_kvcache_keep",
+    "ptoamd_draft_tree", "ptoamd_draft_tree_all", "ptoamd_kvcache_append_rope", "ptoamd_attention_kv8_tree_workspace_bytes", "ptoamd_attention_kv8_tree", "ptoamd_kvcache_keep",
 ]
 
 # Argument types of the entry points called below (p: device address or stream, i: int, l: int64_t, z: size_t, f: float, d: double): with them ctypes takes plain
@@ -84,6 +84,7 @@ _SIGNATURES = {
     "ptoamd_kvcache_append": "pppiipi" + "llll" + "p",
     "ptoamd_attention_kv8": "ppppiiipii" + "llll" + "fii" + "pzp",
     "ptoamd_draft_tree": "pipiipi" + "p",
+    "ptoamd_draft_tree_all": "pipiipi" + "p",
     "ptoamd_kvcache_append_rope": "pppippiipipiiippi" + "llllllll" + "p",
     "ptoamd_attention_kv8_tree": "ppppipiiipii" + "llll" + "fi" + "pzp",
     "ptoamd_kvcache_keep": "pppipi" + "p",
@@ -554,16 +555,17 @@ def draft_tree(parents, sequences, cu_tokens=None, max_tokens=None, stream=None,
     """What each drafted token sees of those drafted with it, itself and its ancestors, as rows of bits: [tokens, ceil(max_tokens / 64)] int64,
     bit t % 64 of word t / 64 for its sequence's token t.  parents [tokens] int32: a token's parent among its sequence's, before it, or -1 (the
     last token that is older); any other value leaves the token's row empty.  cu_tokens [sequences + 1]: where each sequence's tokens start (None: equal
-    shares); at most 256 tokens a sequence.  Rows that cu_tokens gives to no sequence are not written."""
+    shares); at most 256 tokens a sequence.  Rows that cu_tokens gives to no sequence are empty; in a given out they are left as they are."""
     what = "draft_tree"
     _require(parents.dim() == 1, f"{what}: parents must be [tokens]")
     tokens = parents.shape[0]
     cu, most = _tokens_of(what, tokens, sequences, cu_tokens, max_tokens)
+    draft = _lib.ptoamd_draft_tree
     if out is None:
         out = torch.empty((tokens, max(1, (min(most, tokens) + 63) // 64)), dtype=torch.int64, device=parents.device)
+        draft = _lib.ptoamd_draft_tree_all
     address, words = _tree(out, tokens, f"{what}: out")
-    _check(_lib.ptoamd_draft_tree(address, words, _int32(parents, (tokens,), f"{what}: parents"), tokens, sequences, cu, most, _stream(stream)),
-           "ptoamd_draft_tree")
+    _check(draft(address, words, _int32(parents, (tokens,), f"{what}: parents"), tokens, sequences, cu, most, _stream(stream)), "ptoamd_draft_tree")
     return out
 
 

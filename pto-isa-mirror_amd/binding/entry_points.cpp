@@ -525,12 +525,14 @@ PyObject* draft_tree(const Call& c)
     }
     {
         Released no_gil;
+        auto draft = ptoamd_draft_tree;
         if (!out.defined()) {
+            draft = ptoamd_draft_tree_all;
             const int rows = most < tokens ? most : tokens;
             words = rows > 64 ? (rows + 63) / 64 : 1;
             out = empty({tokens, words}, at::kLong, parents);
         }
-        check(ptoamd_draft_tree(address_as<uint64_t>(out), words, address_as<const int32_t>(parents), tokens, sequences.sequences, cu, most, stream()),
+        check(draft(address_as<uint64_t>(out), words, address_as<const int32_t>(parents), tokens, sequences.sequences, cu, most, stream()),
               "ptoamd_draft_tree");
     }
     return wrap(std::move(out));

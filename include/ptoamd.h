@@ -475,7 +475,8 @@ int ptoamd_draft_tree_all(uint64_t* tree, int tree_words, const int32_t* parents
  *   positions  : [tokens] int32, or NULL: a token's place in its sequence, lengths[s] - n + i; with `tree` (only without positions) a drafted token
  *                stands behind the others that it sees: lengths[s] - n + the number of bits of its row without its own
  *   type       : of q, k, v and q_out: PTOAMD_F32 | F16 | BF16
- *   q_out      : may be q (with its strides), and overlap none of the operands in any other way
+ *   q_out      : may be q (with its strides), and overlap none of the operands in any other way (refused, where addresses and strides show it: always for
+ *                what has no strides, for q, k and v where they are views of one tensor with q_out or heads lie together)
  * A token whose position is not in 0 .. table_rows - 1 gets NaN for the rot_dim elements of its queries, and makes its page's key scales NaN.  Queries of
  * tokens that have no place in the cache are turned as the others are.  Rows that no sequence has are neither read nor written.
  */

@@ -4,6 +4,7 @@
 #include "kv8.hpp"
 #include "kv8_codes.hpp"
 #include "kv8_places.hpp"
+#include "overlap.hpp"
 
 namespace ptoamd {
 
@@ -426,6 +427,21 @@ int ptoamd_kvcache_append_rope(const ptoamd_kv8_cache* cache, void* q_out, const
         a.out_token = q_out_token_stride * size;
         a.out_head = q_out_head_stride * size;
     }
+    // (queries are written while other workgroups still read all of these)
+    const HeadRows result{(uint64_t)(uintptr_t)q_out, tokens, heads, q_out_token_stride * size, q_out_head_stride * size, (int64_t)cache->head_dim * size};
+    auto apart = [&](const void* p, int64_t bytes) { return !meet(result, memory_at(p, bytes)); };
+    auto apart_from_rows = [&](const void* p, int n, int64_t token, int64_t head) {
+        return !meet(result, HeadRows{(uint64_t)(uintptr_t)p, tokens, n, token * size, head * size, (int64_t)cache->head_dim * size});
+    };
+    PTOAMD_REQUIRE(q_out == q || apart_from_rows(q, heads, q_token_stride, q_head_stride), PTOAMD_E_INVALID, "%s: q_out must be q or not overlap it", what);
+    PTOAMD_REQUIRE(apart_from_rows(k, cache->kv_heads, k_token_stride, k_head_stride) && apart_from_rows(v, cache->kv_heads, v_token_stride, v_head_stride),
+                   PTOAMD_E_INVALID, "%s: q_out must not overlap k or v", what);
+    PTOAMD_REQUIRE(apart(table, (int64_t)table_rows * rot_dim * 4) && apart(positions, tokens * 4L) && apart(tree, (int64_t)tokens * tree_words * 8), PTOAMD_E_INVALID,
+                   "%s: q_out must not overlap table, positions or tree", what);
+    PTOAMD_REQUIRE(apart(cu_tokens, 4L * (cache->sequences + 1)) && apart(cache->lengths, 4L * cache->sequences) &&
+                       apart(cache->block_table, 4L * cache->sequences * cache->max_pages) && apart(cache->k_scale, 4L * cache->pages * cache->kv_heads) &&
+                       apart(cache->v_scale, 4L * cache->pages * cache->kv_heads),
+                   PTOAMD_E_INVALID, "%s: q_out must not overlap cu_tokens, lengths, block_table or the scales", what);
     a.table = table;
     a.positions = positions;
     a.tree = reinterpret_cast<const uint32_t*>(tree);

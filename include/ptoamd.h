@@ -492,6 +492,7 @@ int ptoamd_kvcache_append_rope(const ptoamd_kv8_cache* cache, void* q_out, const
  *   where j = L - n + t, t >= 0 and bit t of its row is set.
  * window is 0 or at least max_tokens, so that what a token sees of the tree lies within it.  Any bits are taken, a tree's or not: a query that sees
  * nothing at all gets zeros and lse = -infinity.  Codes of drafted tokens must be numbers, whether a query sees them or not.
+ *   tree      : rows of bits, apart from out and lse
  *   workspace : ptoamd_attention_kv8_tree_workspace_bytes(...) bytes, as for ptoamd_attention_kv8
  */
 size_t ptoamd_attention_kv8_tree_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window);
@@ -504,7 +505,7 @@ int ptoamd_attention_kv8_tree(void* out, float* lse, const ptoamd_kv8_cache* cac
  * Keeps a path of the drafted tokens: they move together behind the older ones, in the codes that they have.
  *   kept        : [sequences][max_kept] int32: drafted tokens in ascending order.  A list ends at the first entry that is not above the one before, or
  *                 is none of 0 .. n - 1 (so -1 fills it up); r entries are kept
- *   new_lengths : [sequences] int32, gets lengths[s] - n + r.  Apart from lengths, kept and cu_tokens.
+ *   new_lengths : [sequences] int32, gets lengths[s] - n + r.  Apart from lengths, kept, cu_tokens, block_table and the scales.
  *   cu_tokens   : as for the append: n = cu_tokens[s + 1] - cu_tokens[s], at most max_tokens.  NULL: n = max_tokens
  * Token kept[i] moves from place lengths[s] - n + kept[i] to lengths[s] - n + i.  Within a page its codes are copied.  Where tokens come into a page
  * from others, a = max |code| * (scale of their page) of those, the page's scale becomes s1 = max(s0, a * (1 / Q)) as in an append; what was there and

@@ -1,5 +1,6 @@
 // Attention over a cache of keys and values held in 8 bits: the generic kernel, the choice of a kernel, the entry points.
 #include "attention_kv8.hpp"
+#include "overlap.hpp"
 
 namespace ptoamd {
 
@@ -297,6 +298,12 @@ static int attention(const char* what, void* out, float* lse, const ptoamd_kv8_c
     PTOAMD_REQUIRE(out && q, PTOAMD_E_INVALID, "%s: null operand", what);
     PTOAMD_REQUIRE((reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(q)) % 2 == 0 && reinterpret_cast<uintptr_t>(lse) % 4 == 0, PTOAMD_E_ALIGNMENT,
                    "%s: q, out and lse must be aligned to their elements", what);
+    if (tree != nullptr) {  // (workgroups write results while others still read their rows of bits)
+        const HeadRows bits = memory_at(tree, (int64_t)tokens * tree_words * 8);
+        PTOAMD_REQUIRE(!meet(bits, HeadRows{(uint64_t)(uintptr_t)out, tokens, heads, out_token_stride * 2, out_head_stride * 2, cache->head_dim * 2L}) &&
+                           !meet(bits, memory_at(lse, (int64_t)tokens * heads * 4)),
+                       PTOAMD_E_INVALID, "%s: out and lse must not overlap the tree", what);
+    }
     a.q = static_cast<const uint8_t*>(q);
     a.out = static_cast<uint8_t*>(out);
     a.lse = lse;

@@ -266,6 +266,10 @@ int ptoamd_kvcache_keep(const ptoamd_kv8_cache* cache, int32_t* new_lengths, con
     PTOAMD_REQUIRE(apart(cache->lengths, cache->sequences), PTOAMD_E_INVALID, "%s: new_lengths must not be lengths", what);
     PTOAMD_REQUIRE(apart(kept, (long)cache->sequences * max_kept) && apart(cu_tokens, cache->sequences + 1L), PTOAMD_E_INVALID,
                    "%s: new_lengths must not overlap kept or cu_tokens", what);
+    PTOAMD_REQUIRE(apart(cache->block_table, (long)cache->sequences * cache->max_pages) &&
+                       apart(reinterpret_cast<const int32_t*>(cache->k_scale), (long)cache->pages * cache->kv_heads) &&
+                       apart(reinterpret_cast<const int32_t*>(cache->v_scale), (long)cache->pages * cache->kv_heads),
+                   PTOAMD_E_INVALID, "%s: new_lengths must not overlap block_table or the scales", what);
     a.kept = kept;
     a.new_lengths = new_lengths;
     a.max_kept = max_kept;

@@ -69,3 +69,32 @@ def test_append_into_a_fused_product(head):
     strides = (512, 64)
     rc, error = append(at, "positions", strides, strides, strides, strides)
     assert rc == -1 and "overlap" in error, error
+
+
+def keep(at):
+    """Two sequences of eight drafted tokens, four entries each: (code, text)."""
+    pa = ge.load_package()
+    cache = cache_at(pa, at)
+    rc = pa.lib().ptoamd_kvcache_keep(ctypes.addressof(cache), at["out"], at["q"], 4, at["cu"], 8, None)
+    return rc, pa.lib().ptoamd_last_error().decode()
+
+
+@pytest.mark.parametrize("name", ["block_table", "k_scale", "v_scale"])
+@pytest.mark.parametrize("end", ["first", "last"])
+def test_new_lengths_over_what_keep_reads(name, end):
+    at = places()
+    rc, error = keep({**at, "out": at[name] - 4 if end == "first" else at[name] + BYTES[name] - 4})
+    assert rc == -1 and "new_lengths must not overlap block_table or the scales" in error, error
+
+
+@pytest.mark.parametrize("name", ["out", "lse"])
+@pytest.mark.parametrize("end", ["first", "last"])
+def test_attention_over_its_tree(name, end):
+    pa, at = ge.load_package(), places()
+    cache = cache_at(pa, at)
+    size = OUT if name == "out" else 5 * 4 * 4
+    mine = {"out": at["out"], "lse": None, name: at["tree"] - size + 4 if end == "first" else at["tree"] + BYTES["tree"] - 4}
+    rc = pa.lib().ptoamd_attention_kv8_tree(mine["out"], mine["lse"], ctypes.addressof(cache), at["tree"], 1, at["q"], pa.BF16, 4, 5, at["cu"], 3, 0, 256, 64, 256, 64, 0.125, 0,
+                                            None, 0, None)
+    error = pa.lib().ptoamd_last_error().decode()
+    assert rc == -1 and "out and lse must not overlap the tree" in error, error

@@ -439,7 +439,8 @@ int ptoamd_kvcache_append(const ptoamd_kv8_cache* cache, const void* k, const vo
  * Sums of a softmax, of scores and of values are held in f32; the scores' products take q as f16 scaled by a power of two for each row
  * (bf16 and f16 queries lose nothing that is within 2^-14 of their row's largest element), the values' products take each weight, times its
  * page's value scale, rounded to f16 relative to the largest such so far: full f16 precision down to 2^-25 of that, nothing below 2^-36.  A
- * value scale below 2^-64 counts as 0.  (Kernels are built for heads of 64, 128 and 256; other multiples of 16 up to 256 take the next of them.
+ * value scale below 2^-64 counts as 0.  int8 values are multiplied as code + 128 and the 128 is taken off tile by tile: a result is off by up to 2^-12 of the
+ * sum of e^(s_j) times page scale over that of e^(s_j), which shows where a row's codes are nearly all 0.  (Kernels are built for heads of 64, 128 and 256; other multiples of 16 up to 256 take the next of them.
  * What is left, and caches or strides off 16 bytes, runs on a kernel that is in f32 throughout, and slow.)
  */
 size_t ptoamd_attention_kv8_workspace_bytes(const ptoamd_kv8_cache* cache, int heads, int tokens, int max_tokens, int max_length, int window);

@@ -507,13 +507,14 @@ int ptoamd_attention_kv8_tree(void* out, float* lse, const ptoamd_kv8_cache* cac
  *   kept        : [sequences][max_kept] int32: drafted tokens in ascending order.  A list ends at the first entry that is not above the one before, or
  *                 is none of 0 .. n - 1 (so -1 fills it up); r entries are kept
  *   new_lengths : [sequences] int32, gets lengths[s] - n + r.  Apart from lengths, kept, cu_tokens, block_table and the scales.
- *   cu_tokens   : as for the append: n = cu_tokens[s + 1] - cu_tokens[s], at most max_tokens.  NULL: n = max_tokens
+ *   cu_tokens   : as for the append: n = cu_tokens[s + 1] - cu_tokens[s], at most max_tokens (1 .. 256).  NULL: n = max_tokens
  * Token kept[i] moves from place lengths[s] - n + kept[i] to lengths[s] - n + i.  Within a page its codes are copied.  Where tokens come into a page
  * from others, a = max |code| * (scale of their page) of those, the page's scale becomes s1 = max(s0, a * (1 / Q)) as in an append; what was there and
  * stays becomes round(code * (s0 / s1)) where s1 > s0, and what comes round(code * (scale of its page / s1)).  So a page keeps a scale that the
  * tokens not kept have raised, until it is begun anew.  If a token comes from a page that the table does not name, or whose scale is NaN, the scale of
  * the page that it comes to is NaN from then on; a page that the table does not name takes nothing.  Codes behind the kept tokens are left as they are.
- * A sequence with lengths[s] < n, or beyond max_pages, is left as it is, with its length.
+ * A sequence with lengths[s] < n, or beyond max_pages, is left as it is, with its length.  A path is kept in every layer's cache, a call each: lengths stays as it
+ * is until the last.
  */
 int ptoamd_kvcache_keep(const ptoamd_kv8_cache* cache, int32_t* new_lengths, const int32_t* kept, int max_kept, const int32_t* cu_tokens, int max_tokens,
                         void* stream);

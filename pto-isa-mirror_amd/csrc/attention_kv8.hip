@@ -107,13 +107,16 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 // Of drafted tokens, 128 rows a workgroup (HALVES) where there are no more: us, 256 rows a workgroup / 128, 16 sequences of 8192 keys, 64 / 8 heads of 128
 // E4M3, 16 tokens 147 / 105, one of 131072 150 / 110; of 64, 119 / 77; and 32 tokens, 256 rows, 179 / 180, 48 271 / 281, 64 291 / 334.  The few-rows
 // kernel takes up to 64 rows (32 of heads of 256), and more where its workgroups of 32 rows (16) are few: 2 a CU of heads of 128, 3 of 64, 4 of 256, or
-// 1, 2, 2 of up to two turns of 256 keys; and have 16 turns a CU or fewer, 32, 18.  us, few / many, E4M3, rows a key head x sequences x keys, 64 / 8 heads
-// of 128: 512 x 1 x 300, 1000, 3000, 6000, 16000 9 / 21, 14 / 37, 24 / 42, 32 / 45, 72 / 65; 1024 x 1 x 3000 30 / 45; 256 x 1 x 16000 41 / 49, 60000 137 /
-// 90; 128 x 16 x 300, 1000, 2000 22 / 18, 33 / 30, 45 / 49; 256 x 8 x 300, 1000, 2000 22 / 21, 32 / 42, 45 / 52; 384 x 8 47 / 41, 65 / 66 of 1000, 2000;
-// 80 x 16 x 8192 163 / 100; a quarter to all of 192 x 8 x up to 1000, 2000 21 / 28, 25 / 34; of 64: 512 x 4 x 300, 1000, 3000 12 / 17, 18 / 34, 31 / 46;
-// 384 x 8 x 300, 1000, 2000 16 / 18, 23 / 34, 33 / 58; 128 x 32 x 300, 1000 19 / 14, 31 / 24; 768 x 2 x 8000 58 / 73; 1464 x 7 x 528, 16 / 2 heads, 19 /
-// 26; 512 x 1 x 60000 133 / 115; 16 / 2 of 256, int8: 512 x 4 x 1000 21 / 43; 512 x 8 x 300, 1000, 2000
-// 19 / 28, 31 / 50, 47 / 62; 800 x 8 36 / 29, 58 / 61, 88 / 80; 512 x 16 38 / 30, 59 / 65, 90 / 86; 512 x 1 x 16000 53 / 61, 768 95 / 72.
+// 1, 2, 2 of up to two turns of 256 keys; and have 18 turns a CU or fewer, 32 of heads of 64.  us, few / many, E4M3, rows a key head x sequences x keys, 64 / 8 heads
+// of 128, around that bound: 256 x 8 x 2304, 2560, 2816 47 / 51, 50 / 54, 53 / 56 (18, 20 and 22 turns); 256 x 1 x 16384, 17408, 18432, 19456 (16 to 19) 40 /
+// 49, 62 / 50, 64 / 51, 66 / 51 (the five parts of more than 16384 keys are 1.25 rounds); 512 x 2 x 4096, 4608, 4864 34 / 48, 51 / 49, 52 / 51.  So at 17 and
+// 18 the rule is up to a quarter off for one long sequence, as it is in this table for 768 x 2 x 8000 of 64 (many is taken, 73 for 63), 128 x 16 x 1000 (few,
+// 33 for 30) and 384 x 8 x 300 of 64 (many, 17 for 15).  Of 128: 512 x 1 x 300, 1000, 3000, 6000, 16000 9 / 21, 14 / 37, 24 / 42, 32 / 45, 72 / 65; 1024 x 1 x
+// 3000 30 / 45; 256 x 1 x 16000 41 / 49, 60000 137 / 90; 128 x 16 x 300, 1000, 2000 22 / 18, 33 / 30, 45 / 49; 256 x 8 x 300, 1000, 2000 22 / 21, 32 / 42, 45 /
+// 52; 384 x 8 47 / 41, 65 / 66 of 1000, 2000; 80 x 16 x 8192 163 / 100; a quarter to all of 192 x 8 x up to 1000, 2000 21 / 28, 25 / 34; of 64: 512 x 4 x 300,
+// 1000, 3000 12 / 17, 18 / 34, 31 / 46; 384 x 8 x 300, 1000, 2000 16 / 18, 23 / 34, 33 / 58; 128 x 32 x 300, 1000 19 / 14, 31 / 24; 768 x 2 x 8000 58 / 73;
+// 1464 x 7 x 528, 16 / 2 heads, 19 / 26; 512 x 1 x 60000 133 / 115; 16 / 2 of 256, int8: 512 x 4 x 1000 21 / 43; 512 x 8 x 300, 1000, 2000 19 / 28, 31 / 50, 47
+// / 62; 800 x 8 36 / 29, 58 / 61, 88 / 80; 512 x 16 38 / 30, 59 / 65, 90 / 86; 512 x 1 x 16000 53 / 61, 768 95 / 72.
 // Few rows are 16, 32, or, where the keys are that many, up to 48 a workgroup and 64 of heads of 128: codes are converted once for all of them. 32
 // sequences of 8000 keys, 8 key heads of 128, us, 32 / 48 / 64 rows a workgroup: 32 rows 128 / 153 / 181, 48 226 / 156 / 183, 64 229 / 277 / 188; of 64:
 // 48 rows 114 / 85 / 135, 64 105 / 131 / 125; one sequence of 2000 keys, 48 rows 13.4 / 15.7 / 17.7.  (More than 64: 6 sequences of 7301, 154 rows of
@@ -128,10 +131,10 @@ static int launch_generic(const AttentionArgs& a, int sequences, hipStream_t str
 // us, two tiles a workgroup / one, 64 / 8 heads of 128: 6 tokens over 300 keys 10.8 / 8.4, 1000 14.2 / 11.6, 4000 16.1 / 13.6, 16000 21.6 / 22.2; 4 x 8
 // over 1000 17.5 / 15.7, over 4000 22.8 / 24.0; 16 x 3 over 1000 20.1 / 13.9; 16 x 6 over 300, 384 tiles, 11.2 / 15.0; of 64, 6 over 300 7.5 / 5.9,
 // 8 x 8 over 2000 15.5 / 12.2, 4000 21.7 / 20.7, 32 over 6000 17.9 / 19.9.  And parts are down to one turn
-// of eight waves, as many as one workgroup a CU leaves; whole up to 1024 keys of heads of 64, 768 of 128, 512 of 256.
-// us, whole / parts of 256, 512 keys, 64 / 8 heads of 128: 1 token over 600, 1000, 2000 keys 9.6 / 10.5, 12.2 / 10.7, 17.6 / 10.7; 4 x 6 tokens over 1000, 2000
-// 15.8 / 16.3, 21.4 / 26.8 / 17.9 (two groups of rows: 512 workgroups); 6 over 5000 39 / 25.4 / 16.8; of 64, 4 x 6 over 1000 10.9 / 13.1; 16 / 2 of 256, 2 over 600
-// 14.8 / 14.3.
+// of the workgroup's waves, as many as one workgroup a CU leaves; whole up to 1024 keys of heads of 64, 768 of 128, 512 of 256 (256 with 32 rows a workgroup,
+// whose turn is 128). us, whole / parts of 256, 512 keys, 64 / 8 heads of 128: 1 token over 600, 1000, 2000 keys 9.6 / 10.5, 12.2 / 10.7, 17.6 / 10.7; 4 x 6
+// tokens over 1000, 2000 15.8 / 16.3, 21.4 / 26.8 / 17.9 (two groups of rows: 512 workgroups); 6 over 5000 39 / 25.4 / 16.8; of 64, 4 x 6 over 1000 10.9 /
+// 13.1; 16 / 2 of 256, 2 over 600 14.8 / 14.3.
 // Of drafted tokens, where workgroups are more than CUs they are of the longer sequences first, so that the last to start are short ones; each finds its
 // sequence with the loads that it makes anyway.  us, as sequences come / longer first, E4M3, of any length up to the longest (of which most are short): 40 of
 // 4001 keys and 63 tokens, 16 / 16 heads of 64, 68 / 57 (50 / 38); 64 of 3000 and 8, 32 / 8 of 128, 53 / 44 (42 / 31); 48 of 2000 and 16, 16 / 16, 49 / 45

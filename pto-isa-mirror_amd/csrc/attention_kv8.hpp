@@ -52,8 +52,9 @@ constexpr int MANY_KEYS = 64;
 constexpr int many_start(int head_dim, int tile_rows) { return 448 / MANY_KEYS * (many_rows(head_dim) / tile_rows); }
 
 // The waves of a few-rows workgroup of so many tiles of 16 rows: eight where two fit a SIMD's registers (heads up to 128 elements, one tile), else four.
-// Of drafted tokens, four only of heads of 128 with three tiles or more: what the others' registers lack they leave in LDS.  us, four waves / eight: 32 x 4
-// tokens over 8192 keys, 64 / 8 heads of 128, 134 / 119; of 64, 16 x 4 48 / 37, 16 x 6 59 / 45, 40 x 30 ragged up to 4001 35 / 24; of 256, 48 x 2 57 / 50.
+// Of drafted tokens, four only of heads of 128 with three tiles or more and of 256 with two: what the others' registers lack they leave in LDS.  us, four waves
+// / eight: 32 x 4 tokens over 8192 keys, 64 / 8 heads of 128, 134 / 119; of 64, 16 x 4 48 / 37, 16 x 6 59 / 45, 40 x 30 ragged up to 4001 35 / 24; 16 / 2 of
+// 256, 48 x 2 over 4000 keys 41 / 41, over any number up to 4001 40 / 34.
 constexpr int few_waves(int head_dim, int row_tiles, bool tree = false)
 {
     return (head_dim <= 128 && row_tiles == 1) || (tree && (head_dim == 256 ? row_tiles == 1 : row_tiles == 2 || head_dim == 64)) ? 8 : 4;

@@ -66,7 +66,10 @@ __device__ __forceinline__ uint2 scaled_codes(uint2 w, float by)
 // codes a thread: 64 tokens of heads of 128): everything is read, then everything written, one chain list -> table -> scales and codes -> largest of each page.
 // Else pages that tokens move into one after the other: what a page takes is read before it is written, and what is written lies before all that is still to
 // be read.
-// Bound: the launch and that chain.  48 sequences, 16 heads of 64, up to 24 tokens over three pages of 16: 10.4 us page by page, 6.5 at once.
+// Bound: the launch and that chain.  48 sequences, 16 heads of 64, up to 24 tokens over three pages of 16: 10.4 us page by page, 6.5 at once.  On either side
+// of the bound, us, int8 / E4M3: 16 sequences, 8 heads of 128, pages of 64, 64 tokens of 64 4.4 / 4.4, 65 of 72 7.8 / 8.6; 48, 16 of 64, pages of 16, 64 of 200
+// 8.9 / 12.2, 65 17.9 / 24.6 (128 27.9 / 37.9: 2.5 / 3.3 a further page, the chain of each); 64, 8 of 256, pages of 64, 32 of 40 8.1 / 9.1, 33 10.2 / 11.4.
+// The longest lists, 64 x 200 of 256, 8 heads of 256, pages of 16: 66 / 94.
 template <int CODE>
 __global__ void __launch_bounds__(KEEP_THREADS) kvcache_keep_kernel(KeepArgs a)
 {

@@ -32,4 +32,24 @@ __device__ __forceinline__ uint2 kv8_codes(const float* x)
 template <int CODE>
 constexpr float KV8_PER_LARGEST = CODE == PTOAMD_I8 ? 1.0f / 127.0f : 1.0f / 448.0f;  // a page's scale over its largest magnitude
 
+// A page's scale once values have come into it whose largest magnitude has these bits.  (Bits, so that an infinity or a NaN among them is the largest.)
+template <int CODE>
+__device__ __forceinline__ float kv8_grown_scale(float old, uint32_t largest)
+{
+    float now = u2f(largest) * KV8_PER_LARGEST<CODE>;
+    now = old > now ? old : now;
+    now = now < 0x1p-126f ? 0.0f : now;
+    return largest >= 0x7F800000u || old != old ? NAN : now;
+}
+// Eight codes in a unit that is 1 / `by` of theirs.
+template <int CODE>
+__device__ __forceinline__ uint2 kv8_scaled_codes(uint2 w, float by)
+{
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        x[i] = kv8_value<CODE>(((i < 4 ? w.x : w.y) >> (8 * (i % 4))) & 0xFFu) * by;
+    return kv8_codes<CODE>(x);
+}
+
 }  // namespace ptoamd

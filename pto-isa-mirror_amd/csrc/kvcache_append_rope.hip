@@ -268,11 +268,7 @@ __global__ void __launch_bounds__(THREADS) kvcache_append_rope_kernel(AppendRope
 #pragma unroll
     for (int w = 0; w < THREADS / 64; ++w)
         largest = max(largest, wave_largest[w]);
-    float after = u2f(largest) * KV8_PER_LARGEST<CODE>;
-    after = before > after ? before : after;
-    after = after < 0x1p-126f ? 0.0f : after;
-    if (largest >= 0x7F800000u || before != before)
-        after = NAN;
+    const float after = kv8_grown_scale<CODE>(before, largest);
     if (threadIdx.x == 0)
         *scale = after;
     uint8_t* dst = side.codes + (int64_t)page * side.page + (int64_t)head * side.head;
@@ -281,12 +277,7 @@ __global__ void __launch_bounds__(THREADS) kvcache_append_rope_kernel(AppendRope
         const int chunks = c.head_dim / 8;
         for (int u = threadIdx.x; u < older * chunks; u += THREADS) {
             uint2* p = reinterpret_cast<uint2*>(dst + (int64_t)(u / chunks) * side.token + (u % chunks) * 8);
-            const uint2 w = *p;
-            float x[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-                x[i] = kv8_value<CODE>(((i < 4 ? w.x : w.y) >> (8 * (i % 4))) & 0xFFu) * ratio;
-            *p = kv8_codes<CODE>(x);
+            *p = kv8_scaled_codes<CODE>(*p, ratio);
         }
     }
     const float inverse = after > 0.0f ? 1.0f / after : 0.0f;

@@ -31,15 +31,6 @@ __device__ __forceinline__ uint32_t largest_of_group(uint32_t x, uint32_t* wave_
     return x;
 }
 
-// A page's scale once tokens have come into it whose largest magnitude has these bits.
-template <int CODE>
-__device__ __forceinline__ float grown_scale(float old, uint32_t largest)
-{
-    float now = u2f(largest) * KV8_PER_LARGEST<CODE>;
-    now = old > now ? old : now;
-    now = now < 0x1p-126f ? 0.0f : now;
-    return largest >= 0x7F800000u || old != old ? NAN : now;
-}
 // The largest magnitude among eight codes, in units of their scale.
 template <int CODE>
 __device__ __forceinline__ float largest_code(uint2 w)
@@ -53,13 +44,7 @@ __device__ __forceinline__ float largest_code(uint2 w)
 template <int CODE>
 __device__ __forceinline__ uint2 scaled_codes(uint2 w, float by)
 {
-    if (by == 1.0f)
-        return w;
-    float x[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        x[i] = kv8_value<CODE>(((i < 4 ? w.x : w.y) >> (8 * (i % 4))) & 0xFFu) * by;
-    return kv8_codes<CODE>(x);
+    return by == 1.0f ? w : kv8_scaled_codes<CODE>(w, by);
 }
 
 // One workgroup a sequence, head and side (keys or values).  Tokens only move down, in ascending order.  Lists of up to 64 entries that fit its registers (32
@@ -128,7 +113,7 @@ __global__ void __launch_bounds__(KEEP_THREADS) kvcache_keep_kernel(KeepArgs a)
         }
         __syncthreads();  // (every scale has been read, too)
         const uint32_t largest = comes[min(lane, BLOCKS - 1)];
-        const float block_now = largest != 0 ? grown_scale<CODE>(block_scale, largest - 1) : block_scale;
+        const float block_now = largest != 0 ? kv8_grown_scale<CODE>(block_scale, largest - 1) : block_scale;
         if (tid < blocks && block_page >= 0 && largest != 0)
             *scale_of_page(block_page) = block_now;
 #pragma unroll
@@ -195,7 +180,7 @@ __global__ void __launch_bounds__(KEEP_THREADS) kvcache_keep_kernel(KeepArgs a)
         largest = largest_of_group(largest, wave_largest);
         float now = old;
         if (__syncthreads_or(others)) {
-            now = grown_scale<CODE>(old, largest);
+            now = kv8_grown_scale<CODE>(old, largest);
             if (tid == 0)
                 *scale = now;
         }
